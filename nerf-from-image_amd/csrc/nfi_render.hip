@@ -1571,7 +1571,7 @@ __global__ void __launch_bounds__(256, (NPL <= 2 && SPL <= 2 && NOUT == NO) ? NF
         Ms[rc] = sc[e];
         Mi[rc] = i;
         Mt[rf] = vf;
-        Ms[rf] = sf[e];
+        lds_st(Ms + rf, sf[e]);   // (merged with the next store, its data was rewritten right behind it)
         Mi[rf] = S + i;
 #pragma unroll
         for (int k = 0; k < 3; ++k) {

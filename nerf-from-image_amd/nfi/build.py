@@ -5,14 +5,18 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(HERE), 'csrc')
 OUT = os.path.join(HERE, 'libnfi_hip.so')
 SOURCES = ['nfi_rays.hip', 'nfi_render.hip', 'nfi_producer.hip', 'nfi_conv.hip', 'nfi_gemm.hip', 'nfi_dconv.hip']
 HEADERS = ['nfi_common.h', 'nfi_host.h']
+# -packed-fp32-ops: no v_pk_add / mul / fma_f32 in the build.  Some of their forms have given wrong results
+# on this hardware now and then; measured cost on the renderer 1 % (p3d_car B = 8 step 5.85 -> 5.91 ms, within
+# two runs' spread), none on the inversion step.  (hipcc's host pass warns that it does not know the feature.)
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-shared', '-munsafe-fp-atomics',
-         '-Wall', '-Wno-unused-result']
+         '-Wall', '-Wno-unused-result', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 RENDER_SOURCES = ['nfi_rays.hip', 'nfi_render.hip', 'nfi_common.h', 'nfi_host.h']
@@ -81,10 +85,20 @@ def build(force: bool = False, verbose: bool = True, variant: str = '') -> str:
     extra = {'': [], 'stamps': ['-DNFI_STAMPS'], 'tilecheck': ['-DNFI_TILE_CHECK=1']}.get(variant)
     if extra is None:   # experiment builds: 'D<NAME>=<value>' -> -D<NAME>=<value>
         extra = ['-' + variant] if variant.startswith('D') else []
-    cmd = [hipcc] + FLAGS + extra + ['-o', out + '.tmp'] + [os.path.join(CSRC, s) for s in SOURCES]
-    if verbose:
-        print(' '.join(cmd), file=sys.stderr)
-    subprocess.run(cmd, check=True)
+    # one compiler process per source, all at once (a single command compiles them one after the other)
+    with tempfile.TemporaryDirectory() as tmp:
+        objs, jobs = [], []
+        for s in SOURCES:
+            objs.append(os.path.join(tmp, s.replace('.hip', '.o')))
+            cmd = [hipcc] + [f for f in FLAGS if f != '-shared'] + extra + ['-c', '-o', objs[-1], os.path.join(CSRC, s)]
+            if verbose:
+                print(' '.join(cmd), file=sys.stderr)
+            jobs.append((cmd, subprocess.Popen(cmd)))
+        codes = [(cmd, p.wait()) for cmd, p in jobs]
+        for cmd, rc in codes:
+            if rc:
+                raise subprocess.CalledProcessError(rc, cmd)
+        subprocess.run([hipcc, '--offload-arch=gfx950', '-fPIC', '-shared', '-o', out + '.tmp'] + objs, check=True)
     os.replace(out + '.tmp', out)
     return out
 
