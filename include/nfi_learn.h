@@ -1,0 +1,67 @@
+/*
+ * nfi learn C-ABI: the operators that train the field's mapper heads and the generator's weights.
+ *
+ *   residual norm     one pass over the rows of a residual stream: norm of a block's output, leaky
+ *                     ReLU, gate, shortcut, scale, and the next block's norm (the trunks of
+ *                     generator.py:132-253: LayerNorm, LeakyReLU 0.2, shortcut, sqrt(2)/2)
+ *   grouped product   y[r] = W[e] x[r] + b[e] for runs of rows e of uneven length (the rows of a batch
+ *                     that mixes several heads, each with its own stylegan.py:148-180 layer)
+ *   orthogonalised    an update brought to (nearly) orthogonal columns by Newton-Schulz products, with
+ *   update            its momentum and the weights' step
+ *
+ * Types: NFI_F32, NFI_BF16, NFI_F16; every sum, statistic and norm is held in 32 bits or more.
+ * `stream` is a hipStream_t; work buffers are the caller's, of the size the matching *_bytes entry
+ * gives, and hold nothing between calls.  Return NFI_OK (0) or a negative code (nfi_last_error()).
+ * The python-side mirrors are nerf-from-image_amd/nfi/norms.py, grouped.py and optim.py.
+ */
+#ifndef NFI_LEARN_H
+#define NFI_LEARN_H
+
+#include <stdint.h>
+
+#include "nfi.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define NFI_F32 0
+#define NFI_BF16 1
+#define NFI_F16 2
+
+#define NFI_NORM_NONE 0
+#define NFI_NORM_LAYER 1   /* (v - mean) / sqrt(var + eps) */
+#define NFI_NORM_RMS 2     /* v / sqrt(mean(v^2) + eps) */
+
+#define NFI_RESNORM_MAX_WIDTH 8192
+
+/* x = scale (residual + gate . lrelu(norm(h) . weight + bias, slope));  y = next_norm(x) . next_weight
+ * + next_bias, from the unrounded x.  h, residual, x, y and their gradients are [rows][width] of
+ * `dtype`, contiguous; weight, bias, next_weight, next_bias [width] of `param_dtype`; gate
+ * [gates][width] of `gate_dtype`, row r taking gate r / (rows / gates).  Absent (NULL): residual (0), gate,
+ * weight, next_weight (1), bias, next_bias (0).  y exists when next_norm is not NFI_NORM_NONE.  stats
+ * [rows][4] floats (mean and 1/deviation of both norms) are written when not NULL and read by the
+ * backward.  Backward: gx / gy may be NULL (zero gradients), and so may any output; dgate has gate's
+ * shape and type, the d weights and d biases `param_dtype`; all sums in a fixed order. */
+typedef struct nfi_resnorm_args {
+  const void *h, *residual, *gate, *weight, *bias, *next_weight, *next_bias;
+  void *x, *y;
+  float* stats;
+  const void *gx, *gy;
+  void *dh, *dresidual, *dgate, *dweight, *dbias, *dnext_weight, *dnext_bias;
+  float* work;          /* nfi_resnorm_work_bytes(rows, gates, width); backward only */
+  int64_t rows, gates;  /* gates: 0 without a gate; divides rows */
+  int32_t width, dtype, gate_dtype, param_dtype, norm, next_norm;
+  float slope, scale, eps;
+  int32_t _pad;
+} nfi_resnorm_args;
+
+int64_t nfi_resnorm_work_bytes(int64_t rows, int64_t gates, int32_t width);
+int32_t nfi_resnorm_forward(const nfi_resnorm_args* a, void* stream);
+int32_t nfi_resnorm_backward(const nfi_resnorm_args* a, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* NFI_LEARN_H */

@@ -12,7 +12,7 @@ import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('NFI_LIBRARY') or os.path.join(_HERE, 'libnfi_hip.so')
-ABI_VERSION = 18
+ABI_VERSION = 19
 DEC_SIZE = 7200
 DEC_SIZE_VIEWDIR = 14384
 
@@ -55,6 +55,16 @@ class NfiRenderGradArgs(ctypes.Structure):
                 ('d_palette_ray', c_void_p), ('g_ro', c_void_p), ('g_rd', c_void_p),
                 ('tile_counts', c_void_p), ('workspace', c_void_p), ('workspace_bytes', ctypes.c_int64),
                 ('d_xray', c_void_p)]
+
+
+class NfiResnormArgs(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ('h', 'residual', 'gate', 'weight', 'bias', 'next_weight', 'next_bias', 'x', 'y',
+                                        'stats', 'gx', 'gy', 'dh', 'dresidual', 'dgate', 'dweight', 'dbias',
+                                        'dnext_weight', 'dnext_bias', 'work')] + [
+        ('rows', ctypes.c_int64), ('gates', ctypes.c_int64), ('width', ctypes.c_int32), ('dtype', ctypes.c_int32),
+        ('gate_dtype', ctypes.c_int32), ('param_dtype', ctypes.c_int32), ('norm', ctypes.c_int32),
+        ('next_norm', ctypes.c_int32), ('slope', ctypes.c_float), ('scale', ctypes.c_float), ('eps', ctypes.c_float),
+        ('_pad', ctypes.c_int32)]
 
 
 # symbol -> (restype, argtypes); every entry point of include/nfi.h
@@ -201,6 +211,10 @@ SIGNATURES = {
                                         c_void_p]),
     'nfi_dconv3x3': (ctypes.c_int32, [c_void_p] * 10 + [ctypes.c_int32] * 5 + [c_void_p]),
     'nfi_absmax_scaled_slots': (ctypes.c_int32, [c_void_p, c_void_p] + [ctypes.c_int32] * 3 + [c_void_p, c_void_p]),
+    # include/nfi_learn.h
+    'nfi_resnorm_work_bytes': (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32]),
+    'nfi_resnorm_forward': (ctypes.c_int32, [ctypes.POINTER(NfiResnormArgs), c_void_p]),
+    'nfi_resnorm_backward': (ctypes.c_int32, [ctypes.POINTER(NfiResnormArgs), c_void_p]),
 }
 
 _lib = None

@@ -10,8 +10,9 @@ import tempfile
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(HERE), 'csrc')
 OUT = os.path.join(HERE, 'libnfi_hip.so')
-SOURCES = ['nfi_rays.hip', 'nfi_render.hip', 'nfi_producer.hip', 'nfi_conv.hip', 'nfi_gemm.hip', 'nfi_dconv.hip']
-HEADERS = ['nfi_common.h', 'nfi_host.h']
+SOURCES = ['nfi_rays.hip', 'nfi_render.hip', 'nfi_producer.hip', 'nfi_conv.hip', 'nfi_gemm.hip', 'nfi_dconv.hip',
+           'nfi_norms.hip']
+HEADERS = ['nfi_common.h', 'nfi_host.h', 'nfi_learn.h']
 # -packed-fp32-ops: no v_pk_add / mul / fma_f32 in the build.  Some of their forms have given wrong results
 # on this hardware now and then; measured cost on the renderer 1 % (p3d_car B = 8 step 5.85 -> 5.91 ms, within
 # two runs' spread), none on the inversion step.  (hipcc's host pass warns that it does not know the feature.)
@@ -42,7 +43,7 @@ def _stale() -> bool:
     t = os.path.getmtime(OUT)
     deps = [os.path.join(CSRC, s) for s in SOURCES + HEADERS]
     inc = os.path.join(os.path.dirname(os.path.dirname(HERE)), 'include')
-    deps += [os.path.join(inc, h) for h in ('nfi.h', 'nfi_producer.h')]
+    deps += [os.path.join(inc, h) for h in ('nfi.h', 'nfi_producer.h', 'nfi_learn.h')]
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 

@@ -1,0 +1,69 @@
+"""CPU: what the operators of include/nfi_learn.h refuse before anything is launched, and the layout of their
+argument structs."""
+
+import ctypes
+import os
+import subprocess
+
+import pytest
+import torch
+
+from nfi import _lib, norms
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.mark.parametrize('name,struct', [('nfi_resnorm_args', 'NfiResnormArgs')])
+def test_struct_layout(tmp_path, name, struct):
+    py = getattr(_lib, struct)
+    fields = [f[0] for f in py._fields_]
+    header = os.path.join(ROOT, 'include', 'nfi_learn.h')
+    src = ['#include <stdio.h>', '#include <stddef.h>', f'#include "{header}"', 'int main(void){',
+           f'printf("%zu\\n", sizeof({name}));'] + [f'printf("%zu\\n", offsetof({name}, {f}));' for f in fields] + ['return 0;}']
+    (tmp_path / 'p.c').write_text('\n'.join(src))
+    subprocess.run(['gcc', '-o', str(tmp_path / 'p'), str(tmp_path / 'p.c')], check=True)
+    vals = [int(v) for v in subprocess.run([str(tmp_path / 'p')], check=True, capture_output=True, text=True).stdout.split()]
+    assert vals == [ctypes.sizeof(py)] + [getattr(py, f).offset for f in fields]
+
+
+def test_residual_norm_refuses_cpu_tensors():
+    with pytest.raises(RuntimeError, match='HIP devices only'):
+        norms.residual_norm(torch.zeros(2, 4))
+
+
+def test_resnorm_entry_refuses_bad_arguments():
+    lib = _lib.load()
+    one = ctypes.c_void_p(16)
+
+    def args(**kw):
+        a = _lib.NfiResnormArgs()
+        a.h = a.x = one
+        a.rows, a.width, a.norm, a.eps = 4, 8, 1, 1e-5
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return a
+
+    for kw, word in (({'h': None}, b'null input'), ({'rows': 0}, b'rows'), ({'width': 8193}, b'width'),
+                     ({'dtype': 7}, b'type'), ({'norm': 3}, b'norm'), ({'next_norm': -1}, b'norm'),
+                     ({'gate': one, 'gates': 3}, b'gates'), ({'gates': 2}, b'gates'), ({'eps': -1.0}, b'eps'),
+                     ({'x': None}, b'null output'), ({'next_norm': 1}, b'null output')):
+        assert lib.nfi_resnorm_forward(ctypes.byref(args(**kw)), None) == -1, kw
+        assert word in lib.nfi_last_error(), (kw, lib.nfi_last_error())
+    for kw, word in (({}, b'statistics'), ({'stats': one, 'work': one}, b'no gradient'),
+                     ({'stats': one, 'work': one, 'gy': one}, b'next norm')):
+        assert lib.nfi_resnorm_backward(ctypes.byref(args(**kw)), None) == -1, kw
+        assert word in lib.nfi_last_error(), kw
+
+
+@pytest.mark.parametrize('rows,gates', [(1, 0), (1, 1), (7, 7), (10 ** 6, 0), (10 ** 6, 2), (4096, 512), (4096, 2048), (511 * 3, 511)])
+def test_resnorm_work_holds_every_workgroup(rows, gates):
+    """The plan's workgroups (restated) fit the work buffer for every number of rows a workgroup may hold."""
+    lib = _lib.load()
+    for slots in (1, 4, 8, 16, 32):
+        g = gates if 0 < gates < rows else 1
+        per_gate = rows // g
+        splits = min(max(1, 512 // g), -(-per_gate // slots))
+        segments = g * splits
+        per = 1 if splits > 1 else -(-segments // 512)
+        blocks = -(-segments // per)
+        assert lib.nfi_resnorm_work_bytes(rows, gates, 24) >= blocks * 5 * 24 * 4
