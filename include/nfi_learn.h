@@ -60,6 +60,29 @@ int64_t nfi_resnorm_work_bytes(int64_t rows, int64_t gates, int32_t width);
 int32_t nfi_resnorm_forward(const nfi_resnorm_args* a, void* stream);
 int32_t nfi_resnorm_backward(const nfi_resnorm_args* a, void* stream);
 
+#define NFI_GROUPED_MAX_GROUPS 65535
+#define NFI_GROUPED_MAX_WIDTH 2097152
+
+/* y[r] = w[e] x[r] + bias[e] for off[e] <= r < off[e+1]; rows that no group holds give zeros (y and gx).
+ * x [rows][in_width], w [groups][out_width][in_width], bias [groups][out_width] (may be NULL), y and gy
+ * [rows][out_width], gx and gw like x and w, gb like bias: all of `dtype`, contiguous.  offsets
+ * [groups + 1] on the device, 32-bit, or 64-bit with offsets64: not decreasing; values outside [0, rows]
+ * count as the nearest of its ends.  gx, gw, gb may be NULL.  An empty group's gw and gb are zeros; sums run in a
+ * fixed order.  work: the matching *_work_bytes (of the same arguments), or NULL where that is 0. */
+typedef struct nfi_grouped_args {
+  const void *x, *w, *bias, *offsets;
+  void* y;
+  const void* gy;
+  void *gx, *gw, *gb, *work;
+  int64_t work_bytes, rows;
+  int32_t groups, in_width, out_width, dtype, offsets64, _pad;
+} nfi_grouped_args;
+
+int64_t nfi_grouped_forward_work_bytes(const nfi_grouped_args* a);
+int64_t nfi_grouped_backward_work_bytes(const nfi_grouped_args* a);
+int32_t nfi_grouped_forward(const nfi_grouped_args* a, void* stream);
+int32_t nfi_grouped_backward(const nfi_grouped_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,392 @@
+// Products grouped by ragged runs of rows (include/nfi_learn.h nfi_grouped_*): rows off[e] .. off[e+1] of x
+// [T][K] meet w[e] [N][K]
+//
+//   y[r] = w[e] x[r] + b[e]      d x[r] = w[e]^T dy[r]      d w[e] = sum_r dy[r] x[r]^T      d b[e] = sum_r dy[r]
+//
+// 2 T K N operations each way and product; the offsets stay on the device: a launch covers every tile that
+// any division into groups could need, and a workgroup finds its group by a scan of the tile counts.
+#include <algorithm>
+
+#include "nfi_mm.h"
+
+namespace nfi {
+namespace learn {
+
+struct GroupedArgs {
+  const unsigned char *a, *b;      // operands of the product (see the kernels)
+  const void *offsets, *bias;
+  void* out;
+  float* part;                     // partial results where the rows of a group are split
+  int64_t rows;
+  int groups, n, k;                // the product's columns (of out) and contracted length
+  unsigned lda, ldb;               // bytes between rows
+  int64_t sb;                      // bytes between w's matrices
+  int offsets64, splits, col_tiles;
+};
+
+__device__ __forceinline__ int64_t offset_at(const void* p, int is64, int e, int64_t rows) {
+  const int64_t v = is64 ? ((const int64_t*)p)[e] : (int64_t)((const int32_t*)p)[e];
+  return v < 0 ? 0 : (v > rows ? rows : v);
+}
+
+// Row tile `tile` over the groups' tiles one after the other, then those of the rows that no group holds.
+// Returns the group (groups: rows of none; -1: past the end) and its rows [r0, r1).
+__device__ __forceinline__ int find_tile(const GroupedArgs& p, int64_t tile, int64_t& r0, int64_t& r1) {
+  const int l = lane_id();
+  int64_t before = 0;
+  const int64_t head = offset_at(p.offsets, p.offsets64, 0, p.rows), tail = offset_at(p.offsets, p.offsets64, p.groups, p.rows);
+  for (int e0 = 0; e0 < p.groups + 2; e0 += 64) {
+    // two runs of no group follow the last: the rows before the first group and behind the last
+    const int e = e0 + l;
+    int64_t s = 0, t = 0;
+    if (e < p.groups) {
+      s = offset_at(p.offsets, p.offsets64, e, p.rows);
+      t = offset_at(p.offsets, p.offsets64, e + 1, p.rows);
+    } else if (e == p.groups) {
+      t = head;
+    } else if (e == p.groups + 1) {
+      s = tail;
+      t = p.rows;
+    }
+    const int mine = t > s ? (int)((t - s + TILE - 1) / TILE) : 0;
+    int incl = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int v = __shfl_up(incl, d);
+      if (l >= d) incl += v;
+    }
+    const int64_t at = tile - before - (incl - mine);   // this lane's tile, if it is one of its own
+    const unsigned long long hit = __ballot(at >= 0 && at < mine);
+    if (hit) {
+      const int src = __builtin_ctzll(hit);
+      const int64_t first = s + at * TILE, last = min(first + TILE, t);
+      r0 = __shfl((int)(first & 0xffffffff), src) & 0xffffffffll;
+      r0 |= (int64_t)__shfl((int)(first >> 32), src) << 32;
+      r1 = r0 + __shfl((int)(last - first), src);
+      return min(e0 + src, p.groups);
+    }
+    before += __shfl(incl, 63);
+  }
+  return -1;
+}
+
+template <class T>
+__device__ __forceinline__ void store4(T* p, const float (&v)[4], int count) {
+  if (count >= 4) {
+    store_piece<T, 4>(p, v);
+  } else {
+    for (int r = 0; r < count; ++r) p[r] = (T)v[r];
+  }
+}
+
+// y (SLAB_B false: b = w[e], rows of K) and d x (SLAB_B true: a = dy, b = w[e] as slabs): rows of `a` by tiles
+template <class T, bool SLAB_B>
+__global__ void __launch_bounds__(256) grouped_rows(const GroupedArgs p) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * TILE_BYTES];
+  const int64_t tile = blockIdx.x / p.col_tiles;
+  const int c0 = (int)(blockIdx.x % p.col_tiles) * TILE;
+  int64_t r0, r1;
+  const int e = find_tile(p, tile, r0, r1);
+  if (e < 0) return;
+  const int rows = (int)(r1 - r0), cols = min(TILE, p.n - c0);
+  f4v acc[4][4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) acc[x][y] = f4v{0.f, 0.f, 0.f, 0.f};
+  if (e < p.groups) {
+    const unsigned char* b = p.b + e * p.sb + (SLAB_B ? (int64_t)c0 * (int)sizeof(T) : (int64_t)c0 * p.ldb);
+    tile_product<T, false, SLAB_B>(p.a + r0 * p.lda, p.lda, rows, b, p.ldb, cols, p.k, lds, acc);
+  }
+  const int wave = threadIdx.x >> 6, i = lane_id() & 15, g = lane_id() >> 4;
+#pragma unroll
+  for (int y = 0; y < 4; ++y) {
+    const int n = (wave >> 1) * 64 + y * 16 + 4 * g;
+    float bias[4] = {0.f, 0.f, 0.f, 0.f};
+    if (p.bias && e < p.groups)
+      for (int r = 0; r < 4; ++r)
+        if (n + r < cols) bias[r] = (float)((const T*)p.bias)[(int64_t)e * p.n + c0 + n + r];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int row = (wave & 1) * 64 + x * 16 + i;
+      float v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = acc[x][y][r] + bias[r];
+      if (row < rows) store4<T>((T*)p.out + (r0 + row) * p.n + c0 + n, v, cols - n);
+    }
+  }
+}
+
+// d w[e] [N][K]: a = dy as slabs (its columns are the lines), b = x as slabs; blockIdx.y the group, .z the split
+template <class T>
+__global__ void __launch_bounds__(256) grouped_weights(const GroupedArgs p, int n_rows) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * TILE_BYTES];
+  const int e = blockIdx.y;
+  const int m0 = (int)(blockIdx.x / p.col_tiles) * TILE, c0 = (int)(blockIdx.x % p.col_tiles) * TILE;
+  const int64_t s = offset_at(p.offsets, p.offsets64, e, p.rows), t = max(s, offset_at(p.offsets, p.offsets64, e + 1, p.rows));
+  // pieces of whole steps
+  constexpr int KSTEP = STEP_BYTES / sizeof(T);
+  const int64_t piece = ((t - s + p.splits - 1) / p.splits + KSTEP - 1) / KSTEP * KSTEP;
+  const int64_t r0 = min(t, s + blockIdx.z * piece), r1 = min(t, r0 + piece);
+  const int lines = min(TILE, n_rows - m0), cols = min(TILE, p.n - c0);
+  f4v acc[4][4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) acc[x][y] = f4v{0.f, 0.f, 0.f, 0.f};
+  tile_product<T, true, true>(p.a + r0 * p.lda + m0 * (int64_t)sizeof(T), p.lda, lines, p.b + r0 * p.ldb + c0 * (int64_t)sizeof(T),
+                              p.ldb, cols, r1 - r0, lds, acc);
+  const int wave = threadIdx.x >> 6, i = lane_id() & 15, g = lane_id() >> 4;
+  const int64_t matrix = (int64_t)n_rows * p.n;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const int row = (wave & 1) * 64 + x * 16 + i;
+    if (row >= lines) continue;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int n = (wave >> 1) * 64 + y * 16 + 4 * g;
+      const float v[4] = {acc[x][y][0], acc[x][y][1], acc[x][y][2], acc[x][y][3]};
+      const int64_t at = (int64_t)(m0 + row) * p.n + c0 + n;
+      if (p.splits == 1) store4<T>((T*)p.out + e * matrix + at, v, cols - n);
+      else store4<float>(p.part + ((int64_t)blockIdx.z * p.groups + e) * matrix + at, v, cols - n);
+    }
+  }
+}
+
+// d b[e]: 64 columns x 4 rows at a time; blockIdx.y the group, .z the split
+template <class T>
+__global__ void __launch_bounds__(256) grouped_bias(const GroupedArgs p) {
+  __shared__ float lds[4][64];
+  const int e = blockIdx.y, col = blockIdx.x * 64 + (threadIdx.x & 63), slot = threadIdx.x >> 6;
+  const int64_t s = offset_at(p.offsets, p.offsets64, e, p.rows), t = max(s, offset_at(p.offsets, p.offsets64, e + 1, p.rows));
+  const int64_t piece = (t - s + p.splits - 1) / p.splits;
+  const int64_t r0 = min(t, s + blockIdx.z * piece), r1 = min(t, r0 + piece);
+  float v = 0.f;
+  if (col < p.n) {
+#pragma unroll 4
+    for (int64_t r = r0 + slot; r < r1; r += 4) v += (float)((const T*)p.a)[r * p.n + col];
+  }
+  lds[slot][threadIdx.x & 63] = v;
+  __syncthreads();
+  if (slot == 0 && col < p.n) {
+    v = (lds[0][threadIdx.x] + lds[1][threadIdx.x]) + (lds[2][threadIdx.x] + lds[3][threadIdx.x]);
+    if (p.splits == 1) ((T*)p.out)[(int64_t)e * p.n + col] = (T)v;
+    else p.part[((int64_t)blockIdx.z * p.groups + e) * p.n + col] = v;
+  }
+}
+
+// partial results summed in their order and rounded once
+template <class T>
+__global__ void __launch_bounds__(256) join_parts(const float* __restrict__ part, T* __restrict__ out, int64_t count, int splits) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= count) return;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  const int have = (int)(count - i < 4 ? count - i : 4);
+  for (int s = 0; s < splits; ++s) {
+    const float* q = part + s * count + i;
+    if (have == 4) {
+      float u[4];
+      load_piece<float, 4>(q, u);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] += u[r];
+    } else {
+      for (int r = 0; r < have; ++r) v[r] += q[r];
+    }
+  }
+  store4<T>(out + i, v, have);
+}
+
+// rows of `width` elements to rows of `padded`, zeros behind: a matrix whose rows are not aligned to 16 bytes
+template <class T>
+__global__ void __launch_bounds__(256) pad_rows(const T* __restrict__ src, T* __restrict__ dst, int64_t rows, int width, int padded) {
+  constexpr int V = 16 / sizeof(T);
+  const int per = padded / V;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= rows * per) return;
+  const int64_t row = id / per;
+  const int col = (int)(id - row * per) * V;
+  T v[V];
+  if (col + V <= width) {
+    __builtin_memcpy(v, src + row * width + col, 16);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = col + j < width ? src[row * width + col + j] : (T)0.f;
+  }
+  __builtin_memcpy(dst + row * padded + col, v, 16);
+}
+
+static inline int padded_width(int width, int es) { return (width * es + 15) / 16 * 16 / es; }
+static inline bool rows_aligned(const void* p, int width, int es) { return ((uintptr_t)p & 15) == 0 && width * es % 16 == 0; }
+static inline int64_t up(int64_t v) { return (v + 255) / 256 * 256; }
+
+// The rows of a group are divided where the tiles alone are too few for 256 compute units with two workgroups
+// each; a piece keeps at least 256 rows of an average group
+static int weight_splits(int64_t rows, int groups, int n, int k) {
+  const int64_t tiles = (int64_t)groups * ((n + TILE - 1) / TILE) * ((k + TILE - 1) / TILE);
+  const int64_t want = 1024 / std::max<int64_t>(1, tiles), most = rows / groups / 256;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 64));
+}
+static int bias_splits(int64_t rows, int groups, int n) {
+  const int64_t tiles = (int64_t)groups * ((n + 63) / 64);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(1024 / tiles, rows / groups / 32), 64));
+}
+
+template <class T>
+static const unsigned char* padded(const void* src, int64_t rows, int width, unsigned char*& work, unsigned& ld, hipStream_t s) {
+  const int es = sizeof(T), pw = padded_width(width, es);
+  ld = (unsigned)pw * es;
+  if (rows_aligned(src, width, es)) return (const unsigned char*)src;
+  T* dst = (T*)work;
+  work += up(rows * (int64_t)ld);
+  const int64_t pieces = rows * (pw / (16 / es));
+  pad_rows<T><<<(unsigned)((pieces + 255) / 256), 256, 0, s>>>((const T*)src, dst, rows, width, pw);
+  return (const unsigned char*)dst;
+}
+
+template <class T>
+static void forward(const nfi_grouped_args& a, hipStream_t s) {
+  unsigned char* work = (unsigned char*)a.work;
+  GroupedArgs p = {};
+  p.a = padded<T>(a.x, a.rows, a.in_width, work, p.lda, s);
+  p.b = padded<T>(a.w, (int64_t)a.groups * a.out_width, a.in_width, work, p.ldb, s);
+  p.sb = (int64_t)p.ldb * a.out_width;
+  p.offsets = a.offsets;
+  p.offsets64 = a.offsets64;
+  p.bias = a.bias;
+  p.out = a.y;
+  p.rows = a.rows;
+  p.groups = a.groups;
+  p.n = a.out_width;
+  p.k = a.in_width;
+  p.col_tiles = (a.out_width + TILE - 1) / TILE;
+  const int64_t tiles = ((a.rows + TILE - 1) / TILE + std::min<int64_t>(a.groups + 2, a.rows)) * p.col_tiles;
+  grouped_rows<T, false><<<(unsigned)tiles, 256, 0, s>>>(p);
+}
+
+template <class T>
+static void backward(const nfi_grouped_args& a, hipStream_t s) {
+  unsigned char* work = (unsigned char*)a.work;
+  GroupedArgs p = {};
+  p.offsets = a.offsets;
+  p.offsets64 = a.offsets64;
+  p.rows = a.rows;
+  p.groups = a.groups;
+  unsigned ldg = 0;
+  const unsigned char* g = a.gx || a.gw ? padded<T>(a.gy, a.rows, a.out_width, work, ldg, s) : nullptr;
+  if (a.gx) {
+    p.a = g;
+    p.lda = ldg;
+    p.b = padded<T>(a.w, (int64_t)a.groups * a.out_width, a.in_width, work, p.ldb, s);
+    p.sb = (int64_t)p.ldb * a.out_width;
+    p.out = a.gx;
+    p.n = a.in_width;
+    p.k = a.out_width;
+    p.col_tiles = (a.in_width + TILE - 1) / TILE;
+    const int64_t tiles = ((a.rows + TILE - 1) / TILE + std::min<int64_t>(a.groups + 2, a.rows)) * p.col_tiles;
+    grouped_rows<T, true><<<(unsigned)tiles, 256, 0, s>>>(p);
+  }
+  if (a.gw) {
+    p.a = g;
+    p.lda = ldg;
+    p.b = padded<T>(a.x, a.rows, a.in_width, work, p.ldb, s);
+    p.out = a.gw;
+    p.n = a.in_width;
+    p.col_tiles = (a.in_width + TILE - 1) / TILE;
+    p.splits = weight_splits(a.rows, a.groups, a.out_width, a.in_width);
+    p.part = (float*)work;
+    const int64_t count = (int64_t)a.groups * a.out_width * a.in_width;
+    if (p.splits > 1) work += up(count * 4 * p.splits);
+    grouped_weights<T><<<dim3((unsigned)((a.out_width + TILE - 1) / TILE * p.col_tiles), (unsigned)a.groups, (unsigned)p.splits), 256, 0, s>>>(
+        p, a.out_width);
+    if (p.splits > 1) join_parts<T><<<(unsigned)((count + 1023) / 1024), 256, 0, s>>>(p.part, (T*)a.gw, count, p.splits);
+  }
+  if (a.gb) {
+    p.a = (const unsigned char*)a.gy;
+    p.out = a.gb;
+    p.n = a.out_width;
+    p.splits = bias_splits(a.rows, a.groups, a.out_width);
+    p.part = (float*)work;
+    const int64_t count = (int64_t)a.groups * a.out_width;
+    grouped_bias<T><<<dim3((unsigned)((a.out_width + 63) / 64), (unsigned)a.groups, (unsigned)p.splits), 256, 0, s>>>(p);
+    if (p.splits > 1) join_parts<T><<<(unsigned)((count + 1023) / 1024), 256, 0, s>>>(p.part, (T*)a.gb, count, p.splits);
+  }
+}
+
+static int check(const nfi_grouped_args* a, const char* what) {
+  NFI_REQUIRE(a && a->offsets, "%s: null input", what);
+  NFI_REQUIRE(type_ok(a->dtype), "%s: bad type", what);
+  NFI_REQUIRE(a->rows > 0 && a->rows < (1ll << 31), "%s: %lld rows", what, (long long)a->rows);
+  NFI_REQUIRE(a->groups > 0 && a->groups <= NFI_GROUPED_MAX_GROUPS, "%s: %d groups (1 .. %d)", what, a->groups, NFI_GROUPED_MAX_GROUPS);
+  // (a tile's offsets are 32-bit: 128 rows of at most 8 MB)
+  NFI_REQUIRE(a->in_width > 0 && a->in_width <= NFI_GROUPED_MAX_WIDTH && a->out_width > 0 && a->out_width <= NFI_GROUPED_MAX_WIDTH,
+              "%s: widths %d -> %d (1 .. %d)", what, a->in_width, a->out_width, NFI_GROUPED_MAX_WIDTH);
+  const int64_t widest = std::max(a->in_width, a->out_width);
+  NFI_REQUIRE(((a->rows + TILE - 1) / TILE + a->groups + 2) * ((widest + TILE - 1) / TILE) < (1ll << 31), "%s: too many tiles", what);
+  return NFI_OK;
+}
+
+// (a matrix of whatever alignment may be padded: room is kept where its rows are not of whole pieces, or its address
+// may not be)
+static int64_t pad_bytes(const void* p, int64_t rows, int width, int es) {
+  return rows_aligned(p, width, es) ? 0 : up(rows * (int64_t)padded_width(width, es) * es);
+}
+
+}  // namespace learn
+}  // namespace nfi
+
+using namespace nfi::learn;
+
+extern "C" {
+
+int64_t nfi_grouped_forward_work_bytes(const nfi_grouped_args* a) {
+  if (check(a, "grouped_forward") != NFI_OK) return -1;
+  const int es = type_bytes(a->dtype);
+  return pad_bytes(a->x, a->rows, a->in_width, es) + pad_bytes(a->w, (int64_t)a->groups * a->out_width, a->in_width, es);
+}
+
+int64_t nfi_grouped_backward_work_bytes(const nfi_grouped_args* a) {
+  if (check(a, "grouped_backward") != NFI_OK) return -1;
+  const int es = type_bytes(a->dtype);
+  int64_t n = 0;
+  if (a->gx || a->gw) n += pad_bytes(a->gy, a->rows, a->out_width, es);
+  if (a->gx) n += pad_bytes(a->w, (int64_t)a->groups * a->out_width, a->in_width, es);
+  if (a->gw) {
+    n += pad_bytes(a->x, a->rows, a->in_width, es);
+    const int s = weight_splits(a->rows, a->groups, a->out_width, a->in_width);
+    if (s > 1) n += up((int64_t)a->groups * a->out_width * a->in_width * 4 * s);
+  }
+  if (a->gb) n += up((int64_t)a->groups * a->out_width * 4 * bias_splits(a->rows, a->groups, a->out_width));
+  return n;
+}
+
+int32_t nfi_grouped_forward(const nfi_grouped_args* a, void* stream) {
+  const int e = check(a, "grouped_forward");
+  if (e) return e;
+  NFI_REQUIRE(a->x && a->w && a->y, "grouped_forward: null tensor");
+  const int64_t need = nfi_grouped_forward_work_bytes(a);
+  NFI_REQUIRE(a->work_bytes >= need && (need == 0 || a->work), "grouped_forward: %lld bytes of work, %lld wanted", (long long)a->work_bytes,
+              (long long)need);
+  hipStream_t s = (hipStream_t)stream;
+  if (a->dtype == NFI_F32) forward<float>(*a, s);
+  else if (a->dtype == NFI_BF16) forward<bf16_t>(*a, s);
+  else forward<f16_t>(*a, s);
+  NFI_CHECK_LAUNCH("grouped_forward");
+  return NFI_OK;
+}
+
+int32_t nfi_grouped_backward(const nfi_grouped_args* a, void* stream) {
+  const int e = check(a, "grouped_backward");
+  if (e) return e;
+  NFI_REQUIRE(a->gy && (!a->gx || a->w) && (!a->gw || a->x), "grouped_backward: null tensor");
+  const int64_t need = nfi_grouped_backward_work_bytes(a);
+  NFI_REQUIRE(a->work_bytes >= need && (need == 0 || a->work), "grouped_backward: %lld bytes of work, %lld wanted", (long long)a->work_bytes,
+              (long long)need);
+  hipStream_t s = (hipStream_t)stream;
+  if (a->dtype == NFI_F32) backward<float>(*a, s);
+  else if (a->dtype == NFI_BF16) backward<bf16_t>(*a, s);
+  else backward<f16_t>(*a, s);
+  NFI_CHECK_LAUNCH("grouped_backward");
+  return NFI_OK;
+}
+
+}  // extern "C"

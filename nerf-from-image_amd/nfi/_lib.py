@@ -67,6 +67,12 @@ class NfiResnormArgs(ctypes.Structure):
         ('_pad', ctypes.c_int32)]
 
 
+class NfiGroupedArgs(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ('x', 'w', 'bias', 'offsets', 'y', 'gy', 'gx', 'gw', 'gb', 'work')] + [
+        ('work_bytes', ctypes.c_int64), ('rows', ctypes.c_int64), ('groups', ctypes.c_int32), ('in_width', ctypes.c_int32),
+        ('out_width', ctypes.c_int32), ('dtype', ctypes.c_int32), ('offsets64', ctypes.c_int32), ('_pad', ctypes.c_int32)]
+
+
 # symbol -> (restype, argtypes); every entry point of include/nfi.h
 SIGNATURES = {
     'nfi_abi_version': (ctypes.c_int32, []),
@@ -215,6 +221,10 @@ SIGNATURES = {
     'nfi_resnorm_work_bytes': (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32]),
     'nfi_resnorm_forward': (ctypes.c_int32, [ctypes.POINTER(NfiResnormArgs), c_void_p]),
     'nfi_resnorm_backward': (ctypes.c_int32, [ctypes.POINTER(NfiResnormArgs), c_void_p]),
+    'nfi_grouped_forward_work_bytes': (ctypes.c_int64, [ctypes.POINTER(NfiGroupedArgs)]),
+    'nfi_grouped_backward_work_bytes': (ctypes.c_int64, [ctypes.POINTER(NfiGroupedArgs)]),
+    'nfi_grouped_forward': (ctypes.c_int32, [ctypes.POINTER(NfiGroupedArgs), c_void_p]),
+    'nfi_grouped_backward': (ctypes.c_int32, [ctypes.POINTER(NfiGroupedArgs), c_void_p]),
 }
 
 _lib = None

@@ -29,6 +29,22 @@ def stream(dev):
     return _stream(dev)
 
 
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on(dev):
+    """A context with `dev` as the current device (a launch goes to the current device's streams)."""
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
 def type_code(t, what):
     code = TYPES.get(t.dtype)
     if code is None:

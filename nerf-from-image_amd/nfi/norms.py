@@ -47,7 +47,7 @@ class _ResidualNorm(torch.autograd.Function):
         stats = torch.empty((h.shape[0], 4), device=h.device, dtype=torch.float32) if train else None
         a.x, a.y, a.stats = lo.ptr(x), lo.ptr(y), lo.ptr(stats)
         if h.shape[0]:
-            with torch.cuda.device(h.device):
+            with lo.on(h.device):
                 lo.call('nfi_resnorm_forward', ctypes.byref(a), lo.stream(h.device))
         ctx.conf = conf
         ctx.set_materialize_grads(False)
@@ -77,7 +77,7 @@ class _ResidualNorm(torch.autograd.Function):
         size = _lib.load().nfi_resnorm_work_bytes(a.rows, a.gates, a.width)
         work = torch.empty((size,), device=h.device, dtype=torch.uint8)
         a.work = lo.ptr(work)
-        with torch.cuda.device(h.device):
+        with lo.on(h.device):
             lo.call('nfi_resnorm_backward', ctypes.byref(a), lo.stream(h.device))
         return tuple(out) + (None,)
 

@@ -8,12 +8,12 @@ import subprocess
 import pytest
 import torch
 
-from nfi import _lib, norms
+from nfi import _lib, grouped, norms
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
-@pytest.mark.parametrize('name,struct', [('nfi_resnorm_args', 'NfiResnormArgs')])
+@pytest.mark.parametrize('name,struct', [('nfi_resnorm_args', 'NfiResnormArgs'), ('nfi_grouped_args', 'NfiGroupedArgs')])
 def test_struct_layout(tmp_path, name, struct):
     py = getattr(_lib, struct)
     fields = [f[0] for f in py._fields_]
@@ -67,3 +67,38 @@ def test_resnorm_work_holds_every_workgroup(rows, gates):
         per = 1 if splits > 1 else -(-segments // 512)
         blocks = -(-segments // per)
         assert lib.nfi_resnorm_work_bytes(rows, gates, 24) >= blocks * 5 * 24 * 4
+
+
+def test_grouped_linear_refuses():
+    with pytest.raises(RuntimeError, match='HIP devices only'):
+        grouped.grouped_linear(torch.zeros(2, 4), torch.zeros(1, 3, 4), torch.tensor([0, 2]))
+    lib = _lib.load()
+    one = ctypes.c_void_p(16)
+
+    def args(**kw):
+        a = _lib.NfiGroupedArgs()
+        a.x = a.w = a.y = a.offsets = one
+        a.rows, a.groups, a.in_width, a.out_width = 4, 2, 8, 8
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return a
+
+    for kw, word in (({'offsets': None}, b'null input'), ({'rows': 0}, b'rows'), ({'rows': 1 << 31}, b'rows'), ({'groups': 0}, b'groups'),
+                     ({'groups': 65536}, b'groups'), ({'in_width': 0}, b'widths'), ({'out_width': 1 << 22}, b'widths'),
+                     ({'dtype': 3}, b'type'), ({'x': None}, b'null tensor'), ({'y': None}, b'null tensor'),
+                     ({'in_width': 9}, b'work'), ({'rows': (1 << 31) - 1, 'out_width': 1 << 21}, b'tiles')):
+        assert lib.nfi_grouped_forward(ctypes.byref(args(**kw)), None) == -1, kw
+        assert word in lib.nfi_last_error(), (kw, lib.nfi_last_error())
+    for kw, word in (({}, b'null tensor'), ({'gy': one, 'gx': one, 'w': None}, b'null tensor'),
+                     ({'gy': one, 'gw': one, 'x': None}, b'null tensor'), ({'gy': one, 'gx': one, 'out_width': 7}, b'work')):
+        assert lib.nfi_grouped_backward(ctypes.byref(args(**kw)), None) == -1, kw
+        assert word in lib.nfi_last_error(), kw
+
+
+@pytest.mark.parametrize('sizes,before,behind', [([1], 0, 0), ([0, 0, 5], 3, 0), ([128, 129, 0, 1], 0, 7), ([1] * 200, 1, 1),
+                                                 ([300, 0, 4000, 127], 0, 128), ([0, 0], 2, 1)])
+def test_row_tiles_cover_every_run(sizes, before, behind):
+    """The launch's bound on row tiles (restated) is enough for every run of 128-row tiles, the rows of no group too."""
+    rows = before + sum(sizes) + behind
+    runs = sizes + [before, behind]
+    assert sum(-(-r // 128) for r in runs) <= -(-rows // 128) + min(len(sizes) + 2, rows)
