@@ -83,6 +83,35 @@ int64_t nfi_grouped_backward_work_bytes(const nfi_grouped_args* a);
 int32_t nfi_grouped_forward(const nfi_grouped_args* a, void* stream);
 int32_t nfi_grouped_backward(const nfi_grouped_args* a, void* stream);
 
+#define NFI_ORTHO_MAX_SIDE 262144
+
+/* A run of `count` matrices [rows][cols], one after the other: g the update's input of `g_type`, momentum
+ * (32-bit, updated, or NULL), w the result or the weights of `w_type`. */
+typedef struct nfi_ortho_item {
+  const void* g;
+  void *momentum, *w;
+  int32_t rows, cols, count;
+  float scale;
+} nfi_ortho_item;
+
+/* Every matrix of every item:  M <- momentum M + G (where it has one);  U = G + momentum M with nesterov,
+ * else M (G without M);  X = U / max(|U|_F, eps);  `steps` times X <- (a + b X X^T + c (X X^T)^2) X, for
+ * rows <= cols (else of the transposed matrix);  then w = X, or with update w <- (1 - decay) w - step
+ * scale X.  Products are held to 32-bit accuracy for every type, and the result is rounded once.  `items` is
+ * host memory, read during the call.  A polynomial under which singular values leave [0, 64) is refused.
+ * work: nfi_ortho_work_bytes, or NULL where that is 0. */
+typedef struct nfi_ortho_args {
+  const nfi_ortho_item* items;
+  void* work;
+  int64_t work_bytes;
+  int32_t n_items, g_type, w_type, update, nesterov, steps;
+  float momentum, step, decay, a, b, c, eps;
+  int32_t _pad;
+} nfi_ortho_args;
+
+int64_t nfi_ortho_work_bytes(const nfi_ortho_item* items, int32_t n_items);
+int32_t nfi_ortho(const nfi_ortho_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

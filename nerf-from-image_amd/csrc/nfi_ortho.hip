@@ -1,0 +1,730 @@
+// Orthogonalised updates (include/nfi_learn.h nfi_ortho): X0 = U / max(|U|_F, eps), taken with its smaller side as rows
+// (m <= n), then `steps` times
+//
+//   A = X X^T        Q = a I + b A + c A A        X <- Q X
+//
+// which maps every singular value s to the odd polynomial a s + b s^3 + c s^5 and leaves the singular vectors; with
+// U = G + beta M, M <- beta M + G (or U = M) before, and W <- (1 - decay) W - step X behind.  Per step m^2 n + m^3 + 2 m^2 n
+// operations (A and A A are symmetric: half of each product is computed and mirrored).
+//
+// Small singular values grow by up to `a` each step, and rounding errors with them, so every product is held to 32-bit
+// accuracy whatever the type of the weights: operands are pairs of halves hi = f16(v 2^s), lo = f16(v 2^s - hi), three
+// products hi hi + hi lo + lo hi on the 16-bit matrix cores into 32-bit sums (lo lo is below 2^-22 of the product).  All
+// operands are bounded (singular values start at <= 1 and the polynomial is known), so the scales are constants of the
+// call.  Memory holds 32 hi and 32 lo halves of 32 neighbouring columns together: 128 bytes that are one step of a tile.
+//
+// Matrices of up to 64 rows that fit into LDS run whole in one workgroup each, in 32-bit products; the others run
+// as tiles of 128 x 128, all matrices of the call in each launch: their grid holds one tile after the other.
+#include <algorithm>
+#include <cmath>
+
+#include "nfi_mm.h"
+
+namespace nfi {
+namespace learn {
+
+constexpr int ITEMS = 32;            // matrices (or runs of equal ones) of a launch
+constexpr int NORM_CHUNK = 16384;    // elements of a partial sum of squares
+
+struct Item {
+  const void* g;
+  float* mom;
+  void* w;
+  _Float16 *x, *y, *a, *q;    // workspace: X and the next X [mp][2 np], A and Q [mp][2 mp]
+  double* sums;               // [count][chunks]
+  float scale;                // the step's factor of this matrix
+  int rows, cols, count, m, n, mp, np, chunks;
+};
+
+struct Args {
+  Item item[ITEMS];
+  int items, g_type, w_type, update, nesterov, last;
+  float beta, keep, step, a, b, c, eps;   // keep = 1 - decay
+  float up_x, up_a, up_q;                 // powers of two
+};
+
+typedef _Float16 h4v __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ float typed_at(const void* p, int type, int64_t i) {
+  return type == NFI_F32 ? ((const float*)p)[i] : type == NFI_BF16 ? (float)((const bf16_t*)p)[i] : (float)((const f16_t*)p)[i];
+}
+
+// Work unit `id` of a launch: the item, the matrix of its run, and the unit within it (per(item) units each)
+template <class F>
+__device__ __forceinline__ int locate(const Args& p, int id, int& matrix, int& unit, F per) {
+  for (int i = 0; i < p.items; ++i) {
+    const int u = per(p.item[i]), all = u * p.item[i].count;
+    if (id < all) {
+      matrix = id / u;
+      unit = id - matrix * u;
+      return i;
+    }
+    id -= all;
+  }
+  return -1;
+}
+
+// ---- momentum and norm -------------------------------------------------------------------------------------------
+
+// M <- beta M + G, and the squares' sum of U over a chunk (64-bit: squares of bf16 values pass the 32-bit range)
+__global__ void __launch_bounds__(256) ortho_norm(const Args p) {
+  __shared__ double red[256];
+  int matrix, chunk;
+  const int i = locate(p, blockIdx.x, matrix, chunk, [](const Item& t) { return t.chunks; });
+  if (i < 0) return;
+  const Item& t = p.item[i];
+  const int64_t size = (int64_t)t.rows * t.cols, base = matrix * size;
+  const int64_t e0 = (int64_t)chunk * NORM_CHUNK, e1 = min(e0 + NORM_CHUNK, size);
+  double s = 0.;
+  for (int64_t e = e0 + threadIdx.x * 4; e < e1; e += 1024) {
+    float g[4], m[4];
+    if (e + 4 <= e1) {
+      load_typed<4>(t.g, p.g_type, base + e, g);
+      if (t.mom) load_piece<float, 4>(t.mom + base + e, m);
+    } else {
+      for (int j = 0; j < 4; ++j) {
+        g[j] = e + j < e1 ? typed_at(t.g, p.g_type, base + e + j) : 0.f;
+        m[j] = t.mom && e + j < e1 ? t.mom[base + e + j] : 0.f;
+      }
+    }
+    if (t.mom) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        m[j] = fmaf(p.beta, m[j], g[j]);
+        g[j] = p.nesterov ? fmaf(p.beta, m[j], g[j]) : m[j];
+      }
+      if (e + 4 <= e1) store_piece<float, 4>(t.mom + base + e, m);
+      else
+        for (int j = 0; e + j < e1; ++j) t.mom[base + e + j] = m[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s = fma((double)g[j], (double)g[j], s);
+  }
+  red[threadIdx.x] = s;
+  __syncthreads();
+  for (int d = 128; d > 0; d >>= 1) {
+    if (threadIdx.x < d) red[threadIdx.x] += red[threadIdx.x + d];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) t.sums[(int64_t)matrix * t.chunks + chunk] = red[0];
+}
+
+__device__ __forceinline__ float update_at(const Args& p, const Item& t, int64_t at) {
+  const float g = typed_at(t.g, p.g_type, at);
+  if (!t.mom) return g;
+  const float m = t.mom[at];
+  return p.nesterov ? fmaf(p.beta, m, g) : m;
+}
+
+// 1 / max(norm, eps) of the sums of a matrix, the same in every thread (64-bit: that of a large 32-bit norm is subnormal)
+__device__ __forceinline__ double inverse_norm(const double* sums, int chunks, float eps, double* red) {
+  double s = 0.;
+  for (int k = threadIdx.x; k < chunks; k += blockDim.x) s += sums[k];
+  red[threadIdx.x] = s;
+  __syncthreads();
+  for (int d = blockDim.x / 2; d > 0; d >>= 1) {
+    if ((int)threadIdx.x < d) red[threadIdx.x] += red[threadIdx.x + d];
+    __syncthreads();
+  }
+  const double n = sqrt(red[0]);
+  __syncthreads();
+  return 1. / (n < (double)eps ? (double)eps : n);   // (a NaN stays one)
+}
+
+__device__ __forceinline__ void split4(const float (&v)[4], h4v& hi, h4v& lo) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    hi[j] = (_Float16)v[j];
+    lo[j] = (_Float16)(v[j] - (float)hi[j]);
+  }
+}
+
+// place of column c's hi half in a row; its lo half is 32 further
+__device__ __forceinline__ int64_t half_at(int c) { return ((int64_t)(c >> 5) << 6) + (c & 31); }
+
+// X0 in halves, 64 x 64 at a time, turned where the matrix is taller than wide; zeros in the padding
+__global__ void __launch_bounds__(256) ortho_start(const Args p) {
+  __shared__ float tile[64][65];
+  __shared__ double red[256];
+  int matrix, unit;
+  const int i = locate(p, blockIdx.x, matrix, unit, [](const Item& t) { return t.mp / 64 * (t.np / 64); });
+  if (i < 0) return;
+  const Item& t = p.item[i];
+  const double inv = inverse_norm(t.sums + (int64_t)matrix * t.chunks, t.chunks, p.eps, red) * p.up_x;
+  const int r0 = unit / (t.np / 64) * 64, c0 = unit % (t.np / 64) * 64;
+  const int64_t base = (int64_t)matrix * t.rows * t.cols;
+  const bool turned = t.rows > t.cols;
+  const int a = threadIdx.x & 63, b = threadIdx.x >> 6;
+  for (int k = b; k < 64; k += 4) {
+    // (a runs along memory)
+    const int r = turned ? r0 + a : r0 + k, c = turned ? c0 + k : c0 + a;
+    float v = 0.f;
+    if (r < t.m && c < t.n) v = (float)(update_at(p, t, base + (turned ? (int64_t)c * t.cols + r : (int64_t)r * t.cols + c)) * inv);
+    if (turned) tile[a][k] = v;
+    else tile[k][a] = v;
+  }
+  __syncthreads();
+  _Float16* x = t.x + (int64_t)matrix * t.mp * 2 * t.np;
+  for (int k = threadIdx.x; k < 1024; k += 256) {
+    const int r = k >> 4, c = (k & 15) * 4;
+    const float v[4] = {tile[r][c], tile[r][c + 1], tile[r][c + 2], tile[r][c + 3]};
+    h4v hi, lo;
+    split4(v, hi, lo);
+    _Float16* d = x + (int64_t)(r0 + r) * 2 * t.np + half_at(c0 + c);
+    *reinterpret_cast<h4v*>(d) = hi;
+    *reinterpret_cast<h4v*>(d + 32) = lo;
+  }
+}
+
+// ---- products of pairs of halves -------------------------------------------------------------------------------------
+
+// An operand whose contracted index runs over rows: LDS [32 rows][128 columns hi and lo: 512 bytes]
+struct PairSlab {
+  unsigned off[4];
+  static __device__ __forceinline__ int lds_row(int j) { return ((threadIdx.x >> 6) * 4 + j) * 2 + (lane_id() >> 5); }
+  __device__ __forceinline__ void init(unsigned ld) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int row = lds_row(j);
+      off[j] = row * ld + (((lane_id() & 31) ^ (2 * (row & 7))) << 4);
+    }
+  }
+  __device__ __forceinline__ void issue(const void* base, unsigned char* lds) const {
+    const __amdgpu_buffer_rsrc_t r = descriptor(base);
+    unsigned char* dst = lds + (threadIdx.x >> 6) * 4096;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) load_to_lds(r, dst + j * 1024, off[j]);
+  }
+};
+
+template <int N>
+__device__ __forceinline__ void read_pair_slab(const unsigned char* lds, int line0, int plane, u4v (&f)[N]) {
+  const int i = lane_id() & 15, g = lane_id() >> 4, r0 = 8 * g + (i >> 2), half = (i & 1) * 8;
+#pragma unroll
+  for (int x = 0; x < N; ++x) {
+    const int c = line0 + 16 * x, piece = ((c >> 5) << 3) + ((c & 31) >> 3) + 4 * plane + ((i & 3) >> 1);
+    u2v v[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = r0 + 4 * h;
+      const unsigned char* q = lds + row * 512 + ((piece ^ (2 * (row & 7))) << 4) + half;
+      v[h] = __builtin_bit_cast(u2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*)q));
+    }
+    f[x] = u4v{v[0][0], v[0][1], v[1][0], v[1][1]};
+  }
+}
+
+// acc (a's lines by lane, b's by register) of a 128 x 128 tile; K a multiple of 32, everything inside the padding.
+// a: lines; b: lines, or (SLAB) rows of the contracted index; SWAP: the roles of lane and register exchanged
+template <bool SLAB, bool SWAP>
+__device__ __forceinline__ void pair_product(const _Float16* a, unsigned lda, const _Float16* b, unsigned ldb, int k, unsigned char* lds,
+                                             f4v (&acc)[4][4]) {
+  TileLoad<_Float16, false> la, lb;
+  PairSlab sb;
+  la.init(TILE, lda);
+  if (SLAB) sb.init(ldb);
+  else lb.init(TILE, ldb);
+  const int64_t step_b = SLAB ? (int64_t)32 * ldb : STEP_BYTES;
+  const int wave = threadIdx.x >> 6, line_a = (wave & 1) * 64, line_b = (wave >> 1) * 64, steps = k / 32;
+  const unsigned char *pa = (const unsigned char*)a, *pb = (const unsigned char*)b;
+  auto issue = [&](int t, unsigned char* dst) {
+    la.issue(pa + (int64_t)t * STEP_BYTES, dst, STEP_BYTES);
+    if (SLAB) sb.issue(pb + t * step_b, dst + TILE_BYTES);
+    else lb.issue(pb + t * step_b, dst + TILE_BYTES, STEP_BYTES);
+  };
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) acc[x][y] = f4v{0.f, 0.f, 0.f, 0.f};
+  issue(0, lds);
+  for (int t = 0; t < steps; ++t) {
+    const unsigned char* cur = lds + (t & 1) * 2 * TILE_BYTES;
+    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's loads of step t are in LDS
+    __syncthreads();
+    u4v fa[2][4], fb[2][4];
+#pragma unroll
+    for (int plane = 0; plane < 2; ++plane) {
+      read_fragments<_Float16, false, 4>(cur, line_a, plane, fa[plane]);
+      if (SLAB) read_pair_slab<4>(cur + TILE_BYTES, line_b, plane, fb[plane]);
+      else read_fragments<_Float16, false, 4>(cur + TILE_BYTES, line_b, plane, fb[plane]);
+    }
+    if (t + 1 < steps) issue(t + 1, lds + ((t + 1) & 1) * 2 * TILE_BYTES);
+#pragma unroll
+    for (int pair = 0; pair < 3; ++pair)   // lo hi, hi lo, hi hi: the small ones first
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const u4v va = fa[pair == 0][x], vb = fb[pair == 1][y];
+          acc[x][y] = SWAP ? product<_Float16>(va, vb, acc[x][y]) : product<_Float16>(vb, va, acc[x][y]);
+        }
+  }
+}
+
+// a 128 x 128 tile of a symmetric matrix in halves to (r0, c0), and mirrored to (c0, r0) off the diagonal
+__device__ __forceinline__ void store_symmetric(_Float16* d, int ld, int r0, int c0, const f4v (&v)[4][4], unsigned char* lds) {
+  const int wave = threadIdx.x >> 6, i = lane_id() & 15, g = lane_id() >> 4;
+  const int la = (wave & 1) * 64, lb = (wave >> 1) * 64;
+  float* f = (float*)lds;
+  __syncthreads();   // (the last step's fragments have been read)
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const int row = la + 16 * x + i;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int col = lb + 16 * y + 4 * g;
+      const float u[4] = {v[x][y][0], v[x][y][1], v[x][y][2], v[x][y][3]};
+      h4v hi, lo;
+      split4(u, hi, lo);
+      _Float16* p = d + (int64_t)(r0 + row) * ld + half_at(c0 + col);
+      *reinterpret_cast<h4v*>(p) = hi;
+      *reinterpret_cast<h4v*>(p + 32) = lo;
+      if (r0 != c0) lds_st_fenced(reinterpret_cast<f4v*>(f + row * 128 + (col ^ (((row >> 2) & 3) << 4))), v[x][y]);
+    }
+  }
+  if (r0 == c0) return;
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const int row = la + 16 * x + i;   // a column of the tile
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int col = lb + 16 * y + 4 * g;
+      float u[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) u[r] = f[(col + r) * 128 + (row ^ ((((col + r) >> 2) & 3) << 4))];
+      h4v hi, lo;
+      split4(u, hi, lo);
+      _Float16* p = d + (int64_t)(c0 + row) * ld + half_at(r0 + col);
+      *reinterpret_cast<h4v*>(p) = hi;
+      *reinterpret_cast<h4v*>(p + 32) = lo;
+    }
+  }
+}
+
+__device__ __forceinline__ void triangle(int unit, int& ti, int& tj) {
+  ti = 0;
+  while (unit >= ti + 1) {
+    unit -= ti + 1;
+    ++ti;
+  }
+  tj = unit;
+}
+
+// A = X X^T (SQUARE false) or Q = a I + b A + c A A (SQUARE true), the tiles on and below the diagonal
+template <bool SQUARE>
+__global__ void __launch_bounds__(256) ortho_gram(const Args p) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * TILE_BYTES];
+  int matrix, unit, ti, tj;
+  const int it = locate(p, blockIdx.x, matrix, unit, [](const Item& t) { const int k = t.mp / TILE; return k * (k + 1) / 2; });
+  if (it < 0) return;
+  const Item& t = p.item[it];
+  triangle(unit, ti, tj);
+  const int k = SQUARE ? t.mp : t.np;
+  const _Float16* src = (SQUARE ? t.a : t.x) + (int64_t)matrix * t.mp * 2 * k;
+  const unsigned ld = 4u * k;
+  f4v acc[4][4];
+  pair_product<false, false>(src + (int64_t)ti * TILE * 2 * k, ld, src + (int64_t)tj * TILE * 2 * k, ld, k, lds, acc);
+  const int wave = threadIdx.x >> 6, i = lane_id() & 15, g = lane_id() >> 4;
+  const int r0 = ti * TILE, c0 = tj * TILE;
+  if constexpr (!SQUARE) {
+    const float s = p.up_a / (p.up_x * p.up_x);
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) acc[x][y] *= s;
+  } else {
+    const float s = p.c * p.up_q / (p.up_a * p.up_a), sb = p.b * p.up_q / p.up_a, sa = p.a * p.up_q;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int row = r0 + (wave & 1) * 64 + 16 * x + i;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int col = c0 + (wave >> 1) * 64 + 16 * y + 4 * g;
+        const _Float16* q = src + (int64_t)row * 2 * k + half_at(col);
+        const h4v hi = *reinterpret_cast<const h4v*>(q), lo = *reinterpret_cast<const h4v*>(q + 32);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float a = (float)hi[r] + (float)lo[r];
+          acc[x][y][r] = fmaf(s, acc[x][y][r], fmaf(sb, a, row == col + r ? sa : 0.f));
+        }
+      }
+    }
+  }
+  store_symmetric((SQUARE ? t.q : t.a) + (int64_t)matrix * t.mp * 2 * t.mp, 2 * t.mp, r0, c0, acc, lds);
+}
+
+// X' = Q X, or with `last` the weights' step (or the result)
+__device__ __forceinline__ void put_update(const Args& p, const Item& t, int64_t at, const f4v& acc, float s, int count) {
+  float v[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v[r] = acc[r] * s;
+  if (p.update) {
+    const float step = p.step * t.scale;
+    for (int r = 0; r < count; ++r) v[r] = fmaf(p.keep, typed_at(t.w, p.w_type, at + r), -step * v[r]);
+  }
+  if (p.w_type == NFI_F32) {
+    if (count == 4) store_piece<float, 4>((float*)t.w + at, v);
+    else
+      for (int r = 0; r < count; ++r) ((float*)t.w)[at + r] = v[r];
+  } else {
+    for (int r = 0; r < count; ++r) store_typed(t.w, p.w_type, at + r, v[r]);
+  }
+}
+
+__global__ void __launch_bounds__(256) ortho_apply(const Args p) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * TILE_BYTES];
+  int matrix, unit;
+  const int it = locate(p, blockIdx.x, matrix, unit, [](const Item& t) { return t.mp / TILE * (t.np / TILE); });
+  if (it < 0) return;
+  const Item& t = p.item[it];
+  const int tr = unit % (t.mp / TILE), tc = unit / (t.mp / TILE);   // the tiles of a block of X's columns follow each other
+  const int r0 = tr * TILE, c0 = tc * TILE;
+  const _Float16* q = t.q + (int64_t)matrix * t.mp * 2 * t.mp + (int64_t)r0 * 2 * t.mp;
+  const _Float16* x = t.x + (int64_t)matrix * t.mp * 2 * t.np + half_at(c0);
+  const int wave = threadIdx.x >> 6, i = lane_id() & 15, g = lane_id() >> 4;
+  const int la = (wave & 1) * 64, lb = (wave >> 1) * 64;
+  const float s = 1.f / (p.up_q * p.up_x), down = 1.f / p.up_q;
+  const int64_t base = (int64_t)matrix * t.rows * t.cols;
+  f4v acc[4][4];
+  if (p.last && t.rows > t.cols) {   // (uniform) the turned matrix: a lane holds neighbours along X's rows
+    pair_product<true, true>(q, 4u * t.mp, x, 4u * t.np, t.mp, lds, acc);
+#pragma unroll
+    for (int xx = 0; xx < 4; ++xx)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int row = r0 + la + 16 * xx + 4 * g, col = c0 + lb + 16 * y + i;
+        if (row < t.m && col < t.n) put_update(p, t, base + (int64_t)col * t.cols + row, acc[xx][y], s, min(4, t.m - row));
+      }
+    return;
+  }
+  pair_product<true, false>(q, 4u * t.mp, x, 4u * t.np, t.mp, lds, acc);
+  _Float16* d = t.y + (int64_t)matrix * t.mp * 2 * t.np;
+#pragma unroll
+  for (int xx = 0; xx < 4; ++xx)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int row = r0 + la + 16 * xx + i, col = c0 + lb + 16 * y + 4 * g;
+      if (p.last) {
+        if (row < t.m && col < t.n) put_update(p, t, base + (int64_t)row * t.cols + col, acc[xx][y], s, min(4, t.n - col));
+      } else {
+        const float v[4] = {acc[xx][y][0] * down, acc[xx][y][1] * down, acc[xx][y][2] * down, acc[xx][y][3] * down};
+        h4v hi, lo;
+        split4(v, hi, lo);
+        _Float16* o = d + (int64_t)row * 2 * t.np + half_at(col);
+        *reinterpret_cast<h4v*>(o) = hi;
+        *reinterpret_cast<h4v*>(o + 32) = lo;
+      }
+    }
+}
+
+// ---- small matrices ----------------------------------------------------------------------------------------------------
+
+// One workgroup of 8 waves holds X [mp][np + 4], A and Q [mp][mp + 4] in LDS (32 bits, rows of 16-column blocks padded by
+// 4: the rows of a read lie in different banks) and runs every step in v_mfma_f32_16x16x4_f32.
+constexpr int SMALL_WAVES = 8;
+
+__host__ __device__ __forceinline__ int small_floats(int mp, int np) { return mp * (np + 4) + 2 * mp * (mp + 4) + SMALL_WAVES * 256; }
+
+__device__ __forceinline__ u4v lines4(const float* p, int ld, int line0, int k0) {
+  return *reinterpret_cast<const u4v*>(p + (line0 + (lane_id() & 15)) * ld + k0 + 4 * (lane_id() >> 4));
+}
+
+template <int FLOATS>
+__global__ void __launch_bounds__(64 * SMALL_WAVES) ortho_small(const Args p, int steps) {
+  __shared__ __attribute__((aligned(16))) float lds[FLOATS];
+  __shared__ double red[64 * SMALL_WAVES];
+  int matrix, unit;
+  const int it = locate(p, blockIdx.x, matrix, unit, [](const Item&) { return 1; });
+  if (it < 0) return;
+  const Item& t = p.item[it];
+  const int mp = t.mp, np = t.np, ldx = np + 4, lda = mp + 4, nb = mp / 16;
+  float *X = lds, *A = X + mp * ldx, *Q = A + mp * lda, *P = Q + mp * lda;
+  const int64_t size = (int64_t)t.rows * t.cols, base = matrix * size;
+  const bool turned = t.rows > t.cols;
+  const int tid = threadIdx.x, wave = tid >> 6, l = lane_id(), i = l & 15, g = l >> 4;
+  for (int k = tid; k < mp * ldx; k += 64 * SMALL_WAVES) X[k] = 0.f;
+  __syncthreads();
+  double s = 0.;
+  for (int e = tid; e < (int)size; e += 64 * SMALL_WAVES) {
+    float v = typed_at(t.g, p.g_type, base + e);
+    if (t.mom) {
+      const float m = fmaf(p.beta, t.mom[base + e], v);
+      t.mom[base + e] = m;
+      v = p.nesterov ? fmaf(p.beta, m, v) : m;
+    }
+    const int r = e / t.cols, c = e - r * t.cols;
+    X[turned ? c * ldx + r : r * ldx + c] = v;
+    s = fma((double)v, (double)v, s);
+  }
+  red[tid] = s;
+  __syncthreads();
+  for (int d = 32 * SMALL_WAVES; d > 0; d >>= 1) {
+    if (tid < d) red[tid] += red[tid + d];
+    __syncthreads();
+  }
+  const double norm = sqrt(red[0]);
+  const double inv = 1. / (norm < (double)p.eps ? (double)p.eps : norm);
+  for (int k = tid; k < mp * ldx; k += 64 * SMALL_WAVES) X[k] = (float)(X[k] * inv);
+  // A's blocks over the waves, the columns of X in ks pieces where there are few blocks
+  const int blocks = nb * nb, ks = nb == 1 ? 8 : nb == 2 ? 2 : 1, pieces = np / 16;
+  for (int step = 0; step < steps; ++step) {
+    __syncthreads();
+    for (int task = wave; task < blocks * ks; task += SMALL_WAVES) {
+      const int blk = task / ks, part = task - blk * ks, bi = blk / nb, bj = blk - bi * nb;
+      f4v acc = {0.f, 0.f, 0.f, 0.f};
+      if (bj <= bi)
+        for (int k = pieces * part / ks; k < pieces * (part + 1) / ks; ++k)
+          acc = product<float>(lines4(X, ldx, bi * 16, 16 * k), lines4(X, ldx, bj * 16, 16 * k), acc);
+      // lane: bj's line i, registers: bi's lines 4 g + r
+      if (ks > 1) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) P[task * 256 + (4 * g + r) * 16 + i] = acc[r];
+      } else if (bj <= bi) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          A[(bi * 16 + 4 * g + r) * lda + bj * 16 + i] = acc[r];
+          A[(bj * 16 + i) * lda + bi * 16 + 4 * g + r] = acc[r];
+        }
+      }
+    }
+    __syncthreads();
+    if (ks > 1) {
+      for (int e = tid; e < blocks * 256; e += 64 * SMALL_WAVES) {
+        const int blk = e >> 8, bi = blk / nb, bj = blk - bi * nb, r = (e >> 4) & 15, c = e & 15;
+        if (bj > bi) continue;
+        float v = 0.f;
+        for (int q = 0; q < ks; ++q) v += P[(blk * ks + q) * 256 + (e & 255)];
+        A[(bi * 16 + r) * lda + bj * 16 + c] = v;
+        if (bi != bj) A[(bj * 16 + c) * lda + bi * 16 + r] = v;
+      }
+      __syncthreads();
+    }
+    for (int task = wave; task < blocks; task += SMALL_WAVES) {
+      const int bi = task / nb, bj = task - bi * nb;
+      f4v acc = {0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < nb; ++k) acc = product<float>(lines4(A, lda, bi * 16, 16 * k), lines4(A, lda, bj * 16, 16 * k), acc);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = bi * 16 + 4 * g + r, col = bj * 16 + i;
+        Q[row * lda + col] = fmaf(p.c, acc[r], fmaf(p.b, A[row * lda + col], row == col ? p.a : 0.f));
+      }
+    }
+    __syncthreads();
+    // a wave takes whole blocks of X's columns, which no other one reads: in place
+    for (int cb = wave; cb < pieces; cb += SMALL_WAVES) {
+      f4v acc[4];
+#pragma unroll
+      for (int bi = 0; bi < 4; ++bi) acc[bi] = f4v{0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < nb; ++k) {
+        u4v x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = __float_as_uint(X[(16 * k + 4 * g + r) * ldx + cb * 16 + i]);
+#pragma unroll
+        for (int bi = 0; bi < 4; ++bi)
+          if (bi < nb) acc[bi] = product<float>(lines4(Q, lda, bi * 16, 16 * k), x, acc[bi]);
+      }
+#pragma unroll
+      for (int bi = 0; bi < 4; ++bi)
+        if (bi < nb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) X[(bi * 16 + 4 * g + r) * ldx + cb * 16 + i] = acc[bi][r];
+    }
+  }
+  __syncthreads();
+  const float step = p.step * t.scale;
+  for (int e = tid; e < (int)size; e += 64 * SMALL_WAVES) {
+    const int r = e / t.cols, c = e - r * t.cols;
+    float v = X[turned ? c * ldx + r : r * ldx + c];
+    if (p.update) v = fmaf(p.keep, typed_at(t.w, p.w_type, base + e), -step * v);
+    store_typed(t.w, p.w_type, base + e, v);
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------------
+
+constexpr int SMALL_SIZES[3] = {9216, 18432, 36864};   // floats of LDS: 36, 72, 144 KB
+static inline int ceil_to(int v, int k) { return (v + k - 1) / k * k; }
+static inline int64_t up(int64_t v) { return (v + 255) / 256 * 256; }
+
+// -1: as tiles; else the small kernel's size.  (One workgroup runs a 64 x 448 matrix in the time that the tiles' launches
+// alone take, so whatever fits into LDS runs there.)
+static int small_size(int m, int n) {
+  if (m > 64) return -1;
+  // (n may be any number: the product has to stay in range)
+  if (n > 65536) return -1;
+  const int need = small_floats(ceil_to(m, 16), ceil_to(n, 16));
+  for (int k = 0; k < 3; ++k)
+    if (need <= SMALL_SIZES[k]) return k;
+  return -1;
+}
+
+static int64_t item_bytes(const nfi_ortho_item& s) {
+  const int m = std::min(s.rows, s.cols), n = std::max(s.rows, s.cols);
+  if (small_size(m, n) >= 0) return 0;
+  const int64_t mp = ceil_to(m, TILE), np = ceil_to(n, TILE), size = (int64_t)s.rows * s.cols;
+  return s.count * (2 * up(mp * np * 4) + 2 * up(mp * mp * 4)) + up(s.count * ((size + NORM_CHUNK - 1) / NORM_CHUNK) * 8);
+}
+
+// largest |s q(s^2)| and |q| over s in [0, top]
+static void bounds(float a, float b, float c, double top, double& x, double& q) {
+  x = q = 0.;
+  for (int k = 0; k <= 4096; ++k) {
+    const double s = top * k / 4096, t = s * s, v = a + t * (b + t * c);
+    x = std::max(x, std::fabs(s * v));
+    q = std::max(q, std::fabs(v));
+  }
+}
+
+static int check(const nfi_ortho_args* p, double& most_x, double& most_q) {
+  NFI_REQUIRE(p && p->items && p->n_items > 0, "ortho: no matrices");
+  NFI_REQUIRE(type_ok(p->g_type) && type_ok(p->w_type), "ortho: bad type");
+  NFI_REQUIRE(p->steps >= 1 && p->steps <= 64, "ortho: %d steps (1 .. 64)", p->steps);
+  NFI_REQUIRE(p->eps > 0.f && std::isfinite(p->eps), "ortho: eps %g", (double)p->eps);
+  for (int i = 0; i < p->n_items; ++i) {
+    const nfi_ortho_item& s = p->items[i];
+    NFI_REQUIRE(s.rows > 0 && s.cols > 0 && s.count > 0 && s.rows <= NFI_ORTHO_MAX_SIDE && s.cols <= NFI_ORTHO_MAX_SIDE,
+                "ortho: matrix %d is %d x %d x %d (sides 1 .. %d)", i, s.count, s.rows, s.cols, NFI_ORTHO_MAX_SIDE);
+    const int64_t tr = (s.rows + TILE - 1) / TILE, tc = (s.cols + TILE - 1) / TILE;
+    NFI_REQUIRE(4 * tr * tc * s.count < (1ll << 26), "ortho: matrix %d is too large", i);
+    NFI_REQUIRE(s.g && s.w, "ortho: null tensor");
+  }
+  // the iterates stay bounded under this polynomial
+  double top = 1., x, q;
+  most_x = 1.;
+  most_q = 0.;
+  for (int k = 0; k < p->steps; ++k) {
+    bounds(p->a, p->b, p->c, top * 1.0001, x, q);
+    most_x = std::max(most_x, x);
+    most_q = std::max(most_q, q);
+    top = x;
+    NFI_REQUIRE(std::isfinite(x) && x < 64. && q > 0. && q < 4096., "ortho: the polynomial %g, %g, %g leaves its range", (double)p->a, (double)p->b,
+                (double)p->c);
+  }
+  return NFI_OK;
+}
+
+static float power_below(double limit) { return (float)std::ldexp(1., (int)std::floor(std::log2(limit))); }
+
+}  // namespace learn
+}  // namespace nfi
+
+using namespace nfi::learn;
+
+extern "C" {
+
+int64_t nfi_ortho_work_bytes(const nfi_ortho_item* items, int32_t n_items) {
+  int64_t most = 0, sum = 0;
+  int held = 0;
+  for (int i = 0; i < n_items; ++i) {
+    const int64_t b = item_bytes(items[i]);
+    if (b == 0) continue;
+    sum += b;
+    most = std::max(most, sum);
+    if (++held == ITEMS) held = 0, sum = 0;
+  }
+  return most;
+}
+
+int32_t nfi_ortho(const nfi_ortho_args* p, void* stream) {
+  double most_x, most_q;
+  const int e = check(p, most_x, most_q);
+  if (e) return e;
+  const int64_t need = nfi_ortho_work_bytes(p->items, p->n_items);
+  NFI_REQUIRE(p->work_bytes >= need && (need == 0 || p->work), "ortho: %lld bytes of work, %lld wanted", (long long)p->work_bytes, (long long)need);
+  hipStream_t s = (hipStream_t)stream;
+  Args base = {};
+  base.g_type = p->g_type;
+  base.w_type = p->w_type;
+  base.update = p->update;
+  base.nesterov = p->nesterov;
+  base.beta = p->momentum;
+  base.keep = 1.f - p->decay;
+  base.step = p->step;
+  base.a = p->a;
+  base.b = p->b;
+  base.c = p->c;
+  base.eps = p->eps;
+  // largest halves: entries of a matrix are at most its largest singular value (with room for rounding)
+  base.up_x = power_below(60000. / (1.001 * most_x));
+  base.up_a = power_below(60000. / (1.002 * most_x * most_x));
+  base.up_q = power_below(60000. / (1.002 * most_q));
+  auto item = [&](const nfi_ortho_item& q, int unit) {
+    Item t = {};
+    t.g = q.g;
+    t.mom = (float*)q.momentum;
+    t.w = q.w;
+    t.scale = q.scale;
+    t.rows = q.rows;
+    t.cols = q.cols;
+    t.count = q.count;
+    t.m = std::min(q.rows, q.cols);
+    t.n = std::max(q.rows, q.cols);
+    t.mp = ceil_to(t.m, unit);
+    t.np = ceil_to(t.n, unit);
+    return t;
+  };
+  for (int size = 0; size < 3; ++size) {
+    Args a = base;
+    int64_t blocks = 0;
+    auto flush = [&]() {
+      if (a.items == 0) return;
+      if (size == 0) ortho_small<SMALL_SIZES[0]><<<(unsigned)blocks, 64 * SMALL_WAVES, 0, s>>>(a, p->steps);
+      else if (size == 1) ortho_small<SMALL_SIZES[1]><<<(unsigned)blocks, 64 * SMALL_WAVES, 0, s>>>(a, p->steps);
+      else ortho_small<SMALL_SIZES[2]><<<(unsigned)blocks, 64 * SMALL_WAVES, 0, s>>>(a, p->steps);
+      a.items = 0;
+      blocks = 0;
+    };
+    for (int i = 0; i < p->n_items; ++i) {
+      const nfi_ortho_item& q = p->items[i];
+      if (small_size(std::min(q.rows, q.cols), std::max(q.rows, q.cols)) != size) continue;
+      a.item[a.items++] = item(q, 16);
+      blocks += q.count;
+      if (a.items == ITEMS) flush();
+    }
+    flush();
+  }
+  Args a = base;
+  unsigned char* work = (unsigned char*)p->work;
+  int64_t chunks = 0, starts = 0, grams = 0, tiles = 0;
+  auto flush = [&]() {
+    if (a.items == 0) return;
+    ortho_norm<<<(unsigned)chunks, 256, 0, s>>>(a);
+    ortho_start<<<(unsigned)starts, 256, 0, s>>>(a);
+    for (int k = 0; k < p->steps; ++k) {
+      a.last = k == p->steps - 1;
+      ortho_gram<false><<<(unsigned)grams, 256, 0, s>>>(a);
+      ortho_gram<true><<<(unsigned)grams, 256, 0, s>>>(a);
+      ortho_apply<<<(unsigned)tiles, 256, 0, s>>>(a);
+      for (int i = 0; i < a.items; ++i) std::swap(a.item[i].x, a.item[i].y);
+    }
+    a = base;
+    work = (unsigned char*)p->work;
+    chunks = starts = grams = tiles = 0;
+  };
+  for (int i = 0; i < p->n_items; ++i) {
+    const nfi_ortho_item& q = p->items[i];
+    if (small_size(std::min(q.rows, q.cols), std::max(q.rows, q.cols)) >= 0) continue;
+    Item t = item(q, TILE);
+    const int64_t sx = up((int64_t)t.mp * t.np * 4) * t.count, sa = up((int64_t)t.mp * t.mp * 4) * t.count;
+    t.x = (_Float16*)work;
+    t.y = (_Float16*)(work + sx);
+    t.a = (_Float16*)(work + 2 * sx);
+    t.q = (_Float16*)(work + 2 * sx + sa);
+    t.sums = (double*)(work + 2 * sx + 2 * sa);
+    t.chunks = (int)(((int64_t)q.rows * q.cols + NORM_CHUNK - 1) / NORM_CHUNK);
+    work += item_bytes(q);
+    a.item[a.items++] = t;
+    const int64_t mt = t.mp / TILE;
+    chunks += (int64_t)t.chunks * t.count;
+    starts += (int64_t)(t.mp / 64) * (t.np / 64) * t.count;
+    grams += mt * (mt + 1) / 2 * t.count;
+    tiles += mt * (t.np / TILE) * t.count;
+    if (a.items == ITEMS) flush();
+  }
+  flush();
+  NFI_CHECK_LAUNCH("ortho");
+  return NFI_OK;
+}
+
+}  // extern "C"

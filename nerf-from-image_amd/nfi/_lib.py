@@ -73,6 +73,19 @@ class NfiGroupedArgs(ctypes.Structure):
         ('out_width', ctypes.c_int32), ('dtype', ctypes.c_int32), ('offsets64', ctypes.c_int32), ('_pad', ctypes.c_int32)]
 
 
+class NfiOrthoItem(ctypes.Structure):
+    _fields_ = [('g', c_void_p), ('momentum', c_void_p), ('w', c_void_p), ('rows', ctypes.c_int32), ('cols', ctypes.c_int32),
+                ('count', ctypes.c_int32), ('scale', ctypes.c_float)]
+
+
+class NfiOrthoArgs(ctypes.Structure):
+    _fields_ = [('items', ctypes.POINTER(NfiOrthoItem)), ('work', c_void_p), ('work_bytes', ctypes.c_int64),
+                ('n_items', ctypes.c_int32), ('g_type', ctypes.c_int32), ('w_type', ctypes.c_int32), ('update', ctypes.c_int32),
+                ('nesterov', ctypes.c_int32), ('steps', ctypes.c_int32), ('momentum', ctypes.c_float), ('step', ctypes.c_float),
+                ('decay', ctypes.c_float), ('a', ctypes.c_float), ('b', ctypes.c_float), ('c', ctypes.c_float),
+                ('eps', ctypes.c_float), ('_pad', ctypes.c_int32)]
+
+
 # symbol -> (restype, argtypes); every entry point of include/nfi.h
 SIGNATURES = {
     'nfi_abi_version': (ctypes.c_int32, []),
@@ -225,6 +238,8 @@ SIGNATURES = {
     'nfi_grouped_backward_work_bytes': (ctypes.c_int64, [ctypes.POINTER(NfiGroupedArgs)]),
     'nfi_grouped_forward': (ctypes.c_int32, [ctypes.POINTER(NfiGroupedArgs), c_void_p]),
     'nfi_grouped_backward': (ctypes.c_int32, [ctypes.POINTER(NfiGroupedArgs), c_void_p]),
+    'nfi_ortho_work_bytes': (ctypes.c_int64, [ctypes.POINTER(NfiOrthoItem), ctypes.c_int32]),
+    'nfi_ortho': (ctypes.c_int32, [ctypes.POINTER(NfiOrthoArgs), c_void_p]),
 }
 
 _lib = None

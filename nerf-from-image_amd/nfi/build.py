@@ -11,7 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(HERE), 'csrc')
 OUT = os.path.join(HERE, 'libnfi_hip.so')
 SOURCES = ['nfi_rays.hip', 'nfi_render.hip', 'nfi_producer.hip', 'nfi_conv.hip', 'nfi_gemm.hip', 'nfi_dconv.hip',
-           'nfi_norms.hip', 'nfi_grouped.hip']
+           'nfi_norms.hip', 'nfi_grouped.hip', 'nfi_ortho.hip']
 HEADERS = ['nfi_common.h', 'nfi_host.h', 'nfi_learn.h', 'nfi_mm.h']
 # -packed-fp32-ops: no v_pk_add / mul / fma_f32 in the build.  Some of their forms have given wrong results
 # on this hardware now and then; measured cost on the renderer 1 % (p3d_car B = 8 step 5.85 -> 5.91 ms, within

@@ -1,0 +1,248 @@
+"""nfi.optim on the device against the formula in 64 bits: matrices of every shape and both kernels (whole in a workgroup,
+128 x 128 tiles), types, momentum, decay, empty and degenerate matrices, capture.
+
+Tolerance.  One step X -> a X + (b A + c A^2) X is a function of X whose derivative is at most L = 4 for singular values
+up to 1.2 (the quintic's own is 3.4 at 0 and below 4 at 1.2).  Every product is held to 8 x 2^-22 of its factors' norms
+(a pair of halves keeps 2^-22 of a value, the dropped product is of the same size, sums add 2^-24 for each of their
+steps of 32), so k steps are off by at most (1 + L + ... + L^(k-1)) 8 x 2^-22 |X|_F = 341 x 8 x 2^-22 |X|_F after five.  That is
+the worst case; beside it the error has to be at most 4 times that of the same formula in torch's 32-bit products, plus 2^-21."""
+
+import copy
+import math
+
+import pytest
+import torch
+
+from nfi import optim
+from nfi.producer import EqualizedLinear
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device('cuda:0')
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def formula(u, steps=5, abc=optim.QUINTIC, eps=1e-7):
+    a, b, c = abc
+    turned = u.shape[-2] > u.shape[-1]
+    x = u.transpose(-2, -1) if turned else u
+    x = x / x.square().sum((-2, -1), keepdim=True).sqrt().clamp_min(eps)
+    for _ in range(steps):
+        g = x @ x.transpose(-2, -1).contiguous()
+        x = a * x + (b * g + c * (g @ g)) @ x
+    return x.transpose(-2, -1) if turned else x
+
+
+def near(got, u, dtype, steps=5, abc=optim.QUINTIC):
+    ref = formula(u.double(), steps, abc)
+    plain = formula(u.float(), steps, abc)
+    size = float(ref.norm())
+    e = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+    err = float((got.double() - ref).norm())
+    own = float((plain.double() - ref).norm())
+    assert err <= e * size + 341 * 8 * 2.0 ** -22 * max(size, 1.0), (tuple(u.shape), err, size)
+    if dtype == torch.float32:
+        assert err <= 4 * own + 2.0 ** -21 * max(size, 1e-30), (tuple(u.shape), err, own, size)
+
+
+SHAPES = [(1, 1), (1, 7), (9, 1), (3, 3), (2, 15, 512), (16, 16), (17, 40), (40, 17), (3, 33, 33), (64, 64), (64, 448), (448, 64), (64, 449),
+          (65, 70), (33, 1100), (128, 128), (129, 257), (300, 200), (2, 3, 96, 512), (513, 700), (11, 64), (5, 3000), (1, 70000),
+          (640, 1300)]
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('shape', SHAPES, ids=lambda s: 'x'.join(map(str, s)))
+def test_orthogonalize(shape, dtype):
+    g = torch.Generator(device=DEV).manual_seed(sum(shape))
+    u = (torch.randn(shape, device=DEV, generator=g) * torch.exp2(-2 * torch.rand(shape[-1], device=DEV, generator=g))).to(dtype)
+    out = optim.orthogonalize(u)
+    assert out.shape == u.shape and out.dtype == dtype
+    near(out, u, dtype)
+    assert torch.equal(out, optim.orthogonalize(u))      # the same bits again
+
+
+@pytest.mark.parametrize('steps,abc', [(1, optim.QUINTIC), (3, optim.QUINTIC), (12, (1.5, -0.5, 0.0)), (5, (2.0, -1.5, 0.5)), (10, (1.875, -1.25, 0.375))])
+@pytest.mark.parametrize('shape', [(20, 50), (200, 150)])
+def test_other_polynomials(shape, steps, abc):
+    g = torch.Generator(device=DEV).manual_seed(3)
+    u = torch.randn(shape, device=DEV, generator=g)
+    near(optim.orthogonalize(u, steps, abc), u, torch.float32, steps, abc)
+
+
+@pytest.mark.parametrize('shape', [(12, 30), (150, 260)])
+def test_degenerate_matrices(shape):
+    """Zeros stay zeros, a matrix of rank one gets one singular value, magnitudes do not matter, what is not finite stays
+    in its matrix."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    u = torch.randn((4,) + shape, device=DEV, generator=g)
+    z = u.clone()
+    z[1] = 0
+    z[2] = torch.outer(u[2, :, 0], u[2, 0])
+    out = optim.orthogonalize(z)
+    assert float(out[1].abs().max()) == 0
+    near(out[2], z[2], torch.float32)
+    s = torch.linalg.svdvals(out[2].double().cpu())
+    assert 0.6 < float(s[0]) < 1.3 and float(s[1]) < 1e-3
+    assert torch.equal(out[0], optim.orthogonalize(u)[0])
+    near(optim.orthogonalize(u[0] * 1e-3, eps=1e-30), u[0], torch.float32)
+    near(optim.orthogonalize(u[0] * 2.0 ** -60, eps=1e-30), u[0], torch.float32)
+    near(optim.orthogonalize(u[0] * 2.0 ** 100), u[0], torch.float32)
+    big = (u[0] * 2.0 ** 120).bfloat16()
+    assert torch.equal(optim.orthogonalize(big), optim.orthogonalize((u[0] * 2.0 ** 20).bfloat16()))   # (a power of two)
+    # below eps the update shrinks instead of being raised from noise: X0 = u 1e-12 / 1e-3, and as far from 1 the
+    # polynomial is a X, five times.  Entries of 1e-9 x 2^15 are kept to half a subnormal step of a half, 2^-25: 2^-10 of them
+    small = optim.orthogonalize(u[0] * 1e-12, eps=1e-3)
+    want = optim.QUINTIC[0] ** 5 * 1e-9 * float(u[0].double().norm())
+    assert abs(float(small.double().norm()) - want) <= 2.0 ** -8 * want
+    for bad in (math.nan, math.inf):
+        w = u.clone()
+        w[3, 1, 1] = bad
+        o = optim.orthogonalize(w)
+        assert torch.equal(o[:3], optim.orthogonalize(u)[:3]) and not bool(torch.isfinite(o[3]).all())
+
+
+def test_orthogonalize_views_streams_and_empty():
+    u = torch.randn((60, 200), device=DEV)
+    want = optim.orthogonalize(u)
+    assert torch.equal(optim.orthogonalize(u.t().contiguous().t()), want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = optim.orthogonalize(u)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    assert optim.orthogonalize(torch.zeros((0, 3, 4), device=DEV)).shape == (0, 3, 4)
+    assert optim.orthogonalize(torch.zeros((2, 0, 4), device=DEV)).shape == (2, 0, 4)
+    for bad, word in (((u[0],), 'matrices'), ((u.double(),), 'float32'), ((u, 0), 'steps'), ((u, 5, (1.0, 2.0)), 'coefficients'),
+                      ((u, 5, optim.QUINTIC, 0.0), 'eps')):
+        with pytest.raises((RuntimeError, ValueError), match=word):
+            optim.orthogonalize(*bad)
+    with pytest.raises(RuntimeError, match='polynomial'):
+        optim.orthogonalize(u, 5, (9.0, 9.0, 9.0))
+
+
+def reference_step(w, g, m, lr, beta, decay, nesterov, batched=False):
+    w, g, m = w.double(), g.double(), m.double()
+    m = beta * m + g
+    u = g + beta * m if nesterov else m
+    mat = u if batched else u.reshape(u.shape[0], -1)
+    o = formula(mat)
+    return w * (1 - lr * decay) - lr * math.sqrt(max(1.0, mat.shape[-2] / mat.shape[-1])) * o.reshape(w.shape), m
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('nesterov', [True, False])
+def test_muon_steps(dtype, nesterov):
+    """Several steps over small, tiled, tall, convolution and odd weights, more than a launch's 32 matrices."""
+    g = torch.Generator(device=DEV).manual_seed(11)
+    shapes = [(64, 3), (64, 64), (32, 64), (128, 64, 3, 3), (200, 130), (700, 300), (5, 5), (1, 40), (40, 1), (96, 512, 1, 1)] + [(24, 31)] * 34
+    params = [torch.nn.Parameter(torch.randn(s, device=DEV, generator=g).to(dtype)) for s in shapes]
+    opt = optim.Muon(params, lr=0.05, momentum=0.9, weight_decay=0.1, nesterov=nesterov)
+    ref = [(p.detach().double(), torch.zeros_like(p, dtype=torch.float64)) for p in params]
+    for k in range(3):
+        for p in params:
+            p.grad = (torch.randn(p.shape, device=DEV, generator=g) * 1e-2).to(dtype)
+        before = [p.detach().clone() for p in params]
+        opt.step()
+        for i, p in enumerate(params):
+            w, m = reference_step(before[i], p.grad, ref[i][1], 0.05, 0.9, 0.1, nesterov)
+            ref[i] = (w, m)
+            e = torch.finfo(dtype).eps / 2
+            # the update's own error (see above) times lr, the rounding of W, and 4 roundings of 32 bits
+            tall = math.sqrt(max(1.0, p.shape[0] / (p.numel() // p.shape[0])))
+            tol = e * float(w.norm()) + 0.05 * tall * 341 * 8 * 2.0 ** -22 * 1.2 * math.sqrt(min(p.shape[0], p.numel() // p.shape[0])) + 4 * 2.0 ** -24 * float(w.norm())
+            assert float((p.detach().double() - w).norm()) <= tol, (shapes[i], k)
+            buf = opt.state[p]['momentum_buffer']
+            assert buf.dtype == torch.float32
+            assert float((buf.double() - m).norm()) <= (k + 1) * 2 * 2.0 ** -24 * float(m.norm()) * 2
+
+
+def test_muon_batched_absent_gradients_and_state():
+    g = torch.Generator(device=DEV).manual_seed(2)
+    z = torch.nn.Parameter(torch.randn((4, 15, 512), device=DEV, generator=g))
+    rest = torch.nn.Parameter(torch.randn((30, 20), device=DEV, generator=g))
+    opt = optim.Muon([z, rest], lr=0.1, momentum=0.5, batched=True)
+    z.grad = torch.randn(z.shape, device=DEV, generator=g)
+    w, _ = reference_step(z.detach(), z.grad, torch.zeros_like(z), 0.1, 0.5, 0.0, True, batched=True)
+    kept = rest.detach().clone()
+    opt.step()
+    assert torch.equal(rest.detach(), kept) and 'momentum_buffer' not in opt.state[rest]
+    assert float((z.detach().double() - w).norm()) <= 2.0 ** -20 * float(w.norm())
+    # a state that is saved and loaded goes on as the first one does, also where the parameters are of 16 bits
+    for dtype in (torch.float32, torch.bfloat16):
+        p = torch.nn.Parameter(torch.randn((40, 50), device=DEV, generator=g).to(dtype))
+        a = optim.Muon([p], lr=0.1)
+        p.grad = torch.randn((40, 50), device=DEV, generator=g).to(dtype)
+        a.step()
+        q = torch.nn.Parameter(p.detach().clone())
+        b = optim.Muon([q], lr=0.1)
+        b.load_state_dict(copy.deepcopy(a.state_dict()))
+        q.grad = p.grad = torch.randn((40, 50), device=DEV, generator=g).to(dtype)
+        a.step()
+        b.step()
+        assert torch.equal(p, q) and torch.equal(a.state[p]['momentum_buffer'], b.state[q]['momentum_buffer'])
+
+
+def test_muon_refusals_and_groups():
+    with pytest.raises(ValueError, match='two or more'):
+        optim.Muon([torch.nn.Parameter(torch.zeros(3, device=DEV))])
+    with pytest.raises(ValueError, match='momentum'):
+        optim.Muon([torch.nn.Parameter(torch.zeros((3, 3), device=DEV))], momentum=1.0)
+    p = torch.nn.Parameter(torch.zeros((3, 3)))
+    p.grad = torch.ones((3, 3))
+    with pytest.raises(RuntimeError, match='HIP devices only'):
+        optim.Muon([p]).step()
+    t = torch.nn.Parameter(torch.zeros((4, 3), device=DEV).t())
+    t.grad = torch.ones((3, 4), device=DEV)
+    with pytest.raises(RuntimeError, match='contiguous'):
+        optim.Muon([t]).step()
+    a, b = (torch.nn.Parameter(torch.ones((8, 8), device=DEV)) for _ in range(2))
+    opt = optim.Muon([{'params': [a], 'lr': 0.0}, {'params': [b], 'lr': 1.0}])
+    a.grad = b.grad = torch.eye(8, device=DEV)
+    opt.step()
+    assert torch.equal(a.detach(), torch.ones((8, 8), device=DEV)) and not torch.equal(a, b)
+
+
+def test_a_step_reaches_what_is_cached_by_version():
+    """EqualizedLinear keeps its scaled weight by the parameter's version: an evaluation after a step uses the new one."""
+    lin = EqualizedLinear(64, 64, bias=False).to(DEV)
+    x = torch.randn((5, 64), device=DEV)
+    with torch.no_grad():
+        before = lin(x)
+    opt = optim.Muon([lin.weight], lr=0.5)
+    lin(x).square().sum().backward()
+    opt.step()
+    lin.requires_grad_(False)
+    with torch.no_grad():
+        after = lin(x)
+        assert float((after - x @ (lin.weight * lin.weight_gain).t()).abs().max()) < 1e-4
+    assert float((after - before).abs().max()) > 1e-2
+
+
+def test_captured_step():
+    """Steps replayed from a graph equal eager ones on the same gradients, both kernels, between eager work."""
+    g = torch.Generator(device=DEV).manual_seed(4)
+    shapes = [(64, 64), (200, 300), (30, 512)]
+    p = [torch.nn.Parameter(torch.randn(s, device=DEV, generator=g)) for s in shapes]
+    q = [torch.nn.Parameter(v.detach().clone()) for v in p]
+    grads = [torch.randn(s, device=DEV, generator=g) for s in shapes]
+    oa, ob = optim.Muon(p, lr=0.1), optim.Muon(q, lr=0.1)
+    for v, w, d in zip(p, q, grads):
+        v.grad, w.grad = d, d
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        oa.step()
+    torch.cuda.current_stream().wait_stream(side)
+    ob.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        oa.step()
+    for k in range(4):
+        for d in grads:
+            d.copy_(torch.randn(d.shape, device=DEV, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        ob.step()
+        assert all(torch.equal(a, b) for a, b in zip(p, q)), k
+        assert all(torch.equal(oa.state[a]['momentum_buffer'], ob.state[b]['momentum_buffer']) for a, b in zip(p, q))

@@ -8,12 +8,13 @@ import subprocess
 import pytest
 import torch
 
-from nfi import _lib, grouped, norms
+from nfi import _lib, grouped, norms, optim
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
-@pytest.mark.parametrize('name,struct', [('nfi_resnorm_args', 'NfiResnormArgs'), ('nfi_grouped_args', 'NfiGroupedArgs')])
+@pytest.mark.parametrize('name,struct', [('nfi_resnorm_args', 'NfiResnormArgs'), ('nfi_grouped_args', 'NfiGroupedArgs'),
+                                         ('nfi_ortho_item', 'NfiOrthoItem'), ('nfi_ortho_args', 'NfiOrthoArgs')])
 def test_struct_layout(tmp_path, name, struct):
     py = getattr(_lib, struct)
     fields = [f[0] for f in py._fields_]
@@ -102,3 +103,45 @@ def test_row_tiles_cover_every_run(sizes, before, behind):
     rows = before + sum(sizes) + behind
     runs = sizes + [before, behind]
     assert sum(-(-r // 128) for r in runs) <= -(-rows // 128) + min(len(sizes) + 2, rows)
+
+
+def test_ortho_refuses():
+    with pytest.raises(RuntimeError, match='HIP devices only'):
+        optim.orthogonalize(torch.zeros(2, 4))
+    lib = _lib.load()
+    one = ctypes.c_void_p(16)
+
+    def args(item=None, **kw):
+        it = _lib.NfiOrthoItem(one, None, one, 4, 5, 1, 1.0)
+        for k, v in (item or {}).items():
+            setattr(it, k, v)
+        a = _lib.NfiOrthoArgs()
+        a.items, a.n_items, a.steps, a.eps = ctypes.pointer(it), 1, 5, 1e-7
+        a.a, a.b, a.c = optim.QUINTIC
+        for k, v in kw.items():
+            setattr(a, k, v)
+        a.keep = it
+        return a
+
+    for item, kw, word in (({}, {'n_items': 0}, b'no matrices'), ({}, {'g_type': 5}, b'type'), ({}, {'steps': 0}, b'steps'),
+                           ({}, {'steps': 65}, b'steps'), ({}, {'eps': 0.0}, b'eps'), ({'rows': 0}, {}, b'sides'),
+                           ({'cols': 262145}, {}, b'sides'), ({'count': 0}, {}, b'sides'), ({'count': 1 << 25}, {}, b'too large'),
+                           ({'g': None}, {}, b'null'), ({'w': None}, {}, b'null'), ({}, {'a': 50.0}, b'polynomial'),
+                           ({}, {'a': float('nan')}, b'polynomial'), ({}, {'a': 0.0, 'b': 0.0, 'c': 0.0}, b'polynomial'),
+                           ({'rows': 100, 'cols': 100}, {}, b'work')):
+        assert lib.nfi_ortho(ctypes.byref(args(item, **kw)), None) == -1, (item, kw)
+        assert word in lib.nfi_last_error(), (item, kw, lib.nfi_last_error())
+
+
+def test_ortho_work_is_that_of_the_largest_launch():
+    lib = _lib.load()
+
+    def bytes_of(shapes):
+        arr = (_lib.NfiOrthoItem * len(shapes))(*[_lib.NfiOrthoItem(16, None, 16, r, c, n, 1.0) for r, c, n in shapes])
+        return lib.nfi_ortho_work_bytes(arr, len(shapes))
+
+    assert bytes_of([(64, 64, 5), (15, 512, 32), (512, 15, 1)]) == 0
+    one = bytes_of([(200, 300, 1)])
+    assert one >= 2 * 256 * 384 * 4 + 2 * 256 * 256 * 4
+    assert bytes_of([(300, 200, 1)]) == one and bytes_of([(200, 300, 1)] * 32) == 32 * one
+    assert bytes_of([(200, 300, 1)] * 33) == 32 * one and bytes_of([(64, 64, 1), (200, 300, 1)]) == one
