@@ -37,26 +37,26 @@ extern "C" {
 
 /* x = scale (residual + gate . lrelu(norm(h) . weight + bias, slope));  y = next_norm(x) . next_weight
  * + next_bias, from the unrounded x.  h, residual, x, y and their gradients are [rows][width] of
- * `dtype`, contiguous; weight, bias, next_weight, next_bias [width] of `param_dtype`; gate
- * [gates][width] of `gate_dtype`, row r taking gate r / (rows / gates).  Absent (NULL): residual (0), gate,
- * weight, next_weight (1), bias, next_bias (0).  y exists when next_norm is not NFI_NORM_NONE.  stats
+ * `dtype`, contiguous.  `groups` equal runs of rows (0: none) take their own gate [groups][width] of
+ * `gate_dtype` (1: one for every row) and, with affine_groups, their own weight, bias, next_weight and
+ * next_bias [groups][width] of `param_dtype`; without it those are [width].  Absent (NULL): residual (0),
+ * gate, weight, next_weight (1), bias, next_bias (0).  y exists when next_norm is not NFI_NORM_NONE.  stats
  * [rows][4] floats (mean and 1/deviation of both norms) are written when not NULL and read by the
- * backward.  Backward: gx / gy may be NULL (zero gradients), and so may any output; dgate has gate's
- * shape and type, the d weights and d biases `param_dtype`; all sums in a fixed order. */
+ * backward.  Backward: gx / gy may be NULL (zero gradients), and so may any output; the parameters'
+ * gradients have their shapes and types; all sums in a fixed order. */
 typedef struct nfi_resnorm_args {
   const void *h, *residual, *gate, *weight, *bias, *next_weight, *next_bias;
   void *x, *y;
   float* stats;
   const void *gx, *gy;
   void *dh, *dresidual, *dgate, *dweight, *dbias, *dnext_weight, *dnext_bias;
-  float* work;          /* nfi_resnorm_work_bytes(rows, gates, width); backward only */
-  int64_t rows, gates;  /* gates: 0 without a gate; divides rows */
-  int32_t width, dtype, gate_dtype, param_dtype, norm, next_norm;
+  float* work;           /* nfi_resnorm_work_bytes(rows, groups, affine_groups, width); backward only */
+  int64_t rows, groups;  /* groups divides rows */
+  int32_t width, dtype, gate_dtype, param_dtype, norm, next_norm, affine_groups;
   float slope, scale, eps;
-  int32_t _pad;
 } nfi_resnorm_args;
 
-int64_t nfi_resnorm_work_bytes(int64_t rows, int64_t gates, int32_t width);
+int64_t nfi_resnorm_work_bytes(int64_t rows, int64_t groups, int32_t affine_groups, int32_t width);
 int32_t nfi_resnorm_forward(const nfi_resnorm_args* a, void* stream);
 int32_t nfi_resnorm_backward(const nfi_resnorm_args* a, void* stream);
 

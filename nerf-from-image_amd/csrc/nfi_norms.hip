@@ -50,7 +50,7 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float (*buf)[2][16], int
     constexpr int W = TPR / 64;
     if (lane_id() == 0) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) buf[turn][i][threadIdx.x >> 6] = v[i];
+      for (int i = 0; i < N; ++i) lds_st_fenced(&buf[turn][i][threadIdx.x >> 6], v[i]);
     }
     __syncthreads();
 #pragma unroll
@@ -140,11 +140,11 @@ __global__ void __launch_bounds__((TPR > 256 ? TPR : 256)) resnorm_fwd(const nfi
   int turn = 0;
   const int width = a.width;
   const float inv_d = 1.f / (float)width;
-  const int64_t per_gate = a.gates ? a.rows / a.gates : 1;
-  // rows of one wave at a time: the parameters are held in registers where that is cheap
-  constexpr bool KEEP = NC * R::V <= 8;
+  const int64_t per_gate = a.groups ? a.rows / a.groups : 1;
+  // the parameters are held in registers over the rows where that is cheap
+  const bool keep = NC * R::V <= 8 && !a.affine_groups;
   R w, b, w2, b2;
-  if constexpr (KEEP) {
+  if (keep) {
     w.load_param(a.weight, a.param_dtype, 0, width, 1.f);
     b.load_param(a.bias, a.param_dtype, 0, width, 0.f);
     if (a.next_norm) {
@@ -157,10 +157,11 @@ __global__ void __launch_bounds__((TPR > 256 ? TPR : 256)) resnorm_fwd(const nfi
     R x, res, gate;
     x.load(a.h, at, width);
     if (a.residual) res.load(a.residual, at, width);
-    if (a.gate) gate.load_param(a.gate, a.gate_dtype, gate_of(row, per_gate) * width, width, 1.f);
-    if constexpr (!KEEP) {
-      w.load_param(a.weight, a.param_dtype, 0, width, 1.f);
-      b.load_param(a.bias, a.param_dtype, 0, width, 0.f);
+    const int64_t group = a.groups > 1 ? gate_of(row, per_gate) : 0, param_at = a.affine_groups ? group * width : 0;
+    if (a.gate) gate.load_param(a.gate, a.gate_dtype, group * width, width, 1.f);
+    if (!keep) {
+      w.load_param(a.weight, a.param_dtype, param_at, width, 1.f);
+      b.load_param(a.bias, a.param_dtype, param_at, width, 0.f);
     }
     float mean, rstd, mean2 = 0.f, rstd2 = 1.f;
     statistics<R, TPR, NC>(x, a.norm, width, inv_d, a.eps, mean, rstd, buf, turn);
@@ -177,9 +178,9 @@ __global__ void __launch_bounds__((TPR > 256 ? TPR : 256)) resnorm_fwd(const nfi
     x.store(a.x, at, width);
     if (a.next_norm) {
       statistics<R, TPR, NC>(x, a.next_norm, width, inv_d, a.eps, mean2, rstd2, buf, turn);
-      if constexpr (!KEEP) {
-        w2.load_param(a.next_weight, a.param_dtype, 0, width, 1.f);
-        b2.load_param(a.next_bias, a.param_dtype, 0, width, 0.f);
+      if (!keep) {
+        w2.load_param(a.next_weight, a.param_dtype, param_at, width, 1.f);
+        b2.load_param(a.next_bias, a.param_dtype, param_at, width, 0.f);
       }
 #pragma unroll
       for (int c = 0; c < NC; ++c)
@@ -191,18 +192,20 @@ __global__ void __launch_bounds__((TPR > 256 ? TPR : 256)) resnorm_fwd(const nfi
   }
 }
 
-// Rows in segments: a segment is a piece of one gate's rows (`splits` pieces each), or all rows in
-// `splits` pieces without a gate.  A workgroup takes `per` consecutive segments; with several pieces
-// for each gate per is 1 and the gate's sum leaves as a partial, otherwise the workgroup holds whole gates.
+// Rows in segments: a segment is a piece of one group's rows (`splits` pieces each), or all rows in `splits` pieces
+// without groups.  A workgroup takes `per` consecutive segments; with several pieces for each group per is 1 and the
+// group's sums leave as partials, otherwise the workgroup holds whole groups.
 struct Plan {
   int64_t segments, per, rows_per_gate, rows_per_split;
   int splits, blocks;
 };
 
-__host__ inline Plan make_plan(int64_t rows, int64_t gates, int slots) {
+// (a gate for each row alone needs no sum)
+__host__ inline int64_t summed_groups(int64_t rows, int64_t groups, bool affine) { return groups > 0 && (groups < rows || affine) ? groups : 1; }
+
+__host__ inline Plan make_plan(int64_t rows, int64_t groups, bool affine, int slots) {
   Plan p;
-  const bool grouped = gates > 0 && gates < rows;   // (a gate for each row needs no sum)
-  const int64_t g = grouped ? gates : 1;
+  const int64_t g = summed_groups(rows, groups, affine);
   p.rows_per_gate = rows / g;
   const int64_t want = std::max<int64_t>(1, BLOCKS / g);
   const int64_t most = (p.rows_per_gate + slots - 1) / slots;
@@ -251,7 +254,7 @@ __global__ void __launch_bounds__((TPR > 256 ? TPR : 256)) resnorm_bwd(const nfi
   const int width = a.width;
   const float inv_d = 1.f / (float)width;
   const bool layer = a.norm == NFI_NORM_LAYER, layer2 = a.next_norm == NFI_NORM_LAYER;
-  const bool row_gate = a.gates == a.rows && a.gates > 0;
+  const bool row_gate = a.groups == a.rows && a.groups > 0 && !a.affine_groups;
   const bool gate_sum = a.gate && a.dgate && !row_gate;
   float acc[4][NC][R::V], accg[NC][R::V];
 #pragma unroll
@@ -274,14 +277,15 @@ __global__ void __launch_bounds__((TPR > 256 ? TPR : 256)) resnorm_bwd(const nfi
       if (a.gx) g.load(a.gx, at, width);
       if (a.gy) gy.load(a.gy, at, width);
       if (a.gate) gate.load_param(a.gate, a.gate_dtype, (row_gate ? row : gi) * width, width, 1.f);
-      w.load_param(a.weight, a.param_dtype, 0, width, 1.f);
+      const int64_t param_at = a.affine_groups ? gi * width : 0;
+      w.load_param(a.weight, a.param_dtype, param_at, width, 1.f);
       R b;
-      b.load_param(a.bias, a.param_dtype, 0, width, 0.f);
+      b.load_param(a.bias, a.param_dtype, param_at, width, 0.f);
       const float4 st = *reinterpret_cast<const float4*>(a.stats + 4 * row);
       // h becomes n, res becomes v (the gated value is scale (res + gate v))
       float s[2] = {0.f, 0.f};
       R w2;
-      if (a.gy) w2.load_param(a.next_weight, a.param_dtype, 0, width, 1.f);
+      if (a.gy) w2.load_param(a.next_weight, a.param_dtype, param_at, width, 1.f);
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -364,31 +368,46 @@ __global__ void __launch_bounds__((TPR > 256 ? TPR : 256)) resnorm_bwd(const nfi
         res.store(a.dh, at, width);
       }
     }
-    if (gate_sum && p.splits == 1) {   // a whole gate: its sum is final
+    // a whole group: its sums are final
+    if (p.splits == 1 && gate_sum) {
       slots_sum<R, TPR, NC>(accg, lds, width, [&](int col, float v) { store_typed(a.dgate, a.gate_dtype, gi * width + col, v); });
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int j = 0; j < R::V; ++j) accg[c][j] = 0.f;
     }
+    if (p.splits == 1 && a.affine_groups) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        void* out = k == 0 ? a.dweight : k == 1 ? a.dbias : k == 2 ? a.dnext_weight : a.dnext_bias;
+        if (out) slots_sum<R, TPR, NC>(acc[k], lds, width, [&](int col, float v) { store_typed(out, a.param_dtype, gi * width + col, v); });
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int j = 0; j < R::V; ++j) acc[k][c][j] = 0.f;
+      }
+    }
   }
   float* part = a.work + (int64_t)blockIdx.x * PARAMS * width;
-  if (a.dweight) slots_sum<R, TPR, NC>(acc[0], lds, width, [&](int col, float v) { part[col] = v; });
-  if (a.dbias) slots_sum<R, TPR, NC>(acc[1], lds, width, [&](int col, float v) { part[width + col] = v; });
-  if (a.dnext_weight) slots_sum<R, TPR, NC>(acc[2], lds, width, [&](int col, float v) { part[2 * width + col] = v; });
-  if (a.dnext_bias) slots_sum<R, TPR, NC>(acc[3], lds, width, [&](int col, float v) { part[3 * width + col] = v; });
+  if (p.splits > 1 || !a.affine_groups) {
+    if (a.dweight) slots_sum<R, TPR, NC>(acc[0], lds, width, [&](int col, float v) { part[col] = v; });
+    if (a.dbias) slots_sum<R, TPR, NC>(acc[1], lds, width, [&](int col, float v) { part[width + col] = v; });
+    if (a.dnext_weight) slots_sum<R, TPR, NC>(acc[2], lds, width, [&](int col, float v) { part[2 * width + col] = v; });
+    if (a.dnext_bias) slots_sum<R, TPR, NC>(acc[3], lds, width, [&](int col, float v) { part[3 * width + col] = v; });
+  }
   if (gate_sum && p.splits > 1) slots_sum<R, TPR, NC>(accg, lds, width, [&](int col, float v) { part[4 * width + col] = v; });
 }
 
-// The workgroups' partials summed in their order, 16 columns x 64 slices of workgroups at a time: blockIdx.y < 4 the
-// parameters over all workgroups, then each gate over its own
+// The workgroups' partials summed in their order, 16 columns x 64 slices of workgroups at a time: blockIdx.y the
+// parameter (4: the gate), blockIdx.z the group (its own workgroups), or 0 for parameters of all rows
 __global__ void __launch_bounds__(1024) resnorm_join(const nfi_resnorm_args a, const Plan p) {
   __shared__ float lds[64][17];
-  const int which = blockIdx.y < 4 ? blockIdx.y : 4;
+  const int which = blockIdx.y;
   void* out = which == 0 ? a.dweight : which == 1 ? a.dbias : which == 2 ? a.dnext_weight : which == 3 ? a.dnext_bias : a.dgate;
-  if (out == nullptr) return;
-  const int64_t gi = blockIdx.y - 4;
-  const int first = which < 4 ? 0 : (int)(gi * p.splits), count = which < 4 ? p.blocks : p.splits;
+  const bool grouped = which == 4 || a.affine_groups;
+  const int64_t gi = blockIdx.z;
+  if (out == nullptr || (!grouped && gi > 0) || (grouped && p.splits == 1)) return;
+  const int first = grouped ? (int)(gi * p.splits) : 0, count = grouped ? p.splits : p.blocks;
   const int col = blockIdx.x * 16 + (threadIdx.x & 15), slice = threadIdx.x >> 4;
   float s = 0.f;
   if (col < a.width) {
@@ -402,7 +421,7 @@ __global__ void __launch_bounds__(1024) resnorm_join(const nfi_resnorm_args a, c
     float t = 0.f;
 #pragma unroll 16
     for (int k = 0; k < 64; ++k) t += lds[k][threadIdx.x & 15];
-    store_typed(out, which < 4 ? a.param_dtype : a.gate_dtype, (which < 4 ? 0 : gi * a.width) + col, t);
+    store_typed(out, which < 4 ? a.param_dtype : a.gate_dtype, gi * a.width + col, t);
   }
 }
 
@@ -414,11 +433,13 @@ static void launch(const nfi_resnorm_args& a, bool backward, hipStream_t s) {
     resnorm_fwd<T, V, TPR, NC, EXACT><<<(unsigned)std::min<int64_t>(need, 8192), R::BLK, 0, s>>>(a);
     return;
   }
-  const Plan p = make_plan(a.rows, a.gates, R::SLOTS);
+  const Plan p = make_plan(a.rows, a.groups, a.affine_groups, R::SLOTS);
   resnorm_bwd<T, V, TPR, NC, EXACT><<<(unsigned)p.blocks, R::BLK, 0, s>>>(a, p);
-  const bool gate_sum = a.dgate && a.gates < a.rows && p.splits > 1;
-  if (a.dweight || a.dbias || a.dnext_weight || a.dnext_bias || gate_sum)
-    resnorm_join<<<dim3((unsigned)((a.width + 15) / 16), (unsigned)(4 + (gate_sum ? a.gates : 0))), 1024, 0, s>>>(a, p);
+  const bool params = (a.dweight || a.dbias || a.dnext_weight || a.dnext_bias) && (p.splits > 1 || !a.affine_groups);
+  const bool gate = a.dgate && (a.groups < a.rows || a.affine_groups) && p.splits > 1;
+  const bool each = gate || (params && a.affine_groups);   // (a group's own sums: fewer than BLOCKS groups)
+  if (params || gate)
+    resnorm_join<<<dim3((unsigned)((a.width + 15) / 16), gate ? 5 : 4, (unsigned)(each ? a.groups : 1)), 1024, 0, s>>>(a, p);
 }
 
 template <class T, int TPR, int NC>
@@ -450,8 +471,8 @@ static int check(const nfi_resnorm_args* a, const char* what) {
               (long long)a->rows, a->width, NFI_RESNORM_MAX_WIDTH);
   NFI_REQUIRE(type_ok(a->dtype) && type_ok(a->param_dtype) && type_ok(a->gate_dtype), "%s: bad type", what);
   NFI_REQUIRE(a->norm >= 0 && a->norm <= 2 && a->next_norm >= 0 && a->next_norm <= 2, "%s: bad norm kind", what);
-  NFI_REQUIRE((a->gate != nullptr) == (a->gates > 0) && (a->gates == 0 || a->rows % a->gates == 0),
-              "%s: %lld gates for %lld rows", what, (long long)a->gates, (long long)a->rows);
+  NFI_REQUIRE(a->groups >= 0 && ((a->gate == nullptr && !a->affine_groups) || a->groups > 0) && (a->groups == 0 || a->rows % a->groups == 0),
+              "%s: %lld groups of %lld rows", what, (long long)a->groups, (long long)a->rows);
   NFI_REQUIRE(a->eps >= 0.f, "%s: eps %g", what, (double)a->eps);
   return NFI_OK;
 }
@@ -469,10 +490,10 @@ using namespace nfi::learn;
 
 extern "C" {
 
-int64_t nfi_resnorm_work_bytes(int64_t rows, int64_t gates, int32_t width) {
-  if (rows <= 0 || gates < 0 || width <= 0) return 0;
+int64_t nfi_resnorm_work_bytes(int64_t rows, int64_t groups, int32_t affine_groups, int32_t width) {
+  if (rows <= 0 || groups < 0 || width <= 0) return 0;
   // (the plan's workgroups, whatever number of rows one holds)
-  const int64_t g = gates > 0 && gates < rows ? gates : 1;
+  const int64_t g = summed_groups(rows, groups, affine_groups != 0);
   const int64_t blocks = g >= BLOCKS ? BLOCKS : g * std::max<int64_t>(1, BLOCKS / g);
   return blocks * PARAMS * (int64_t)width * 4;
 }

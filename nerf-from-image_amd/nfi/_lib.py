@@ -61,10 +61,10 @@ class NfiResnormArgs(ctypes.Structure):
     _fields_ = [(n, c_void_p) for n in ('h', 'residual', 'gate', 'weight', 'bias', 'next_weight', 'next_bias', 'x', 'y',
                                         'stats', 'gx', 'gy', 'dh', 'dresidual', 'dgate', 'dweight', 'dbias',
                                         'dnext_weight', 'dnext_bias', 'work')] + [
-        ('rows', ctypes.c_int64), ('gates', ctypes.c_int64), ('width', ctypes.c_int32), ('dtype', ctypes.c_int32),
+        ('rows', ctypes.c_int64), ('groups', ctypes.c_int64), ('width', ctypes.c_int32), ('dtype', ctypes.c_int32),
         ('gate_dtype', ctypes.c_int32), ('param_dtype', ctypes.c_int32), ('norm', ctypes.c_int32),
-        ('next_norm', ctypes.c_int32), ('slope', ctypes.c_float), ('scale', ctypes.c_float), ('eps', ctypes.c_float),
-        ('_pad', ctypes.c_int32)]
+        ('next_norm', ctypes.c_int32), ('affine_groups', ctypes.c_int32), ('slope', ctypes.c_float),
+        ('scale', ctypes.c_float), ('eps', ctypes.c_float)]
 
 
 class NfiGroupedArgs(ctypes.Structure):
@@ -231,7 +231,7 @@ SIGNATURES = {
     'nfi_dconv3x3': (ctypes.c_int32, [c_void_p] * 10 + [ctypes.c_int32] * 5 + [c_void_p]),
     'nfi_absmax_scaled_slots': (ctypes.c_int32, [c_void_p, c_void_p] + [ctypes.c_int32] * 3 + [c_void_p, c_void_p]),
     # include/nfi_learn.h
-    'nfi_resnorm_work_bytes': (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32]),
+    'nfi_resnorm_work_bytes': (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32]),
     'nfi_resnorm_forward': (ctypes.c_int32, [ctypes.POINTER(NfiResnormArgs), c_void_p]),
     'nfi_resnorm_backward': (ctypes.c_int32, [ctypes.POINTER(NfiResnormArgs), c_void_p]),
     'nfi_grouped_forward_work_bytes': (ctypes.c_int64, [ctypes.POINTER(NfiGroupedArgs)]),

@@ -235,6 +235,10 @@ class InversionConfig:
                                          # 'foreach' (torch's default on CUDA, the reference's run.py:2007):
                                          # the same update formula, rounded differently at ulp level
                                          # (tests/test_gpu_inversion.py bounds the trajectories' distance)
+    latent_update: str = 'adam'          # 'muon' (GPU): the latent's update orthogonalised for each image
+                                         # (nfi.optim.Muon, momentum betas[0]); the pose stays with Adam
+    latent_lr: Optional[float] = None    # 'muon': length of the latent's step; None: lr sqrt(512), whose entries
+                                         # are as large on average as Adam's first steps
 
 
 @dataclass
@@ -437,8 +441,18 @@ class _State:
         if cfg.adam not in ('fused', 'foreach'):
             raise ValueError(f"InversionConfig.adam must be 'fused' or 'foreach', not {cfg.adam!r}")
         fused = bool(params[0].is_cuda) and cfg.adam == 'fused'
-        self.opt = torch.optim.Adam(params, lr=cfg.lr, betas=cfg.betas, capturable=capturable,
-                                    **({'fused': True} if fused else {}))
+        if cfg.latent_update not in ('adam', 'muon'):
+            raise ValueError(f"InversionConfig.latent_update must be 'adam' or 'muon', not {cfg.latent_update!r}")
+        muon = cfg.latent_update == 'muon'
+        self.opts = []
+        if muon:
+            from .optim import Muon
+            lr = cfg.lr * math.sqrt(max(self.z_.shape[-2:])) if cfg.latent_lr is None else cfg.latent_lr
+            self.opts.append(Muon([self.z_], lr=lr, momentum=cfg.betas[0], batched=True))
+        rest = params[1:] if muon else params
+        if rest:
+            self.opts.append(torch.optim.Adam(rest, lr=cfg.lr, betas=cfg.betas, capturable=capturable,
+                                              **({'fused': True} if fused else {})))
         self.target = target_img[..., :3]
         if capturable:
             # a private static buffer: later batches are copied into it (load), which must never
@@ -472,12 +486,10 @@ class _State:
             for dst, src in ((self.center, center), (self.bbox, bbox)):
                 if dst is not None:
                     dst.copy_(src)
-            for p in self.params:
-                state = self.opt.state.get(p)
-                if state:
-                    state['step'].zero_()
-                    state['exp_avg'].zero_()
-                    state['exp_avg_sq'].zero_()
+            for opt in self.opts:
+                for state in opt.state.values():
+                    for v in state.values():
+                        v.zero_()
 
     def step(self, rfn, kw):
         """One step (run.py:2256-2310): producer + render, loss, backward, Adam, projections.
@@ -502,8 +514,9 @@ class _State:
                 t.record_stream(main)
         loss = image_loss(cfg.loss, rgb, self.target, self.lpips_net, cfg.white_background, prepared=prepared)
         loss.backward()
-        self.opt.step()
-        self.opt.zero_grad()
+        for opt in self.opts:
+            opt.step()
+            opt.zero_grad()
         project_pose(self.z0_, self.s_, self.q_)
         return loss
 

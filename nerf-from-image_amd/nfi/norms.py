@@ -28,10 +28,11 @@ def _args(h, residual, gate, weight, bias, next_weight, next_bias, conf):
     a.h, a.residual, a.gate, a.weight, a.bias = map(lo.ptr, (h, residual, gate, weight, bias))
     a.next_weight, a.next_bias = lo.ptr(next_weight), lo.ptr(next_bias)
     a.rows, a.width = h.shape
-    a.gates = 0 if gate is None else gate.shape[0]
+    p = next((t for t in (weight, bias, next_weight, next_bias) if t is not None), h)
+    a.affine_groups = p is not h and p.dim() == 2
+    a.groups = gate.shape[0] if gate is not None else p.shape[0] if a.affine_groups else 0
     a.dtype = lo.TYPES[h.dtype]
     a.gate_dtype = a.dtype if gate is None else lo.TYPES[gate.dtype]
-    p = next((t for t in (weight, bias, next_weight, next_bias) if t is not None), h)
     a.param_dtype = lo.TYPES[p.dtype]
     a.norm, a.next_norm, a.slope, a.scale, a.eps = norm, next_norm, slope, scale, eps
     return a
@@ -74,7 +75,7 @@ class _ResidualNorm(torch.autograd.Function):
         a.stats, a.gx, a.gy = lo.ptr(stats), lo.ptr(gx), lo.ptr(gy)
         a.dh, a.dresidual, a.dgate, a.dweight, a.dbias = map(lo.ptr, out[:5])
         a.dnext_weight, a.dnext_bias = (lo.ptr(out[k]) if gy is not None else None for k in (5, 6))
-        size = _lib.load().nfi_resnorm_work_bytes(a.rows, a.gates, a.width)
+        size = _lib.load().nfi_resnorm_work_bytes(a.rows, a.groups, a.affine_groups, a.width)
         work = torch.empty((size,), device=h.device, dtype=torch.uint8)
         a.work = lo.ptr(work)
         with lo.on(h.device):
@@ -90,10 +91,10 @@ def residual_norm(h: torch.Tensor, residual: Optional[torch.Tensor] = None, gate
 
         x = scale * (residual + gate * leaky_relu(norm(h) * weight + bias, slope)),  y = next_norm(x) * next_weight + next_bias
 
-    `norm` and `next_norm`: 'layer', 'rms' or None.  residual: h's shape and type.  weight, bias, next_weight,
-    next_bias: [D], all of one type.  gate: [D], or [G, D] where G divides the number of rows and row r takes gate
-    r // (rows / G) (rows of an image side by side: one gate for each image; G = rows: a gate for each row).
-    Statistics and sums are held in 32 bits and every output is rounded once; y is taken from x before its rounding.
+    `norm` and `next_norm`: 'layer', 'rms' or None.  residual: h's shape and type.  gate: [D], or [G, D] where G divides
+    the number of rows and row r takes gate r // (rows / G) (an image's rows side by side: one gate for each image; G = rows:
+    a gate for each row).  weight, bias, next_weight, next_bias: all [D], or all [G, D] with the gate's G (a conditional
+    norm: each image's own), all of one type.  Statistics and sums are held in 32 bits and every output is rounded once; y is taken from x before its rounding.
     Gradients reach every tensor argument, in a fixed order of summation (no double backward)."""
     what = 'residual_norm'
     lo.same_device(what, h, residual=residual, gate=gate, weight=weight, bias=bias, next_weight=next_weight,
@@ -108,26 +109,32 @@ def residual_norm(h: torch.Tensor, residual: Optional[torch.Tensor] = None, gate
         raise ValueError(f'{what}: residual is {tuple(residual.shape)} {residual.dtype}, h {tuple(h.shape)} {h.dtype}')
     if next_norm is None and (next_weight is not None or next_bias is not None):
         raise ValueError(f'{what}: next_weight and next_bias need next_norm')
-    kind = None
+    rows = h.numel() // d
+    first = None
     for name, t in (('weight', weight), ('bias', bias), ('next_weight', next_weight), ('next_bias', next_bias)):
         if t is None:
             continue
         lo.type_code(t, f'{what}: {name}')
-        if t.shape != (d,) or (kind is not None and t.dtype != kind):
-            raise ValueError(f'{what}: {name} is {tuple(t.shape)} {t.dtype}; [{d}] is wanted, all of one type')
-        kind = t.dtype
+        fits = t.shape == (d,) or (t.dim() == 2 and t.shape[1] == d and t.shape[0] >= 1 and rows % t.shape[0] == 0)
+        if not fits or (first is not None and (t.dtype != first.dtype or t.shape != first.shape)):
+            raise ValueError(f'{what}: {name} is {tuple(t.shape)} {t.dtype}; [{d}], or [G, {d}] with G a divisor of {rows} '
+                             'rows is wanted, all of one shape and type')
+        first = t
     if eps < 0:
         raise ValueError(f'{what}: eps {eps}')
-    shape, rows = h.shape, h.numel() // d
+    shape = h.shape
+    affine = first is not None and first.dim() == 2
     if gate is not None:
         lo.type_code(gate, f'{what}: gate')
         if gate.dim() == 1:
             gate = gate[None]
         if gate.dim() != 2 or gate.shape[1] != d or gate.shape[0] < 1 or rows % gate.shape[0]:
             raise ValueError(f'{what}: gate is {tuple(gate.shape)}; [{d}] or [G, {d}] with G a divisor of {rows} rows is wanted')
+        if affine and gate.shape[0] != first.shape[0]:
+            if gate.shape[0] != 1:
+                raise ValueError(f'{what}: {gate.shape[0]} gates and {first.shape[0]} groups of parameters')
+            gate = gate.expand(first.shape[0], d)
         gate = gate.contiguous()
-        if rows == 0:
-            gate = gate[:1]
     conf = (KINDS[norm], KINDS[next_norm], float(slope), float(scale), float(eps))
     flat = [None if t is None else t.reshape(rows, d).contiguous() for t in (h, residual)]
     params = [None if t is None else t.contiguous() for t in (weight, bias, next_weight, next_bias)]

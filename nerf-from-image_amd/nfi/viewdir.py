@@ -15,6 +15,10 @@ from __future__ import annotations
 import math
 
 import torch
+import torch.nn.functional as F
+
+from .grouped import grouped_linear
+from .norms import residual_norm
 
 
 def viewdir_trunk(mapper, viewdir: torch.Tensor) -> torch.Tensor:
@@ -60,3 +64,40 @@ class ViewDirectionMapper(torch.nn.Module):
 
     def forward(self, viewdir):
         return viewdir_trunk(self, viewdir)
+
+
+class ViewDirectionMapperBank(torch.nn.Module):
+    """Several mappers' trunks over one batch of rays: image b's rays go through mapper `mapper_of_image[b]` (a batch that
+    mixes categories, each with a mapper of its own).  The layers are viewdir_trunk's, all mappers in each launch: grouped
+    products (nfi.grouped) and one fused norm, activation and shortcut for each (nfi.norms), the norms' weights taken image
+    by image.  Gradients reach the mappers' own parameters and viewdir."""
+
+    def __init__(self, mappers):
+        super().__init__()
+        self.mappers = torch.nn.ModuleList(mappers)
+
+    def _linear(self, name, x, offsets):
+        layers = [getattr(m, name) for m in self.mappers]
+        w = torch.stack([m.weight for m in layers]) * layers[0].weight_gain
+        b = None if layers[0].bias is None else torch.stack([m.bias for m in layers]) * layers[0].bias_gain
+        return grouped_linear(x, w, offsets, b)
+
+    def _norm(self, name, h, image, shortcut=None):
+        layers = [getattr(m, name) for m in self.mappers]
+        w, b = (torch.stack([getattr(n, k) for n in layers])[image] for k in ('weight', 'bias'))
+        return residual_norm(h, shortcut, None, w, b, slope=0.2, scale=1.0 if shortcut is None else math.sqrt(2) / 2,
+                             eps=layers[0].eps)
+
+    def forward(self, viewdir: torch.Tensor, mapper_of_image: torch.Tensor) -> torch.Tensor:
+        """viewdir [images, rays, 3], mapper_of_image [images] int64 on the device, not decreasing -> [images, rays, 32]."""
+        images, rays = viewdir.shape[:2]
+        if mapper_of_image.shape != (images,) or mapper_of_image.dtype != torch.int64:
+            raise ValueError(f'mapper_of_image [{images}] int64 is wanted, not {tuple(mapper_of_image.shape)} {mapper_of_image.dtype}')
+        ends = torch.arange(len(self.mappers) + 1, device=viewdir.device)
+        offsets = torch.searchsorted(mapper_of_image.contiguous(), ends) * rays
+        x = F.leaky_relu(self._linear('fc0', viewdir.reshape(images * rays, 3), offsets), 0.2)
+        for a, b in ((1, 2), (3, 4)):
+            h = self._norm(f'norm{a}', self._linear(f'fc{a}', x, offsets), mapper_of_image)
+            x = self._norm(f'norm{b}', self._linear(f'fc{b}', h, offsets), mapper_of_image, shortcut=x)
+        x = F.leaky_relu(self._linear('fc5', x, offsets), 0.2)
+        return self._linear('fc6', x, offsets).view(images, rays, -1)

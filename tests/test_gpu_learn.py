@@ -1,0 +1,106 @@
+"""The operators that train the field's heads, used together: a bank of view-direction mappers over a batch that mixes
+categories, against each mapper's own trunk (viewdir_trunk in 64 bits), its gradients, steps of its weights by Muon, and
+the inversion loop with orthogonalised latent updates."""
+
+import copy
+
+import pytest
+import torch
+
+import nfi
+from nfi import inversion, optim
+from nfi.viewdir import ViewDirectionMapper, ViewDirectionMapperBank, viewdir_trunk
+from test_producer import inversion_setup
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device('cuda:0')
+U = 2.0 ** -24
+
+
+def bank(count, seed=0):
+    torch.manual_seed(seed)
+    mappers = [ViewDirectionMapper(10).to(DEV) for _ in range(count)]
+    for m in mappers:
+        for k in range(1, 5):
+            with torch.no_grad():
+                getattr(m, f'norm{k}').weight.add_(torch.randn(64, device=DEV) * 0.1)
+                getattr(m, f'norm{k}').bias.add_(torch.randn(64, device=DEV) * 0.1)
+    return ViewDirectionMapperBank(mappers)
+
+
+@pytest.mark.parametrize('which', [[0, 0, 1, 2], [0], [1, 1, 3], [2, 2, 2]])
+def test_bank_against_each_trunk(which):
+    """Depth: 7 products (longest sum 64) and 4 norms, each amplifying what it gets by at most its row's 1 / deviation (about
+    1 to 4 here): 2^9 u of the largest value is 7 layers' own errors times that, with room."""
+    b = bank(4)
+    rays = 133
+    v = torch.nn.functional.normalize(torch.randn((len(which), rays, 3), device=DEV), dim=-1).requires_grad_()
+    image = torch.tensor(which, device=DEV)
+    x = b(v, image)
+    g = torch.randn_like(x)
+    params = dict(b.named_parameters())
+    used = [k for k in params if 'output' not in k]
+    got = torch.autograd.grad(x, [v] + [params[k] for k in used], g)
+    b64 = copy.deepcopy(b).double()
+    v64 = v.detach().double().requires_grad_()
+    ref = torch.stack([viewdir_trunk(b64.mappers[m], v64[i].unsqueeze(-2)).squeeze(-2) for i, m in enumerate(which)])
+    params64 = dict(b64.named_parameters())
+    want = torch.autograd.grad(ref, [v64] + [params64[k] for k in used], g.double(), allow_unused=True)
+    assert float((x.double() - ref).abs().max()) <= 2 ** 9 * U * max(1.0, float(ref.abs().max()))
+    for k, a, w in zip(['viewdir'] + used, got, want):
+        if w is None:
+            assert float(a.abs().max()) == 0, k     # a mapper that no image went through
+        else:
+            # (by norm; sums over up to 400 rows, and the slope's steps at zero are the same on both sides for these seeds)
+            assert float((a.double() - w).norm()) <= 2 ** 11 * U * float(w.norm()) + 1e-12, k
+
+
+def test_training_steps_of_a_bank():
+    """Two steps by Muon on the mappers' matrices: each weight moves as the formula says for its gradient."""
+    b = bank(3, 1)
+    image = torch.tensor([0, 1, 1, 2], device=DEV)
+    v = torch.nn.functional.normalize(torch.randn((4, 200, 3), device=DEV), dim=-1)
+    target = torch.randn((4, 200, 32), device=DEV)
+    weights = [p for k, p in b.named_parameters() if p.dim() == 2 and 'output' not in k]
+    opt = optim.Muon(weights, lr=0.02)
+    for _ in range(2):
+        opt.zero_grad()
+        (b(v, image) - target).square().mean().backward()
+        before = [w.detach().clone() for w in weights]
+        state = [opt.state[w]['momentum_buffer'].clone() if w in opt.state else torch.zeros_like(w) for w in weights]
+        opt.step()
+        for w, old, m in zip(weights, before, state):
+            m = 0.95 * m + w.grad
+            o = optim.orthogonalize(w.grad + 0.95 * m)
+            tall = max(1.0, w.shape[0] / w.shape[1]) ** 0.5
+            assert float((w.detach() - (old - 0.02 * tall * o)).abs().max()) <= 1e-5
+
+
+def test_bank_refuses():
+    b = bank(2)
+    with pytest.raises(ValueError, match='mapper_of_image'):
+        b(torch.zeros((2, 5, 3), device=DEV), torch.zeros((3,), device=DEV, dtype=torch.int64))
+    with pytest.raises(ValueError, match='mapper_of_image'):
+        b(torch.zeros((2, 5, 3), device=DEV), torch.zeros((2,), device=DEV, dtype=torch.int32))
+
+
+@pytest.mark.parametrize('graph', [False, True])
+def test_inversion_with_orthogonalised_latent_steps(graph):
+    """InversionConfig.latent_update = 'muon': each image's latent moves by an orthogonalised step of the given length, the
+    pose as with Adam; eager and replayed, twice over the same graph."""
+    gen, d, meta, cfg = inversion_setup(DEV)
+    nfi.configure(scene_range=float(meta['scene_range']), white_background=False, fine_sampling=True, use_sdf=True,
+                  attention_values=10, use_viewdir=False)
+    cfg.latent_update, cfg.latent_lr, cfg.steps, cfg.graph = 'muon', 0.05, 4, graph
+    for _ in range(2):
+        seen = [d['w_init'].to(DEV).expand(d['target'].shape[0], -1, -1).clone()]
+        res = inversion.invert(gen, d['target'], d['cam0'], d['focal0'], d['w_init'], cfg, checkpoints=(1, 2, 3, 4),
+                               on_checkpoint=lambda it, v: seen.append(v[0].detach().clone() * cfg.gain_z))
+        assert len(res.losses) == 4 and all(torch.isfinite(torch.tensor(res.losses)))
+        for a, c in zip(seen, seen[1:]):
+            step = (c - a) / cfg.gain_z / 0.05                      # 15 x 512: singular values near 1 where the gradient has any
+            s = torch.linalg.svdvals(step.double().cpu())
+            assert float(s.max()) < 1.3 and float(s[:, 0].min()) > 0.6
+    cfg.latent_update = 'sgd'
+    with pytest.raises(ValueError, match='latent_update'):
+        inversion.invert(gen, d['target'], d['cam0'], d['focal0'], d['w_init'], cfg)

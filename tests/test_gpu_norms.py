@@ -183,6 +183,49 @@ def test_mixed_parameter_types_and_broadcast_gate():
         assert float((a.double() - b).norm()) <= e * float(b.norm()) + 128 * U * 50 * (1 + float(b.norm())), name
 
 
+@pytest.mark.parametrize('rows,groups,width,gate', [(4, 4, 512, True), (12, 3, 40, False), (600, 2, 64, True), (1, 1, 9, True),
+                                                    (2048, 1024, 72, True), (4096, 4, 130, False)])
+def test_parameters_of_groups(rows, groups, width, gate):
+    """Each group of rows with its own weight, bias and next norm (a conditional norm), some gradients left out."""
+    g = torch.Generator(device=DEV).manual_seed(rows)
+
+    def rnd(*shape, shift=0.0):
+        return (torch.randn(shape, device=DEV, generator=g) * 0.3 + shift).requires_grad_()
+    p = {'h': rnd(rows, width), 'residual': rnd(rows, width), 'gate': rnd(groups, width, shift=1) if gate else None,
+         'weight': rnd(groups, width, shift=1), 'bias': rnd(groups, width), 'next_weight': rnd(groups, width, shift=1),
+         'next_bias': rnd(groups, width)}
+    p64 = {k: None if v is None else v.detach().double().requires_grad_() for k, v in p.items()}
+    spread = {k: (v if v is None or k in ('h', 'residual', 'gate') else v.repeat_interleave(rows // groups, 0)) for k, v in p64.items()}
+    x, y = run(p, 'layer', 'rms', 1.0, 0.7)
+    rx, ry = formula(spread, 'layer', 'rms', 1.0, 0.7)
+    near(x.detach(), rx.detach(), torch.float32, 8)
+    near(y.detach(), ry.detach(), torch.float32, 32)
+    gx, gy = torch.randn((rows, width), device=DEV, generator=g), torch.randn((rows, width), device=DEV, generator=g)
+    keys = [k for k in NAMES if p[k] is not None]
+    got = torch.autograd.grad([x, y], [p[k] for k in keys], [gx, gy], retain_graph=True)
+    ref = torch.autograd.grad([rx, ry], [p64[k] for k in keys], [gx.double(), gy.double()])
+    for k, a, b in zip(keys, got, ref):
+        assert float((a.double() - b).norm()) <= (64 + rows / 16) * U * 16 * float(b.norm()), k
+    some = torch.autograd.grad([x, y], [p['bias'], p['next_weight']], [gx, gy])
+    assert torch.equal(some[0], got[keys.index('bias')]) and torch.equal(some[1], got[keys.index('next_weight')])
+
+
+def test_refusals():
+    h = torch.zeros((6, 8), device=DEV)
+    w = torch.ones((8,), device=DEV)
+    for kw, word in ((dict(norm='batch'), 'norms are'), (dict(residual=h[:3]), 'residual'), (dict(residual=h.half()), 'residual'),
+                     (dict(weight=w[:7]), 'weight'), (dict(weight=w, bias=w.half()), 'bias'), (dict(next_weight=w), 'next_norm'),
+                     (dict(gate=torch.ones((4, 8), device=DEV)), 'gate'), (dict(weight=torch.ones((4, 8), device=DEV)), 'weight'),
+                     (dict(weight=torch.ones((2, 8), device=DEV), gate=torch.ones((3, 8), device=DEV)), 'gates'),
+                     (dict(eps=-1.0), 'eps'), (dict(weight=w.double()), 'float32'), (dict(weight=w.cpu()), 'cpu')):
+        with pytest.raises((RuntimeError, ValueError), match=word):
+            norms.residual_norm(h, **kw)
+    with pytest.raises(RuntimeError, match='float32'):
+        norms.residual_norm(h.double())
+    with pytest.raises(ValueError, match='rows of 1'):
+        norms.residual_norm(torch.zeros((1, 8193), device=DEV))
+
+
 def test_partial_gradients_and_one_output():
     """A gradient for one output, or for one argument, gives what the whole gives in that place."""
     p = {k: v.requires_grad_() for k, v in inputs(24, 72, torch.float32, 4, True, 4).items()}

@@ -46,7 +46,7 @@ def test_resnorm_entry_refuses_bad_arguments():
 
     for kw, word in (({'h': None}, b'null input'), ({'rows': 0}, b'rows'), ({'width': 8193}, b'width'),
                      ({'dtype': 7}, b'type'), ({'norm': 3}, b'norm'), ({'next_norm': -1}, b'norm'),
-                     ({'gate': one, 'gates': 3}, b'gates'), ({'gates': 2}, b'gates'), ({'eps': -1.0}, b'eps'),
+                     ({'gate': one, 'groups': 3}, b'groups'), ({'gate': one}, b'groups'), ({'affine_groups': 1}, b'groups'), ({'eps': -1.0}, b'eps'),
                      ({'x': None}, b'null output'), ({'next_norm': 1}, b'null output')):
         assert lib.nfi_resnorm_forward(ctypes.byref(args(**kw)), None) == -1, kw
         assert word in lib.nfi_last_error(), (kw, lib.nfi_last_error())
@@ -56,18 +56,19 @@ def test_resnorm_entry_refuses_bad_arguments():
         assert word in lib.nfi_last_error(), kw
 
 
-@pytest.mark.parametrize('rows,gates', [(1, 0), (1, 1), (7, 7), (10 ** 6, 0), (10 ** 6, 2), (4096, 512), (4096, 2048), (511 * 3, 511)])
-def test_resnorm_work_holds_every_workgroup(rows, gates):
+@pytest.mark.parametrize('affine', [0, 1])
+@pytest.mark.parametrize('rows,groups', [(1, 0), (1, 1), (7, 7), (10 ** 6, 0), (10 ** 6, 2), (4096, 512), (4096, 2048), (511 * 3, 511)])
+def test_resnorm_work_holds_every_workgroup(rows, groups, affine):
     """The plan's workgroups (restated) fit the work buffer for every number of rows a workgroup may hold."""
     lib = _lib.load()
     for slots in (1, 4, 8, 16, 32):
-        g = gates if 0 < gates < rows else 1
-        per_gate = rows // g
-        splits = min(max(1, 512 // g), -(-per_gate // slots))
+        g = groups if groups and (groups < rows or affine) else 1
+        per_group = rows // g
+        splits = min(max(1, 512 // g), -(-per_group // slots))
         segments = g * splits
         per = 1 if splits > 1 else -(-segments // 512)
         blocks = -(-segments // per)
-        assert lib.nfi_resnorm_work_bytes(rows, gates, 24) >= blocks * 5 * 24 * 4
+        assert lib.nfi_resnorm_work_bytes(rows, groups, affine, 24) >= blocks * 5 * 24 * 4
 
 
 def test_grouped_linear_refuses():
