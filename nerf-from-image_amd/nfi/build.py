@@ -47,29 +47,44 @@ def _stale() -> bool:
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
-TORCH_OPS_SRC = os.path.join(CSRC, 'nfi_torch.cpp')
+TORCH_OPS_SRCS = [os.path.join(CSRC, 'nfi_torch.cpp'), os.path.join(CSRC, 'nfi_torch_learn.cpp')]
 TORCH_OPS_OUT = os.path.join(HERE, 'libnfi_torch.so')
 
 
+def _run_all(commands, verbose):
+    """One process per command, all at once (a single compiler command takes its sources one after the other)."""
+    jobs = []
+    for cmd in commands:
+        if verbose:
+            print(' '.join(cmd), file=sys.stderr)
+        jobs.append(subprocess.Popen(cmd))
+    codes = [p.wait() for p in jobs]
+    for cmd, rc in zip(commands, codes):
+        if rc:
+            raise subprocess.CalledProcessError(rc, cmd)
+
+
 def build_torch_ops(force: bool = False, verbose: bool = True) -> str:
-    """nfi/libnfi_torch.so: the TORCH_LIBRARY(nfi, ...) operators (csrc/nfi_torch.cpp) over the C-ABI,
+    """nfi/libnfi_torch.so: the TORCH_LIBRARY(nfi, ...) operators (csrc/nfi_torch.cpp, nfi_torch_learn.cpp) over the C-ABI,
     host C++ only (g++ against torch's headers and libraries), linked to nfi/libnfi_hip.so by rpath
     $ORIGIN; loaded with torch.ops.load_library (nfi.torch_ops)."""
-    deps = [TORCH_OPS_SRC, OUT, os.path.join(os.path.dirname(os.path.dirname(HERE)), 'include', 'nfi.h')]
+    inc = os.path.join(os.path.dirname(os.path.dirname(HERE)), 'include')
+    deps = TORCH_OPS_SRCS + [OUT, os.path.join(inc, 'nfi.h'), os.path.join(inc, 'nfi_learn.h')]
     if (not force and os.path.exists(TORCH_OPS_OUT)
             and all(os.path.getmtime(d) <= os.path.getmtime(TORCH_OPS_OUT) for d in deps if os.path.exists(d))):
         return TORCH_OPS_OUT
     import torch
     ti = os.path.dirname(torch.__file__)
     abi = int(torch.compiled_with_cxx11_abi())
-    cmd = [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', TORCH_OPS_SRC, '-o',
-           TORCH_OPS_OUT + '.tmp', f'-I{ti}/include', f'-I{ti}/include/torch/csrc/api/include', '-I/opt/rocm/include',
-           '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1', f'-D_GLIBCXX_USE_CXX11_ABI={abi}', f'-L{ti}/lib', '-lc10',
-           '-lc10_hip', '-ltorch', '-ltorch_cpu', '-ltorch_hip', f'-L{HERE}', '-lnfi_hip', "-Wl,-rpath,$ORIGIN",
-           f'-Wl,-rpath,{ti}/lib']
-    if verbose:
-        print(' '.join(cmd), file=sys.stderr)
-    subprocess.run(cmd, check=True)
+    cxx = [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', f'-I{ti}/include',
+           f'-I{ti}/include/torch/csrc/api/include', '-I/opt/rocm/include', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1',
+           f'-D_GLIBCXX_USE_CXX11_ABI={abi}']
+    with tempfile.TemporaryDirectory() as tmp:
+        objs = [os.path.join(tmp, os.path.basename(src) + '.o') for src in TORCH_OPS_SRCS]
+        _run_all([cxx + ['-c', '-o', o, src] for o, src in zip(objs, TORCH_OPS_SRCS)], verbose)
+        _run_all([[cxx[0], '-shared', '-o', TORCH_OPS_OUT + '.tmp'] + objs
+                  + [f'-L{ti}/lib', '-lc10', '-lc10_hip', '-ltorch', '-ltorch_cpu', '-ltorch_hip', f'-L{HERE}', '-lnfi_hip',
+                     "-Wl,-rpath,$ORIGIN", f'-Wl,-rpath,{ti}/lib']], verbose)
     os.replace(TORCH_OPS_OUT + '.tmp', TORCH_OPS_OUT)
     return TORCH_OPS_OUT
 
@@ -86,20 +101,11 @@ def build(force: bool = False, verbose: bool = True, variant: str = '') -> str:
     extra = {'': [], 'stamps': ['-DNFI_STAMPS'], 'tilecheck': ['-DNFI_TILE_CHECK=1']}.get(variant)
     if extra is None:   # experiment builds: 'D<NAME>=<value>' -> -D<NAME>=<value>
         extra = ['-' + variant] if variant.startswith('D') else []
-    # one compiler process per source, all at once (a single command compiles them one after the other)
     with tempfile.TemporaryDirectory() as tmp:
-        objs, jobs = [], []
-        for s in SOURCES:
-            objs.append(os.path.join(tmp, s.replace('.hip', '.o')))
-            cmd = [hipcc] + [f for f in FLAGS if f != '-shared'] + extra + ['-c', '-o', objs[-1], os.path.join(CSRC, s)]
-            if verbose:
-                print(' '.join(cmd), file=sys.stderr)
-            jobs.append((cmd, subprocess.Popen(cmd)))
-        codes = [(cmd, p.wait()) for cmd, p in jobs]
-        for cmd, rc in codes:
-            if rc:
-                raise subprocess.CalledProcessError(rc, cmd)
-        subprocess.run([hipcc, '--offload-arch=gfx950', '-fPIC', '-shared', '-o', out + '.tmp'] + objs, check=True)
+        objs = [os.path.join(tmp, s.replace('.hip', '.o')) for s in SOURCES]
+        _run_all([[hipcc] + [f for f in FLAGS if f != '-shared'] + extra + ['-c', '-o', o, os.path.join(CSRC, s)]
+                  for o, s in zip(objs, SOURCES)], verbose)
+        _run_all([[hipcc, '--offload-arch=gfx950', '-fPIC', '-shared', '-o', out + '.tmp'] + objs], verbose)
     os.replace(out + '.tmp', out)
     return out
 

@@ -10,32 +10,22 @@ generator and its mapper heads (linear and convolution weights; a convolution's 
 
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Iterable, Sequence
 
 import torch
 
-from . import _lib, learn_ops as lo
+from . import torch_ops
 
 QUINTIC = (3.4445, -4.7750, 2.0315)
-MAX_SIDE = 262144
+_ops: dict = {}
 
 
-def _launch(items, dev, g_type, w_type, update, nesterov, steps, momentum, step, decay, coefficients, eps):
-    arr = (_lib.NfiOrthoItem * len(items))(*items)
-    a = _lib.NfiOrthoArgs()
-    a.items, a.n_items = arr, len(items)
-    a.g_type, a.w_type, a.update, a.nesterov, a.steps = g_type, w_type, update, nesterov, steps
-    a.momentum, a.step, a.decay, a.eps = momentum, step, decay, eps
-    a.a, a.b, a.c = coefficients
-    size = _lib.load().nfi_ortho_work_bytes(arr, len(items))
-    work = None
-    if size:
-        work = torch.empty((size,), device=dev, dtype=torch.uint8)
-        a.work, a.work_bytes = work.data_ptr(), size
-    with lo.on(dev):
-        lo.call('nfi_ortho', ctypes.byref(a), lo.stream(dev))
+def _op(name):
+    op = _ops.get(name)
+    if op is None:
+        op = _ops[name] = torch_ops.op(name)
+    return op
 
 
 def _check(what, steps, coefficients, eps):
@@ -47,36 +37,13 @@ def _check(what, steps, coefficients, eps):
         raise ValueError(f'{what}: eps {eps}')
 
 
-def _check_sides(what, rows, cols, count):
-    if not (1 <= rows <= MAX_SIDE and 1 <= cols <= MAX_SIDE):
-        raise ValueError(f'{what}: sides of 1 to {MAX_SIDE} are wanted, not {rows} x {cols}')
-    if 4 * (-(-rows // 128)) * (-(-cols // 128)) * count >= 1 << 26:
-        raise ValueError(f'{what}: {count} matrices of {rows} x {cols} are too much for one call')
-
-
 @torch.no_grad()
 def orthogonalize(u: torch.Tensor, steps: int = 5, coefficients: Sequence[float] = QUINTIC, eps: float = 1e-7) -> torch.Tensor:
     """u [..., m, n] (float32, bfloat16 or float16) with each matrix's singular values brought near 1: X = u / max(|u|_F,
     eps), then `steps` times X <- (a + b X X^T + c (X X^T)^2) X, (a, b, c) = `coefficients`.  Products are held to 32-bit
     accuracy whatever u's type; the result is rounded once.  Not differentiable."""
-    what = 'orthogonalize'
-    lo.same_device(what, u)
-    code = lo.type_code(u, what)
-    _check(what, steps, coefficients, eps)
-    if u.dim() < 2:
-        raise ValueError(f'{what}: matrices are wanted, not {tuple(u.shape)}')
-    rows, cols = u.shape[-2:]
-    src = u.contiguous()
-    out = torch.empty_like(src)
-    count = 1
-    for n in u.shape[:-2]:
-        count *= n
-    if out.numel() == 0:
-        return out
-    _check_sides(what, rows, cols, count)
-    item = _lib.NfiOrthoItem(src.data_ptr(), None, out.data_ptr(), rows, cols, count, 1.0)
-    _launch([item], u.device, code, code, 0, 0, int(steps), 0.0, 0.0, 0.0, coefficients, eps)
-    return out
+    _check('orthogonalize', steps, coefficients, eps)
+    return _op('orthogonalize')(u, int(steps), *coefficients, eps)
 
 
 class Muon(torch.optim.Optimizer):
@@ -103,47 +70,29 @@ class Muon(torch.optim.Optimizer):
                     raise ValueError(f'Muon: parameters of two or more dimensions are wanted, not {tuple(p.shape)} '
                                      '(biases and gains belong to another optimiser)')
 
-    @staticmethod
-    def _sides(p, batched):
-        if batched:
-            rows, cols = p.shape[-2:]
-            return rows, cols, p.numel() // (rows * cols)
-        return p.shape[0], p.numel() // p.shape[0], 1
-
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        op = _op('muon_step')
         for group in self.param_groups:
-            lots = {}
+            params, grads, momenta = [], [], []
             for p in group['params']:
                 g = p.grad
                 if g is None or p.numel() == 0:
                     continue
-                if g.is_sparse or not p.is_contiguous():
-                    raise RuntimeError('Muon: dense gradients and contiguous parameters are wanted')
-                key = (p.device, p.dtype, g.dtype)
-                lot = lots.get(key)
-                if lot is None:
-                    lo.same_device('Muon', p)
-                    lot = lots[key] = (lo.type_code(g, 'Muon'), lo.type_code(p, 'Muon'), [], [], [])
                 state = self.state[p]
                 m = state.get('momentum_buffer')
                 if m is None:
                     m = state['momentum_buffer'] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
-                if not g.is_contiguous():
-                    g = g.contiguous()
-                    lot[3].append(g)                # kept until the call is made
-                rows, cols, count = self._sides(p, group['batched'])
-                lot[2].append((g.data_ptr(), m.data_ptr(), p.data_ptr(), rows, cols, count, math.sqrt(max(1.0, rows / cols))))
-                lot[4].extend((p, m))
-            for (dev, _, _), (gt, wt, items, _, written) in lots.items():
-                _launch(items, dev, gt, wt, 1, int(group['nesterov']), group['steps'], group['momentum'], group['lr'],
-                        group['lr'] * group['weight_decay'], group['coefficients'], group['eps'])
-                for t in written:                   # what is cached by a tensor's version is out of date
-                    torch.autograd.graph.increment_version(t)
+                params.append(p)
+                grads.append(g)
+                momenta.append(m)
+            if params:
+                op(params, grads, momenta, group['batched'], group['lr'], group['momentum'], group['weight_decay'], group['nesterov'],
+                   group['steps'], *group['coefficients'], group['eps'])
         return loss
 
     def load_state_dict(self, state_dict):

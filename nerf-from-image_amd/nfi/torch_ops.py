@@ -11,6 +11,8 @@ arguments as nfi.ops / nfi.stages; load() fails loudly when the library is missi
   torch.ops.nfi.volume_render_fwd / volume_render_bwd      the two halves (CUDA + Meta kernels)
   torch.ops.nfi.sample_pdf / compute_near_far_planes / cumprod_exclusive /
   render_volume_density_weights_only                        the nerf_utils seams
+  torch.ops.nfi.residual_norm / grouped_linear / orthogonalize / muon_step
+                              behind nfi.norms, nfi.grouped and nfi.optim (csrc/nfi_torch_learn.cpp)
 """
 
 from __future__ import annotations
@@ -25,7 +27,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIBRARY = os.path.join(HERE, 'libnfi_torch.so')
 OPS = ('rays', 'pack_decoder', 'volume_render', 'volume_render_fwd', 'volume_render_bwd', 'sample_pdf',
        'compute_near_far_planes', 'cumprod_exclusive', 'render_volume_density_weights_only',
-       'render_fwd', 'render_bwd', 'composite_fwd', 'composite_bwd', 'triplane_mlp_fwd', 'triplane_mlp_bwd')
+       'render_fwd', 'render_bwd', 'composite_fwd', 'composite_bwd', 'triplane_mlp_fwd', 'triplane_mlp_bwd',
+       'residual_norm', 'grouped_linear', 'orthogonalize', 'muon_step')
 _loaded = False
 
 
@@ -39,6 +42,12 @@ def load() -> None:
     _lib.load()                       # the C-ABI library it links (and the ABI check)
     torch.ops.load_library(LIBRARY)
     _loaded = True
+
+
+def op(name: str):
+    """The operator nfi::name, the library loaded."""
+    load()
+    return getattr(torch.ops.nfi, name).default
 
 
 def render_script_source() -> str:

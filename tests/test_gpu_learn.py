@@ -76,6 +76,17 @@ def test_training_steps_of_a_bank():
             assert float((w.detach() - (old - 0.02 * tall * o)).abs().max()) <= 1e-5
 
 
+def test_no_double_backward():
+    """A graph of the gradients is refused, not built without them."""
+    from nfi.grouped import grouped_linear
+    from nfi.norms import residual_norm
+    x = torch.randn((6, 8), device=DEV, requires_grad=True)
+    w = torch.randn((1, 5, 8), device=DEV, requires_grad=True)
+    for y in (residual_norm(x), grouped_linear(x, w, torch.tensor([0, 6], device=DEV))):
+        with pytest.raises(RuntimeError, match='double backward'):
+            torch.autograd.grad(y.sum(), [x], create_graph=True)
+
+
 def test_bank_refuses():
     b = bank(2)
     with pytest.raises(ValueError, match='mapper_of_image'):
