@@ -13,8 +13,8 @@
 // operands are bounded (singular values start at <= 1 and the polynomial is known), so the scales are constants of the
 // call.  Memory holds 32 hi and 32 lo halves of 32 neighbouring columns together: 128 bytes that are one step of a tile.
 //
-// Matrices of up to 64 rows that fit into LDS run whole in one workgroup each, in 32-bit products; the others run
-// as tiles of 128 x 128, all matrices of the call in each launch: their grid holds one tile after the other.
+// Matrices of up to 64 rows that fit into LDS run whole in one workgroup each; the others run as tiles of 128 x 128, all
+// matrices of the call in each launch: their grid holds one tile after the other.
 #include <algorithm>
 #include <cmath>
 
@@ -420,148 +420,346 @@ __global__ void __launch_bounds__(256) ortho_apply(const Args p) {
 
 // ---- small matrices ----------------------------------------------------------------------------------------------------
 
-// One workgroup of 8 waves holds X [mp][np + 4], A and Q [mp][mp + 4] in LDS (32 bits, rows of 16-column blocks padded by
-// 4: the rows of a read lie in different banks) and runs every step in v_mfma_f32_16x16x4_f32.
-constexpr int SMALL_WAVES = 8;
-
-__host__ __device__ __forceinline__ int small_floats(int mp, int np) { return mp * (np + 4) + 2 * mp * (mp + 4) + SMALL_WAVES * 256; }
-
-__device__ __forceinline__ u4v lines4(const float* p, int ld, int line0, int k0) {
-  return *reinterpret_cast<const u4v*>(p + (line0 + (lane_id() & 15)) * ld + k0 + 4 * (lane_id() >> 4));
-}
-
-template <int FLOATS>
-__global__ void __launch_bounds__(64 * SMALL_WAVES) ortho_small(const Args p, int steps) {
-  __shared__ __attribute__((aligned(16))) float lds[FLOATS];
-  __shared__ double red[64 * SMALL_WAVES];
+// Up to 16 rows: 8 waves hold X in registers, in 32 bits, as v_mfma_f32_16x16x4_f32 takes it for Q X: block b of wave w is the
+// 16 columns from 16 (w + 8 b), lane (i, g) = (l & 15, l >> 4) holding rows 4 g .. + 3 of column i, which is also how the product
+// leaves them.  For A the blocks are turned through LDS of the wave's own; its part of A is the only thing that the waves
+// exchange (one barrier a step): each sums all parts in their order and has A, and by symmetry A A and Q, as an operand.
+// (32-bit products, not pairs of halves: with few rows the pairs' errors, 2^-23 of A and Q each step, do not average out.)
+template <int B>
+__global__ void __launch_bounds__(512) ortho_rows16(const Args p, int steps) {
+  constexpr int TURN = 16 * 20;   // floats of a turned block (rows of 20: those of one access lie in different banks)
+  constexpr int TURNS = B < 4 ? B : 4;
+  __shared__ __attribute__((aligned(16))) float parts[2][8][256];
+  __shared__ __attribute__((aligned(16))) float turned_blocks[8][TURNS][TURN];
+  __shared__ double red[8];
   int matrix, unit;
   const int it = locate(p, blockIdx.x, matrix, unit, [](const Item&) { return 1; });
   if (it < 0) return;
   const Item& t = p.item[it];
-  const int mp = t.mp, np = t.np, ldx = np + 4, lda = mp + 4, nb = mp / 16;
-  float *X = lds, *A = X + mp * ldx, *Q = A + mp * lda, *P = Q + mp * lda;
-  const int64_t size = (int64_t)t.rows * t.cols, base = matrix * size;
+  const int64_t base = (int64_t)matrix * t.rows * t.cols;
+  const bool turned = t.rows > t.cols;
+  const int wave = threadIdx.x >> 6, i = lane_id() & 15, g = lane_id() >> 4;
+  auto place = [&](int b, int r) {   // of X's row 4 g + r, column i of block b; -1 outside
+    const int row = 4 * g + r, col = 16 * (wave + 8 * b) + i;
+    return row < t.m && col < t.n ? (turned ? col * t.cols + row : row * t.cols + col) : -1;
+  };
+  f4v x[B];
+  double s = 0.;
+#pragma unroll
+  for (int b = 0; b < B; ++b)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int at = place(b, r);
+      float v = 0.f;
+      if (at >= 0) {
+        v = typed_at(t.g, p.g_type, base + at);
+        if (t.mom) {
+          const float m = fmaf(p.beta, t.mom[base + at], v);
+          t.mom[base + at] = m;
+          v = p.nesterov ? fmaf(p.beta, m, v) : m;
+        }
+      }
+      x[b][r] = v;
+      s = fma((double)v, (double)v, s);
+    }
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if (lane_id() == 0) red[wave] = s;
+  __syncthreads();
+  s = 0.;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) s += red[w];
+  const double norm = sqrt(s), inv = 1. / (norm < (double)p.eps ? (double)p.eps : norm);   // (a NaN stays one)
+#pragma unroll
+  for (int b = 0; b < B; ++b)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[b][r] = (float)(x[b][r] * inv);
+  for (int step = 0; step < steps; ++step) {
+    f4v acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int b0 = 0; b0 < B; b0 += TURNS) {
+#pragma unroll
+      for (int b = 0; b < TURNS; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) lds_st_fenced(&turned_blocks[wave][b][(4 * g + r) * 20 + i], x[b0 + b][r]);
+#pragma unroll
+      for (int b = 0; b < TURNS; ++b) {
+        const u4v f = *reinterpret_cast<const u4v*>(&turned_blocks[wave][b][i * 20 + 4 * g]);
+        acc = product<float>(f, f, acc);
+      }
+    }
+    // lane (i, g): rows 4 g + r, column i, and as well row i, columns 4 g + r
+    lds_st_fenced(reinterpret_cast<f4v*>(&parts[step & 1][wave][16 * i + 4 * g]), acc);
+    __syncthreads();
+    f4v a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 8; ++w) a += *reinterpret_cast<const f4v*>(&parts[step & 1][w][16 * i + 4 * g]);
+    const u4v af = __builtin_bit_cast(u4v, a);
+    const f4v aa = product<float>(af, af, f4v{0.f, 0.f, 0.f, 0.f});
+    f4v q;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) q[r] = fmaf(p.c, aa[r], fmaf(p.b, a[r], i == 4 * g + r ? p.a : 0.f));
+#pragma unroll
+    for (int b = 0; b < B; ++b) x[b] = product<float>(__builtin_bit_cast(u4v, q), __builtin_bit_cast(u4v, x[b]), f4v{0.f, 0.f, 0.f, 0.f});
+  }
+  const float step = p.step * t.scale;
+#pragma unroll
+  for (int b = 0; b < B; ++b)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int at = place(b, r);
+      if (at < 0) continue;
+      float v = x[b][r];
+      if (p.update) v = fmaf(p.keep, typed_at(t.w, p.w_type, base + at), -step * v);
+      store_typed(t.w, p.w_type, base + at, v);
+    }
+}
+
+// One workgroup of 8 waves holds X [16 nb][n], A and Q [m][m] in LDS, each as a plane of hi and one of lo halves, and runs
+// every step there.  m16 = 16 nb rows are held; A and Q have rows and columns up to the next multiple of 32 (the contracted
+// length of a product), zeros behind.  Rows are padded by 8 halves, so that those of one read lie in different banks.  Bound
+// by the latency of the four phases of a step (A's pieces, A, Q, X), not by the products: 64 x 64 takes 24 products of
+// 16 x 16 x 32 on the longest path.
+constexpr int SMALL_WAVES = 8;
+constexpr int SMALL_THREADS = 64 * SMALL_WAVES;
+
+struct SmallShape {
+  int nb, m16, m32, n32, ldx, lda;   // leading dimensions in halves
+  __host__ __device__ SmallShape(int m, int n) {
+    nb = (m + 15) / 16;
+    m16 = 16 * nb;
+    m32 = (m + 31) / 32 * 32;
+    n32 = (n + 31) / 32 * 32;
+    ldx = n32 + 8;
+    lda = m32 + 8;
+  }
+  // pieces of A (32 bits), X, A, Q in two planes each, 16 zeros
+  __host__ __device__ int bytes() const { return SMALL_WAVES * 1024 + 4 * m16 * ldx + 2 * 4 * m32 * lda + 32; }
+};
+
+__device__ __forceinline__ u4v line8(const _Float16* p, int ld, int line0, int k0) {
+  return *reinterpret_cast<const u4v*>(p + (line0 + (lane_id() & 15)) * ld + k0 + 8 * (lane_id() >> 4));
+}
+// acc += first second^T over 32 contracted values of pairs: registers hold first's lines 4 g + r, lanes second's line i
+__device__ __forceinline__ f4v pair_products(const u4v (&first)[2], const u4v (&second)[2], f4v acc) {
+  acc = product<_Float16>(first[1], second[0], acc);
+  acc = product<_Float16>(first[0], second[1], acc);
+  return product<_Float16>(first[0], second[0], acc);
+}
+__device__ __forceinline__ void store_pair4(_Float16* hi, _Float16* lo, int at, const float (&v)[4]) {
+  h4v h, l;
+  split4(v, h, l);
+  lds_st_fenced(reinterpret_cast<h4v*>(hi + at), h);
+  lds_st_fenced(reinterpret_cast<h4v*>(lo + at), l);
+}
+
+template <int BYTES>
+__global__ void __launch_bounds__(SMALL_THREADS) ortho_small(const Args p, int steps) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[BYTES];
+  __shared__ double red[SMALL_WAVES];
+  int matrix, unit;
+  const int it = locate(p, blockIdx.x, matrix, unit, [](const Item&) { return 1; });
+  if (it < 0) return;
+  const Item& t = p.item[it];
+  const SmallShape d(t.m, t.n);
+  float* P = (float*)lds;
+  _Float16 *Xh = (_Float16*)(lds + SMALL_WAVES * 1024), *Xl = Xh + d.m16 * d.ldx;
+  _Float16 *Ah = Xl + d.m16 * d.ldx, *Al = Ah + d.m32 * d.lda, *Qh = Al + d.m32 * d.lda, *Ql = Qh + d.m32 * d.lda;
+  _Float16* zeros = Ql + d.m32 * d.lda;
+  const int size = t.rows * t.cols;
+  const int64_t base = (int64_t)matrix * size;
   const bool turned = t.rows > t.cols;
   const int tid = threadIdx.x, wave = tid >> 6, l = lane_id(), i = l & 15, g = l >> 4;
-  for (int k = tid; k < mp * ldx; k += 64 * SMALL_WAVES) X[k] = 0.f;
-  __syncthreads();
+  const int words = (d.bytes() - SMALL_WAVES * 1024) / 16;
+  for (int k = tid; k < words; k += SMALL_THREADS) lds_st_fenced((u4v*)Xh + k, u4v{0, 0, 0, 0});
+  // the update's square sum (the momentum is updated by the way) ...
   double s = 0.;
-  for (int e = tid; e < (int)size; e += 64 * SMALL_WAVES) {
-    float v = typed_at(t.g, p.g_type, base + e);
-    if (t.mom) {
-      const float m = fmaf(p.beta, t.mom[base + e], v);
-      t.mom[base + e] = m;
-      v = p.nesterov ? fmaf(p.beta, m, v) : m;
+  for (int e = tid * 4; e < size; e += SMALL_THREADS * 4) {
+    float v[4], m[4];
+    const int have = min(4, size - e);
+    if (have == 4) {
+      load_typed<4>(t.g, p.g_type, base + e, v);
+      if (t.mom) load_piece<float, 4>(t.mom + base + e, m);
+    } else {
+      for (int j = 0; j < 4; ++j) {
+        v[j] = j < have ? typed_at(t.g, p.g_type, base + e + j) : 0.f;
+        m[j] = t.mom && j < have ? t.mom[base + e + j] : 0.f;
+      }
     }
-    const int r = e / t.cols, c = e - r * t.cols;
-    X[turned ? c * ldx + r : r * ldx + c] = v;
-    s = fma((double)v, (double)v, s);
+    if (t.mom) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        m[j] = fmaf(p.beta, m[j], v[j]);
+        v[j] = p.nesterov ? fmaf(p.beta, m[j], v[j]) : m[j];
+      }
+      if (have == 4) store_piece<float, 4>(t.mom + base + e, m);
+      else
+        for (int j = 0; j < have; ++j) t.mom[base + e + j] = m[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s = fma((double)v[j], (double)v[j], s);
   }
-  red[tid] = s;
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if (l == 0) red[wave] = s;
   __syncthreads();
-  for (int d = 32 * SMALL_WAVES; d > 0; d >>= 1) {
-    if (tid < d) red[tid] += red[tid + d];
-    __syncthreads();
+  s = 0.;
+#pragma unroll
+  for (int w = 0; w < SMALL_WAVES; ++w) s += red[w];
+  const double norm = sqrt(s);
+  const double inv = (double)p.up_x / (norm < (double)p.eps ? (double)p.eps : norm);   // (a NaN stays one)
+  // ... and X0 (its own loads again, from the cache: each thread reads what it read and wrote)
+  for (int e = tid * 4; e < size; e += SMALL_THREADS * 4) {
+    const int have = min(4, size - e);
+    int r = e / t.cols, c = e - r * t.cols;
+    for (int j = 0; j < have; ++j) {
+      const float v = (float)(update_at(p, t, base + e + j) * inv);
+      const _Float16 h = (_Float16)v;
+      const int at = turned ? c * d.ldx + r : r * d.ldx + c;
+      Xh[at] = h;
+      Xl[at] = (_Float16)(v - (float)h);
+      if (++c == t.cols) c = 0, ++r;
+    }
   }
-  const double norm = sqrt(red[0]);
-  const double inv = 1. / (norm < (double)p.eps ? (double)p.eps : norm);
-  for (int k = tid; k < mp * ldx; k += 64 * SMALL_WAVES) X[k] = (float)(X[k] * inv);
-  // A's blocks over the waves, the columns of X in ks pieces where there are few blocks
-  const int blocks = nb * nb, ks = nb == 1 ? 8 : nb == 2 ? 2 : 1, pieces = np / 16;
+  const float to_a = p.up_a / (p.up_x * p.up_x), to_x = 1.f / p.up_q;
+  const float qs = p.c * p.up_q / (p.up_a * p.up_a), qb = p.b * p.up_q / p.up_a, qa = p.a * p.up_q;
+  const int lower = d.nb * (d.nb + 1) / 2, ks = d.nb == 1 ? 8 : d.nb == 2 ? 2 : 1, deep = d.n32 / 32;
   for (int step = 0; step < steps; ++step) {
     __syncthreads();
-    for (int task = wave; task < blocks * ks; task += SMALL_WAVES) {
-      const int blk = task / ks, part = task - blk * ks, bi = blk / nb, bj = blk - bi * nb;
+    // A: the blocks on and below the diagonal over the waves, in ks pieces of X's columns where they are few
+    for (int task = wave; task < lower * ks; task += SMALL_WAVES) {
+      const int blk = task / ks, part = task - blk * ks;
+      int bi, bj;
+      triangle(blk, bi, bj);
       f4v acc = {0.f, 0.f, 0.f, 0.f};
-      if (bj <= bi)
-        for (int k = pieces * part / ks; k < pieces * (part + 1) / ks; ++k)
-          acc = product<float>(lines4(X, ldx, bi * 16, 16 * k), lines4(X, ldx, bj * 16, 16 * k), acc);
-      // lane: bj's line i, registers: bi's lines 4 g + r
+      const int k1 = deep * (part + 1) / ks;
+      for (int k = deep * part / ks; k < k1; ++k) {
+        const u4v a[2] = {line8(Xh, d.ldx, bi * 16, 32 * k), line8(Xl, d.ldx, bi * 16, 32 * k)};
+        const u4v b[2] = {line8(Xh, d.ldx, bj * 16, 32 * k), line8(Xl, d.ldx, bj * 16, 32 * k)};
+        acc = pair_products(b, a, acc);
+      }
       if (ks > 1) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) P[task * 256 + (4 * g + r) * 16 + i] = acc[r];
-      } else if (bj <= bi) {
+        for (int r = 0; r < 4; ++r) P[task * 256 + i * 16 + 4 * g + r] = acc[r];
+      } else {
+        const float v[4] = {acc[0] * to_a, acc[1] * to_a, acc[2] * to_a, acc[3] * to_a};
+        store_pair4(Ah, Al, (bi * 16 + i) * d.lda + bj * 16 + 4 * g, v);
+        if (bi != bj) {
+          h4v h, lo;
+          split4(v, h, lo);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          A[(bi * 16 + 4 * g + r) * lda + bj * 16 + i] = acc[r];
-          A[(bj * 16 + i) * lda + bi * 16 + 4 * g + r] = acc[r];
+          for (int r = 0; r < 4; ++r) {
+            Ah[(bj * 16 + 4 * g + r) * d.lda + bi * 16 + i] = h[r];
+            Al[(bj * 16 + 4 * g + r) * d.lda + bi * 16 + i] = lo[r];
+          }
         }
       }
     }
     __syncthreads();
     if (ks > 1) {
-      for (int e = tid; e < blocks * 256; e += 64 * SMALL_WAVES) {
-        const int blk = e >> 8, bi = blk / nb, bj = blk - bi * nb, r = (e >> 4) & 15, c = e & 15;
-        if (bj > bi) continue;
+      for (int e = tid; e < lower * 256; e += SMALL_THREADS) {
+        int bi, bj;
+        triangle(e >> 8, bi, bj);
+        const int r = (e >> 4) & 15, c = e & 15;
         float v = 0.f;
-        for (int q = 0; q < ks; ++q) v += P[(blk * ks + q) * 256 + (e & 255)];
-        A[(bi * 16 + r) * lda + bj * 16 + c] = v;
-        if (bi != bj) A[(bj * 16 + c) * lda + bi * 16 + r] = v;
+        for (int q = 0; q < ks; ++q) v += P[((e >> 8) * ks + q) * 256 + (e & 255)];
+        v *= to_a;
+        const _Float16 h = (_Float16)v, lo = (_Float16)(v - (float)h);
+        Ah[(bi * 16 + r) * d.lda + bj * 16 + c] = h;
+        Al[(bi * 16 + r) * d.lda + bj * 16 + c] = lo;
+        if (bi != bj) {
+          Ah[(bj * 16 + c) * d.lda + bi * 16 + r] = h;
+          Al[(bj * 16 + c) * d.lda + bi * 16 + r] = lo;
+        }
       }
       __syncthreads();
     }
-    for (int task = wave; task < blocks; task += SMALL_WAVES) {
-      const int bi = task / nb, bj = task - bi * nb;
+    for (int task = wave; task < d.nb * d.nb; task += SMALL_WAVES) {
+      const int bi = task / d.nb, bj = task - bi * d.nb;
       f4v acc = {0.f, 0.f, 0.f, 0.f};
-      for (int k = 0; k < nb; ++k) acc = product<float>(lines4(A, lda, bi * 16, 16 * k), lines4(A, lda, bj * 16, 16 * k), acc);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = bi * 16 + 4 * g + r, col = bj * 16 + i;
-        Q[row * lda + col] = fmaf(p.c, acc[r], fmaf(p.b, A[row * lda + col], row == col ? p.a : 0.f));
+      for (int k = 0; k < d.m32; k += 32) {
+        const u4v a[2] = {line8(Ah, d.lda, bi * 16, k), line8(Al, d.lda, bi * 16, k)};
+        const u4v b[2] = {line8(Ah, d.lda, bj * 16, k), line8(Al, d.lda, bj * 16, k)};
+        acc = pair_products(b, a, acc);
       }
+      const int row = bi * 16 + i, col = bj * 16 + 4 * g;
+      const h4v h = *reinterpret_cast<const h4v*>(Ah + row * d.lda + col), lo = *reinterpret_cast<const h4v*>(Al + row * d.lda + col);
+      float v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = fmaf(qs, acc[r], fmaf(qb, (float)h[r] + (float)lo[r], row == col + r ? qa : 0.f));
+      store_pair4(Qh, Ql, row * d.lda + col, v);
     }
     __syncthreads();
-    // a wave takes whole blocks of X's columns, which no other one reads: in place
-    for (int cb = wave; cb < pieces; cb += SMALL_WAVES) {
+    // X: a wave takes whole blocks of columns, which no other one reads: in place
+    for (int cb = wave; cb < d.n32 / 16; cb += SMALL_WAVES) {
       f4v acc[4];
 #pragma unroll
       for (int bi = 0; bi < 4; ++bi) acc[bi] = f4v{0.f, 0.f, 0.f, 0.f};
-      for (int k = 0; k < nb; ++k) {
-        u4v x;
+      for (int k = 0; k < d.m32; k += 32) {
+        u4v x[2];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = __float_as_uint(X[(16 * k + 4 * g + r) * ldx + cb * 16 + i]);
+        for (int plane = 0; plane < 2; ++plane) {
+          u2v v[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int row = k + 8 * g + 4 * h + (i >> 2);
+            const _Float16* q = row < d.m16 ? (plane ? Xl : Xh) + row * d.ldx + cb * 16 + 4 * (i & 3) : zeros + 4 * (i & 3);
+            v[h] = __builtin_bit_cast(u2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*)q));
+          }
+          x[plane] = u4v{v[0][0], v[0][1], v[1][0], v[1][1]};
+        }
 #pragma unroll
         for (int bi = 0; bi < 4; ++bi)
-          if (bi < nb) acc[bi] = product<float>(lines4(Q, lda, bi * 16, 16 * k), x, acc[bi]);
+          if (bi < d.nb) {
+            const u4v q[2] = {line8(Qh, d.lda, bi * 16, k), line8(Ql, d.lda, bi * 16, k)};
+            acc[bi] = pair_products(x, q, acc[bi]);
+          }
       }
 #pragma unroll
       for (int bi = 0; bi < 4; ++bi)
-        if (bi < nb)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) X[(bi * 16 + 4 * g + r) * ldx + cb * 16 + i] = acc[bi][r];
+        if (bi < d.nb) {
+          const float v[4] = {acc[bi][0] * to_x, acc[bi][1] * to_x, acc[bi][2] * to_x, acc[bi][3] * to_x};
+          store_pair4(Xh, Xl, (bi * 16 + i) * d.ldx + cb * 16 + 4 * g, v);
+        }
     }
   }
   __syncthreads();
-  const float step = p.step * t.scale;
-  for (int e = tid; e < (int)size; e += 64 * SMALL_WAVES) {
-    const int r = e / t.cols, c = e - r * t.cols;
-    float v = X[turned ? c * ldx + r : r * ldx + c];
-    if (p.update) v = fmaf(p.keep, typed_at(t.w, p.w_type, base + e), -step * v);
-    store_typed(t.w, p.w_type, base + e, v);
+  const float step = p.step * t.scale, down = 1.f / p.up_x;
+  for (int e = tid * 4; e < size; e += SMALL_THREADS * 4) {
+    const int have = min(4, size - e);
+    int r = e / t.cols, c = e - r * t.cols;
+    float v[4];
+    for (int j = 0; j < have; ++j) {
+      const int at = turned ? c * d.ldx + r : r * d.ldx + c;
+      v[j] = ((float)Xh[at] + (float)Xl[at]) * down;
+      if (p.update) v[j] = fmaf(p.keep, typed_at(t.w, p.w_type, base + e + j), -step * v[j]);
+      if (++c == t.cols) c = 0, ++r;
+    }
+    if (have == 4 && p.w_type == NFI_F32) store_piece<float, 4>((float*)t.w + base + e, v);
+    else
+      for (int j = 0; j < have; ++j) store_typed(t.w, p.w_type, base + e + j, v[j]);
   }
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
 
-constexpr int SMALL_SIZES[3] = {9216, 18432, 36864};   // floats of LDS: 36, 72, 144 KB
+constexpr int SMALL_SIZES[3] = {40960, 79872, 155648};   // bytes of LDS: four, two or one workgroup for a compute unit
+constexpr int KINDS = 6;
 static inline int ceil_to(int v, int k) { return (v + k - 1) / k * k; }
 static inline int64_t up(int64_t v) { return (v + 255) / 256 * 256; }
 
-// -1: as tiles; else the small kernel's size.  (One workgroup runs a 64 x 448 matrix in the time that the tiles' launches
-// alone take, so whatever fits into LDS runs there.)
-static int small_size(int m, int n) {
-  if (m > 64) return -1;
-  // (n may be any number: the product has to stay in range)
-  if (n > 65536) return -1;
-  const int need = small_floats(ceil_to(m, 16), ceil_to(n, 16));
+// How a matrix runs: -1 as tiles, 0 .. 2 in registers (blocks of 16 columns for each wave: 1, 4, 16), 3 .. 5 in LDS
+static int kind_of(int m, int n) {
+  if (m <= 16 && n <= 2048) return n <= 128 ? 0 : n <= 512 ? 1 : 2;
+  if (m > 64 || n > 65536) return -1;
+  const int need = SmallShape(m, n).bytes();
   for (int k = 0; k < 3; ++k)
-    if (need <= SMALL_SIZES[k]) return k;
+    if (need <= SMALL_SIZES[k]) return 3 + k;
   return -1;
 }
+static int kind_of(const nfi_ortho_item& q) { return kind_of(std::min(q.rows, q.cols), std::max(q.rows, q.cols)); }
 
 static int64_t item_bytes(const nfi_ortho_item& s) {
   const int m = std::min(s.rows, s.cols), n = std::max(s.rows, s.cols);
-  if (small_size(m, n) >= 0) return 0;
+  if (kind_of(s) >= 0) return 0;
   const int64_t mp = ceil_to(m, TILE), np = ceil_to(n, TILE), size = (int64_t)s.rows * s.cols;
   return s.count * (2 * up(mp * np * 4) + 2 * up(mp * mp * 4)) + up(s.count * ((size + NORM_CHUNK - 1) / NORM_CHUNK) * 8);
 }
@@ -664,20 +862,24 @@ int32_t nfi_ortho(const nfi_ortho_args* p, void* stream) {
     t.np = ceil_to(t.n, unit);
     return t;
   };
-  for (int size = 0; size < 3; ++size) {
+  for (int kind = 0; kind < KINDS; ++kind) {
     Args a = base;
     int64_t blocks = 0;
     auto flush = [&]() {
       if (a.items == 0) return;
-      if (size == 0) ortho_small<SMALL_SIZES[0]><<<(unsigned)blocks, 64 * SMALL_WAVES, 0, s>>>(a, p->steps);
-      else if (size == 1) ortho_small<SMALL_SIZES[1]><<<(unsigned)blocks, 64 * SMALL_WAVES, 0, s>>>(a, p->steps);
-      else ortho_small<SMALL_SIZES[2]><<<(unsigned)blocks, 64 * SMALL_WAVES, 0, s>>>(a, p->steps);
+      const unsigned n = (unsigned)blocks;
+      if (kind == 0) ortho_rows16<1><<<n, 512, 0, s>>>(a, p->steps);
+      else if (kind == 1) ortho_rows16<4><<<n, 512, 0, s>>>(a, p->steps);
+      else if (kind == 2) ortho_rows16<16><<<n, 512, 0, s>>>(a, p->steps);
+      else if (kind == 3) ortho_small<SMALL_SIZES[0]><<<n, SMALL_THREADS, 0, s>>>(a, p->steps);
+      else if (kind == 4) ortho_small<SMALL_SIZES[1]><<<n, SMALL_THREADS, 0, s>>>(a, p->steps);
+      else ortho_small<SMALL_SIZES[2]><<<n, SMALL_THREADS, 0, s>>>(a, p->steps);
       a.items = 0;
       blocks = 0;
     };
     for (int i = 0; i < p->n_items; ++i) {
       const nfi_ortho_item& q = p->items[i];
-      if (small_size(std::min(q.rows, q.cols), std::max(q.rows, q.cols)) != size) continue;
+      if (kind_of(q) != kind) continue;
       a.item[a.items++] = item(q, 16);
       blocks += q.count;
       if (a.items == ITEMS) flush();
@@ -704,7 +906,7 @@ int32_t nfi_ortho(const nfi_ortho_args* p, void* stream) {
   };
   for (int i = 0; i < p->n_items; ++i) {
     const nfi_ortho_item& q = p->items[i];
-    if (small_size(std::min(q.rows, q.cols), std::max(q.rows, q.cols)) >= 0) continue;
+    if (kind_of(q) >= 0) continue;
     Item t = item(q, TILE);
     const int64_t sx = up((int64_t)t.mp * t.np * 4) * t.count, sa = up((int64_t)t.mp * t.mp * 4) * t.count;
     t.x = (_Float16*)work;

@@ -44,7 +44,7 @@ def near(got, u, dtype, steps=5, abc=optim.QUINTIC):
         assert err <= 4 * own + 2.0 ** -21 * max(size, 1e-30), (tuple(u.shape), err, own, size)
 
 
-SHAPES = [(1, 1), (1, 7), (9, 1), (3, 3), (2, 15, 512), (16, 16), (17, 40), (40, 17), (3, 33, 33), (64, 64), (64, 448), (448, 64), (64, 449),
+SHAPES = [(1, 1), (1, 7), (9, 1), (3, 3), (2, 15, 512), (16, 16), (17, 40), (40, 17), (3, 33, 33), (64, 64), (64, 448), (448, 64), (64, 449), (64, 384), (384, 60), (50, 390), (48, 500), (20, 900), (31, 33), (16, 1900), (15, 2049), (4, 128), (130, 16), (2048, 9),
           (65, 70), (33, 1100), (128, 128), (129, 257), (300, 200), (2, 3, 96, 512), (513, 700), (11, 64), (5, 3000), (1, 70000),
           (640, 1300)]
 
