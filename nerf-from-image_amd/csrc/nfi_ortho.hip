@@ -37,10 +37,15 @@ struct Item {
 };
 
 struct Args {
-  Item item[ITEMS];
   int items, g_type, w_type, update, nesterov, last;
   float beta, keep, step, a, b, c, eps;   // keep = 1 - decay
   float up_x, up_a, up_q;                 // powers of two
+};
+
+// The launch's arguments: a kernel takes room for 1, 8 or 32 items (3.4 KB of arguments cost 10 us of a launch)
+template <int N>
+struct Table : Args {
+  Item item[N];
 };
 
 typedef _Float16 h4v __attribute__((ext_vector_type(4)));
@@ -50,8 +55,8 @@ __device__ __forceinline__ float typed_at(const void* p, int type, int64_t i) {
 }
 
 // Work unit `id` of a launch: the item, the matrix of its run, and the unit within it (per(item) units each)
-template <class F>
-__device__ __forceinline__ int locate(const Args& p, int id, int& matrix, int& unit, F per) {
+template <int N, class F>
+__device__ __forceinline__ int locate(const Table<N>& p, int id, int& matrix, int& unit, F per) {
   for (int i = 0; i < p.items; ++i) {
     const int u = per(p.item[i]), all = u * p.item[i].count;
     if (id < all) {
@@ -67,7 +72,8 @@ __device__ __forceinline__ int locate(const Args& p, int id, int& matrix, int& u
 // ---- momentum and norm -------------------------------------------------------------------------------------------
 
 // M <- beta M + G, and the squares' sum of U over a chunk (64-bit: squares of bf16 values pass the 32-bit range)
-__global__ void __launch_bounds__(256) ortho_norm(const Args p) {
+template <int N>
+__global__ void __launch_bounds__(256) ortho_norm(const Table<N> p) {
   __shared__ double red[256];
   int matrix, chunk;
   const int i = locate(p, blockIdx.x, matrix, chunk, [](const Item& t) { return t.chunks; });
@@ -143,7 +149,8 @@ __device__ __forceinline__ void split4(const float (&v)[4], h4v& hi, h4v& lo) {
 __device__ __forceinline__ int64_t half_at(int c) { return ((int64_t)(c >> 5) << 6) + (c & 31); }
 
 // X0 in halves, 64 x 64 at a time, turned where the matrix is taller than wide; zeros in the padding
-__global__ void __launch_bounds__(256) ortho_start(const Args p) {
+template <int N>
+__global__ void __launch_bounds__(256) ortho_start(const Table<N> p) {
   __shared__ float tile[64][65];
   __shared__ double red[256];
   int matrix, unit;
@@ -312,8 +319,8 @@ __device__ __forceinline__ void triangle(int unit, int& ti, int& tj) {
 }
 
 // A = X X^T (SQUARE false) or Q = a I + b A + c A A (SQUARE true), the tiles on and below the diagonal
-template <bool SQUARE>
-__global__ void __launch_bounds__(256) ortho_gram(const Args p) {
+template <bool SQUARE, int N>
+__global__ void __launch_bounds__(256) ortho_gram(const Table<N> p) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[4 * TILE_BYTES];
   int matrix, unit, ti, tj;
   const int it = locate(p, blockIdx.x, matrix, unit, [](const Item& t) { const int k = t.mp / TILE; return k * (k + 1) / 2; });
@@ -372,7 +379,8 @@ __device__ __forceinline__ void put_update(const Args& p, const Item& t, int64_t
   }
 }
 
-__global__ void __launch_bounds__(256) ortho_apply(const Args p) {
+template <int N>
+__global__ void __launch_bounds__(256) ortho_apply(const Table<N> p) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[4 * TILE_BYTES];
   int matrix, unit;
   const int it = locate(p, blockIdx.x, matrix, unit, [](const Item& t) { return t.mp / TILE * (t.np / TILE); });
@@ -420,107 +428,134 @@ __global__ void __launch_bounds__(256) ortho_apply(const Args p) {
 
 // ---- small matrices ----------------------------------------------------------------------------------------------------
 
-// Up to 16 rows: 8 waves hold X in registers, in 32 bits, as v_mfma_f32_16x16x4_f32 takes it for Q X: block b of wave w is the
-// 16 columns from 16 (w + 8 b), lane (i, g) = (l & 15, l >> 4) holding rows 4 g .. + 3 of column i, which is also how the product
+constexpr int SMALL_WAVES = 16;
+constexpr int SMALL_THREADS = 64 * SMALL_WAVES;
+
+// g's value at `at` through `type`, 0 where at < 0 (the load is made all the same: loads in a row wait for each other's branches)
+template <class T>
+__device__ __forceinline__ float value_or_zero(const void* p, int64_t base, int at) {
+  const float v = (float)((const T*)p)[base + (at < 0 ? 0 : at)];
+  return at < 0 ? 0.f : v;
+}
+
+// Up to 16 rows: the waves hold X in registers, in 32 bits, as v_mfma_f32_16x16x4_f32 takes it for Q X: block b of wave w is the
+// 16 columns from 16 (w + 16 b), lane (i, g) = (l & 15, l >> 4) holding rows 4 g .. + 3 of column i, which is also how the product
 // leaves them.  For A the blocks are turned through LDS of the wave's own; its part of A is the only thing that the waves
 // exchange (one barrier a step): each sums all parts in their order and has A, and by symmetry A A and Q, as an operand.
 // (32-bit products, not pairs of halves: with few rows the pairs' errors, 2^-23 of A and Q each step, do not average out.)
+constexpr int TURN = 16 * 20;   // floats of a turned block (rows of 20: those of one access lie in different banks)
+constexpr int ROWS16_BYTES = 2 * SMALL_WAVES * 1024 + SMALL_WAVES * 2 * TURN * 4;
+
 template <int B>
-__global__ void __launch_bounds__(512) ortho_rows16(const Args p, int steps) {
-  constexpr int TURN = 16 * 20;   // floats of a turned block (rows of 20: those of one access lie in different banks)
-  constexpr int TURNS = B < 4 ? B : 4;
-  __shared__ __attribute__((aligned(16))) float parts[2][8][256];
-  __shared__ __attribute__((aligned(16))) float turned_blocks[8][TURNS][TURN];
-  __shared__ double red[8];
-  int matrix, unit;
-  const int it = locate(p, blockIdx.x, matrix, unit, [](const Item&) { return 1; });
-  if (it < 0) return;
-  const Item& t = p.item[it];
+__device__ __forceinline__ void run_rows16(const Args& p, const Item& t, int matrix, int steps, unsigned char* lds, double* red) {
+  constexpr int TURNS = B < 2 ? B : 2;
+  float* parts = (float*)lds;                              // [2][waves][256]
   const int64_t base = (int64_t)matrix * t.rows * t.cols;
   const bool turned = t.rows > t.cols;
   const int wave = threadIdx.x >> 6, i = lane_id() & 15, g = lane_id() >> 4;
+  float* turn = parts + 2 * SMALL_WAVES * 256 + wave * 2 * TURN;   // [TURNS][16][20], this wave's own
   auto place = [&](int b, int r) {   // of X's row 4 g + r, column i of block b; -1 outside
-    const int row = 4 * g + r, col = 16 * (wave + 8 * b) + i;
+    const int row = 4 * g + r, col = 16 * (wave + SMALL_WAVES * b) + i;
     return row < t.m && col < t.n ? (turned ? col * t.cols + row : row * t.cols + col) : -1;
   };
   f4v x[B];
+  auto fetch = [&](auto type, const void* from, f4v (&to)[B]) {
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) to[b][r] = value_or_zero<decltype(type)>(from, base, place(b, r));
+  };
+  auto fetch_typed = [&](int type, const void* from, f4v (&to)[B]) {
+    if (type == NFI_F32) fetch(float(), from, to);
+    else if (type == NFI_BF16) fetch(bf16_t(), from, to);
+    else fetch(f16_t(), from, to);
+  };
+  fetch_typed(p.g_type, t.g, x);
+  if (t.mom) {
+    f4v m[B];
+    fetch(float(), t.mom, m);
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float v = fmaf(p.beta, m[b][r], x[b][r]);
+        x[b][r] = p.nesterov ? fmaf(p.beta, v, x[b][r]) : v;
+        const int at = place(b, r);
+        if (at >= 0) t.mom[base + at] = v;
+      }
+  }
   double s = 0.;
 #pragma unroll
   for (int b = 0; b < B; ++b)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int at = place(b, r);
-      float v = 0.f;
-      if (at >= 0) {
-        v = typed_at(t.g, p.g_type, base + at);
-        if (t.mom) {
-          const float m = fmaf(p.beta, t.mom[base + at], v);
-          t.mom[base + at] = m;
-          v = p.nesterov ? fmaf(p.beta, m, v) : m;
-        }
-      }
-      x[b][r] = v;
-      s = fma((double)v, (double)v, s);
-    }
+    for (int r = 0; r < 4; ++r) s = fma((double)x[b][r], (double)x[b][r], s);
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-  if (lane_id() == 0) red[wave] = s;
+  if (lane_id() == 0) lds_st_fenced(red + wave, s);
   __syncthreads();
   s = 0.;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) s += red[w];
+  for (int w = 0; w < SMALL_WAVES; ++w) s += red[w];
   const double norm = sqrt(s), inv = 1. / (norm < (double)p.eps ? (double)p.eps : norm);   // (a NaN stays one)
 #pragma unroll
   for (int b = 0; b < B; ++b)
 #pragma unroll
     for (int r = 0; r < 4; ++r) x[b][r] = (float)(x[b][r] * inv);
+  const int used = min(SMALL_WAVES, (t.n + 15) / 16);   // waves that hold a column
   for (int step = 0; step < steps; ++step) {
-    f4v acc = {0.f, 0.f, 0.f, 0.f};
+    float* part = parts + (step & 1) * SMALL_WAVES * 256;
+    if (wave < used) {
+      f4v acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int b0 = 0; b0 < B; b0 += TURNS) {
+      for (int b0 = 0; b0 < B; b0 += TURNS) {
 #pragma unroll
-      for (int b = 0; b < TURNS; ++b)
+        for (int b = 0; b < TURNS; ++b)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) lds_st_fenced(&turned_blocks[wave][b][(4 * g + r) * 20 + i], x[b0 + b][r]);
+          for (int r = 0; r < 4; ++r) lds_st_fenced(turn + b * TURN + (4 * g + r) * 20 + i, x[b0 + b][r]);
 #pragma unroll
-      for (int b = 0; b < TURNS; ++b) {
-        const u4v f = *reinterpret_cast<const u4v*>(&turned_blocks[wave][b][i * 20 + 4 * g]);
-        acc = product<float>(f, f, acc);
+        for (int b = 0; b < TURNS; ++b) {
+          const u4v f = *reinterpret_cast<const u4v*>(turn + b * TURN + i * 20 + 4 * g);
+          acc = product<float>(f, f, acc);
+        }
       }
+      // lane (i, g): rows 4 g + r, column i, and as well row i, columns 4 g + r
+      lds_st_fenced(reinterpret_cast<f4v*>(part + wave * 256 + 16 * i + 4 * g), acc);
     }
-    // lane (i, g): rows 4 g + r, column i, and as well row i, columns 4 g + r
-    lds_st_fenced(reinterpret_cast<f4v*>(&parts[step & 1][wave][16 * i + 4 * g]), acc);
     __syncthreads();
-    f4v a = {0.f, 0.f, 0.f, 0.f};
+    if (wave < used) {
+      f4v a = {0.f, 0.f, 0.f, 0.f};
+      for (int w = 0; w < used; ++w) a += *reinterpret_cast<const f4v*>(part + w * 256 + 16 * i + 4 * g);
+      const u4v af = __builtin_bit_cast(u4v, a);
+      const f4v aa = product<float>(af, af, f4v{0.f, 0.f, 0.f, 0.f});
+      f4v q;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) a += *reinterpret_cast<const f4v*>(&parts[step & 1][w][16 * i + 4 * g]);
-    const u4v af = __builtin_bit_cast(u4v, a);
-    const f4v aa = product<float>(af, af, f4v{0.f, 0.f, 0.f, 0.f});
-    f4v q;
+      for (int r = 0; r < 4; ++r) q[r] = fmaf(p.c, aa[r], fmaf(p.b, a[r], i == 4 * g + r ? p.a : 0.f));
 #pragma unroll
-    for (int r = 0; r < 4; ++r) q[r] = fmaf(p.c, aa[r], fmaf(p.b, a[r], i == 4 * g + r ? p.a : 0.f));
-#pragma unroll
-    for (int b = 0; b < B; ++b) x[b] = product<float>(__builtin_bit_cast(u4v, q), __builtin_bit_cast(u4v, x[b]), f4v{0.f, 0.f, 0.f, 0.f});
+      for (int b = 0; b < B; ++b) x[b] = product<float>(__builtin_bit_cast(u4v, q), __builtin_bit_cast(u4v, x[b]), f4v{0.f, 0.f, 0.f, 0.f});
+    }
   }
   const float step = p.step * t.scale;
+  if (p.update) {
+    f4v w[B];
+    fetch_typed(p.w_type, t.w, w);
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[b][r] = fmaf(p.keep, w[b][r], -step * x[b][r]);
+  }
 #pragma unroll
   for (int b = 0; b < B; ++b)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int at = place(b, r);
-      if (at < 0) continue;
-      float v = x[b][r];
-      if (p.update) v = fmaf(p.keep, typed_at(t.w, p.w_type, base + at), -step * v);
-      store_typed(t.w, p.w_type, base + at, v);
+      if (at >= 0) store_typed(t.w, p.w_type, base + at, x[b][r]);
     }
 }
 
-// One workgroup of 8 waves holds X [16 nb][n], A and Q [m][m] in LDS, each as a plane of hi and one of lo halves, and runs
+// More rows: a workgroup of 16 waves holds X [16 nb][n], A and Q [m][m] in LDS, each as a plane of hi and one of lo halves, and runs
 // every step there.  m16 = 16 nb rows are held; A and Q have rows and columns up to the next multiple of 32 (the contracted
 // length of a product), zeros behind.  Rows are padded by 8 halves, so that those of one read lie in different banks.  Bound
-// by the latency of the four phases of a step (A's pieces, A, Q, X), not by the products: 64 x 64 takes 24 products of
-// 16 x 16 x 32 on the longest path.
-constexpr int SMALL_WAVES = 8;
-constexpr int SMALL_THREADS = 64 * SMALL_WAVES;
+// by the latency of a step's phases (A's pieces, A, Q, X), not by the products: 64 x 64 takes 18 products of 16 x 16 x 32 on
+// the longest path.
 
 struct SmallShape {
   int nb, m16, m32, n32, ldx, lda;   // leading dimensions in halves
@@ -536,9 +571,6 @@ struct SmallShape {
   __host__ __device__ int bytes() const { return SMALL_WAVES * 1024 + 4 * m16 * ldx + 2 * 4 * m32 * lda + 32; }
 };
 
-__device__ __forceinline__ u4v line8(const _Float16* p, int ld, int line0, int k0) {
-  return *reinterpret_cast<const u4v*>(p + (line0 + (lane_id() & 15)) * ld + k0 + 8 * (lane_id() >> 4));
-}
 // acc += first second^T over 32 contracted values of pairs: registers hold first's lines 4 g + r, lanes second's line i
 __device__ __forceinline__ f4v pair_products(const u4v (&first)[2], const u4v (&second)[2], f4v acc) {
   acc = product<_Float16>(first[1], second[0], acc);
@@ -552,14 +584,8 @@ __device__ __forceinline__ void store_pair4(_Float16* hi, _Float16* lo, int at, 
   lds_st_fenced(reinterpret_cast<h4v*>(lo + at), l);
 }
 
-template <int BYTES>
-__global__ void __launch_bounds__(SMALL_THREADS) ortho_small(const Args p, int steps) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds[BYTES];
-  __shared__ double red[SMALL_WAVES];
-  int matrix, unit;
-  const int it = locate(p, blockIdx.x, matrix, unit, [](const Item&) { return 1; });
-  if (it < 0) return;
-  const Item& t = p.item[it];
+template <int NB>
+__device__ __forceinline__ void run_lds(const Args& p, const Item& t, int matrix, int steps, unsigned char* lds, double* red) {
   const SmallShape d(t.m, t.n);
   float* P = (float*)lds;
   _Float16 *Xh = (_Float16*)(lds + SMALL_WAVES * 1024), *Xl = Xh + d.m16 * d.ldx;
@@ -599,7 +625,7 @@ __global__ void __launch_bounds__(SMALL_THREADS) ortho_small(const Args p, int s
     for (int j = 0; j < 4; ++j) s = fma((double)v[j], (double)v[j], s);
   }
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-  if (l == 0) red[wave] = s;
+  if (l == 0) lds_st_fenced(red + wave, s);
   __syncthreads();
   s = 0.;
 #pragma unroll
@@ -621,104 +647,165 @@ __global__ void __launch_bounds__(SMALL_THREADS) ortho_small(const Args p, int s
   }
   const float to_a = p.up_a / (p.up_x * p.up_x), to_x = 1.f / p.up_q;
   const float qs = p.c * p.up_q / (p.up_a * p.up_a), qb = p.b * p.up_q / p.up_a, qa = p.a * p.up_q;
-  const int lower = d.nb * (d.nb + 1) / 2, ks = d.nb == 1 ? 8 : d.nb == 2 ? 2 : 1, deep = d.n32 / 32;
+  // each wave's place in a step's phases: a block of A on or below the diagonal (in ks pieces of X's columns where the blocks
+  // are few), a block of Q, and blocks of X
+  constexpr int LOWER = NB * (NB + 1) / 2, KS = SMALL_WAVES / LOWER, DEEP_M = (NB + 1) / 2;
+  const int deep = d.n32 / 32, cbs = d.n32 / 16, plane_x = d.m16 * d.ldx, plane_a = d.m32 * d.lda;
+  int bi, bj;
+  triangle(wave / KS, bi, bj);
+  const bool has_a = wave < LOWER * KS, has_q = wave < NB * NB;
+  const int k0 = deep * (wave % KS) / KS, k1 = deep * (wave % KS + 1) / KS;
+  const _Float16 *xa = Xh + (bi * 16 + i) * d.ldx + 8 * g, *xb = Xh + (bj * 16 + i) * d.ldx + 8 * g;
+  _Float16 *a_to = Ah + (bi * 16 + i) * d.lda + bj * 16 + 4 * g, *a_mirror = Ah + (bj * 16 + 4 * g) * d.lda + bi * 16 + i;
+  const int qi = wave / NB, qj = wave % NB;
+  const _Float16 *qa_from = Ah + (qi * 16 + i) * d.lda + 8 * g, *qb_from = Ah + (qj * 16 + i) * d.lda + 8 * g;
+  const int q_at = (qi * 16 + i) * d.lda + qj * 16 + 4 * g;
+  const bool split = NB * cbs <= 2 * SMALL_WAVES;
+  auto pair_at = [](const _Float16* q, int plane, u4v (&v)[2]) {
+    v[0] = *reinterpret_cast<const u4v*>(q);
+    v[1] = *reinterpret_cast<const u4v*>(q + plane);
+  };
+  // rows of X that a lane reads for Q X (16 lanes read 4 rows of 16 columns, and each gets a column's 4 rows)
+  int x_row[DEEP_M][2];
+  bool x_in[DEEP_M][2];
+#pragma unroll
+  for (int k = 0; k < DEEP_M; ++k)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = 32 * k + 8 * g + 4 * h + (i >> 2);
+      x_in[k][h] = row < d.m16;
+      x_row[k][h] = row * d.ldx + 4 * (i & 3);
+    }
+  auto read_x = [&](int cb, int k, u4v (&x)[2]) {
+#pragma unroll
+    for (int plane = 0; plane < 2; ++plane) {
+      u2v v[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const _Float16* q = x_in[k][h] ? Xh + plane * plane_x + x_row[k][h] + cb * 16 : zeros;
+        v[h] = __builtin_bit_cast(u2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*)q));
+      }
+      x[plane] = u4v{v[0][0], v[0][1], v[1][0], v[1][1]};
+    }
+  };
+  auto put_x = [&](int b, int cb, const f4v& acc) {
+    const float v[4] = {acc[0] * to_x, acc[1] * to_x, acc[2] * to_x, acc[3] * to_x};
+    store_pair4(Xh, Xl, (b * 16 + i) * d.ldx + cb * 16 + 4 * g, v);
+  };
   for (int step = 0; step < steps; ++step) {
     __syncthreads();
-    // A: the blocks on and below the diagonal over the waves, in ks pieces of X's columns where they are few
-    for (int task = wave; task < lower * ks; task += SMALL_WAVES) {
-      const int blk = task / ks, part = task - blk * ks;
-      int bi, bj;
-      triangle(blk, bi, bj);
+    if (has_a) {
       f4v acc = {0.f, 0.f, 0.f, 0.f};
-      const int k1 = deep * (part + 1) / ks;
-      for (int k = deep * part / ks; k < k1; ++k) {
-        const u4v a[2] = {line8(Xh, d.ldx, bi * 16, 32 * k), line8(Xl, d.ldx, bi * 16, 32 * k)};
-        const u4v b[2] = {line8(Xh, d.ldx, bj * 16, 32 * k), line8(Xl, d.ldx, bj * 16, 32 * k)};
-        acc = pair_products(b, a, acc);
+      u4v a[2], b[2];
+      if (k0 < k1) {
+        pair_at(xa + 32 * k0, plane_x, a);
+        pair_at(xb + 32 * k0, plane_x, b);
       }
-      if (ks > 1) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) P[task * 256 + i * 16 + 4 * g + r] = acc[r];
+      for (int k = k0; k < k1; ++k) {
+        u4v na[2], nb[2];
+        const int next = k + 1 < k1 ? k + 1 : k;
+        pair_at(xa + 32 * next, plane_x, na);
+        pair_at(xb + 32 * next, plane_x, nb);
+        acc = pair_products(b, a, acc);
+        a[0] = na[0], a[1] = na[1], b[0] = nb[0], b[1] = nb[1];
+      }
+      if constexpr (KS > 1) {
+        lds_st_fenced(reinterpret_cast<f4v*>(P + wave * 256 + i * 16 + 4 * g), acc);
       } else {
         const float v[4] = {acc[0] * to_a, acc[1] * to_a, acc[2] * to_a, acc[3] * to_a};
-        store_pair4(Ah, Al, (bi * 16 + i) * d.lda + bj * 16 + 4 * g, v);
+        store_pair4(a_to, a_to + plane_a, 0, v);
         if (bi != bj) {
           h4v h, lo;
           split4(v, h, lo);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            Ah[(bj * 16 + 4 * g + r) * d.lda + bi * 16 + i] = h[r];
-            Al[(bj * 16 + 4 * g + r) * d.lda + bi * 16 + i] = lo[r];
+            a_mirror[r * d.lda] = h[r];
+            a_mirror[r * d.lda + plane_a] = lo[r];
           }
         }
       }
     }
     __syncthreads();
-    if (ks > 1) {
-      for (int e = tid; e < lower * 256; e += SMALL_THREADS) {
-        int bi, bj;
-        triangle(e >> 8, bi, bj);
+    if constexpr (KS > 1) {
+      for (int e = tid; e < LOWER * 256; e += SMALL_THREADS) {
+        int ei, ej;
+        triangle(e >> 8, ei, ej);
         const int r = (e >> 4) & 15, c = e & 15;
         float v = 0.f;
-        for (int q = 0; q < ks; ++q) v += P[((e >> 8) * ks + q) * 256 + (e & 255)];
+#pragma unroll
+        for (int q = 0; q < KS; ++q) v += P[((e >> 8) * KS + q) * 256 + (e & 255)];
         v *= to_a;
         const _Float16 h = (_Float16)v, lo = (_Float16)(v - (float)h);
-        Ah[(bi * 16 + r) * d.lda + bj * 16 + c] = h;
-        Al[(bi * 16 + r) * d.lda + bj * 16 + c] = lo;
-        if (bi != bj) {
-          Ah[(bj * 16 + c) * d.lda + bi * 16 + r] = h;
-          Al[(bj * 16 + c) * d.lda + bi * 16 + r] = lo;
+        Ah[(ei * 16 + r) * d.lda + ej * 16 + c] = h;
+        Al[(ei * 16 + r) * d.lda + ej * 16 + c] = lo;
+        if (ei != ej) {
+          Ah[(ej * 16 + c) * d.lda + ei * 16 + r] = h;
+          Al[(ej * 16 + c) * d.lda + ei * 16 + r] = lo;
         }
       }
       __syncthreads();
     }
-    for (int task = wave; task < d.nb * d.nb; task += SMALL_WAVES) {
-      const int bi = task / d.nb, bj = task - bi * d.nb;
+    if (has_q) {
       f4v acc = {0.f, 0.f, 0.f, 0.f};
-      for (int k = 0; k < d.m32; k += 32) {
-        const u4v a[2] = {line8(Ah, d.lda, bi * 16, k), line8(Al, d.lda, bi * 16, k)};
-        const u4v b[2] = {line8(Ah, d.lda, bj * 16, k), line8(Al, d.lda, bj * 16, k)};
-        acc = pair_products(b, a, acc);
+      u4v a[DEEP_M][2], b[DEEP_M][2];
+#pragma unroll
+      for (int k = 0; k < DEEP_M; ++k) {
+        pair_at(qa_from + 32 * k, plane_a, a[k]);
+        pair_at(qb_from + 32 * k, plane_a, b[k]);
       }
-      const int row = bi * 16 + i, col = bj * 16 + 4 * g;
-      const h4v h = *reinterpret_cast<const h4v*>(Ah + row * d.lda + col), lo = *reinterpret_cast<const h4v*>(Al + row * d.lda + col);
+      const h4v h = *reinterpret_cast<const h4v*>(Ah + q_at), lo = *reinterpret_cast<const h4v*>(Al + q_at);
+#pragma unroll
+      for (int k = 0; k < DEEP_M; ++k) acc = pair_products(b[k], a[k], acc);
       float v[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = fmaf(qs, acc[r], fmaf(qb, (float)h[r] + (float)lo[r], row == col + r ? qa : 0.f));
-      store_pair4(Qh, Ql, row * d.lda + col, v);
+      for (int r = 0; r < 4; ++r)
+        v[r] = fmaf(qs, acc[r], fmaf(qb, (float)h[r] + (float)lo[r], qi == qj && i == 4 * g + r ? qa : 0.f));
+      store_pair4(Qh, Ql, q_at, v);
     }
     __syncthreads();
-    // X: a wave takes whole blocks of columns, which no other one reads: in place
-    for (int cb = wave; cb < d.n32 / 16; cb += SMALL_WAVES) {
-      f4v acc[4];
+    // X, in place.  With few blocks each wave takes one or two of 16 x 16, and everything is read before anything is written;
+    // with many it takes whole blocks of columns, which no other wave reads
+    if (split) {
+      f4v acc[2];
 #pragma unroll
-      for (int bi = 0; bi < 4; ++bi) acc[bi] = f4v{0.f, 0.f, 0.f, 0.f};
-      for (int k = 0; k < d.m32; k += 32) {
-        u4v x[2];
+      for (int k2 = 0; k2 < 2; ++k2) {
+        acc[k2] = f4v{0.f, 0.f, 0.f, 0.f};
+        const int task = wave + SMALL_WAVES * k2, b = task % NB, cb = task / NB;
+        if (cb >= cbs) continue;
+        u4v x[DEEP_M][2], q[DEEP_M][2];
 #pragma unroll
-        for (int plane = 0; plane < 2; ++plane) {
-          u2v v[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int row = k + 8 * g + 4 * h + (i >> 2);
-            const _Float16* q = row < d.m16 ? (plane ? Xl : Xh) + row * d.ldx + cb * 16 + 4 * (i & 3) : zeros + 4 * (i & 3);
-            v[h] = __builtin_bit_cast(u2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*)q));
-          }
-          x[plane] = u4v{v[0][0], v[0][1], v[1][0], v[1][1]};
+        for (int k = 0; k < DEEP_M; ++k) {
+          read_x(cb, k, x[k]);
+          pair_at(Qh + (b * 16 + i) * d.lda + 8 * g + 32 * k, plane_a, q[k]);
         }
 #pragma unroll
-        for (int bi = 0; bi < 4; ++bi)
-          if (bi < d.nb) {
-            const u4v q[2] = {line8(Qh, d.lda, bi * 16, k), line8(Ql, d.lda, bi * 16, k)};
-            acc[bi] = pair_products(x, q, acc[bi]);
-          }
+        for (int k = 0; k < DEEP_M; ++k) acc[k2] = pair_products(x[k], q[k], acc[k2]);
       }
+      __syncthreads();
 #pragma unroll
-      for (int bi = 0; bi < 4; ++bi)
-        if (bi < d.nb) {
-          const float v[4] = {acc[bi][0] * to_x, acc[bi][1] * to_x, acc[bi][2] * to_x, acc[bi][3] * to_x};
-          store_pair4(Xh, Xl, (bi * 16 + i) * d.ldx + cb * 16 + 4 * g, v);
+      for (int k2 = 0; k2 < 2; ++k2) {
+        const int task = wave + SMALL_WAVES * k2, b = task % NB, cb = task / NB;
+        if (cb < cbs) put_x(b, cb, acc[k2]);
+      }
+    } else {
+      for (int cb = wave; cb < cbs; cb += SMALL_WAVES) {
+        f4v acc[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[b] = f4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < DEEP_M; ++k) {
+          u4v x[2];
+          read_x(cb, k, x);
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            u4v q[2];
+            pair_at(Qh + (b * 16 + i) * d.lda + 8 * g + 32 * k, plane_a, q);
+            acc[b] = pair_products(x, q, acc[b]);
+          }
         }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) put_x(b, cb, acc[b]);
+      }
     }
   }
   __syncthreads();
@@ -739,23 +826,68 @@ __global__ void __launch_bounds__(SMALL_THREADS) ortho_small(const Args p, int s
   }
 }
 
+// Both: one workgroup for each matrix
+template <int BYTES, int N>
+__global__ void __launch_bounds__(SMALL_THREADS) ortho_small(const Table<N> p, int steps) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[BYTES];
+  __shared__ double red[SMALL_WAVES];
+  int matrix, unit;
+  const int it = locate(p, blockIdx.x, matrix, unit, [](const Item&) { return 1; });
+  if (it < 0) return;
+  const Item& t = p.item[it];
+  if (t.m > 48) run_lds<4>(p, t, matrix, steps, lds, red);
+  else if (t.m > 32) run_lds<3>(p, t, matrix, steps, lds, red);
+  else if (t.m > 16) run_lds<2>(p, t, matrix, steps, lds, red);
+  else if (t.n <= 256) run_rows16<1>(p, t, matrix, steps, lds, red);
+  else if (t.n <= 512) run_rows16<2>(p, t, matrix, steps, lds, red);
+  else run_rows16<8>(p, t, matrix, steps, lds, red);
+}
+
 // ---- host --------------------------------------------------------------------------------------------------------------
 
-constexpr int SMALL_SIZES[3] = {40960, 79872, 155648};   // bytes of LDS: four, two or one workgroup for a compute unit
-constexpr int KINDS = 6;
+constexpr int SMALL_SIZES[2] = {81920, 155648};   // bytes of LDS: two workgroups for a compute unit, or one
+static_assert(ROWS16_BYTES <= SMALL_SIZES[0], "rows16 fits");
 static inline int ceil_to(int v, int k) { return (v + k - 1) / k * k; }
 static inline int64_t up(int64_t v) { return (v + 255) / 256 * 256; }
 
-// How a matrix runs: -1 as tiles, 0 .. 2 in registers (blocks of 16 columns for each wave: 1, 4, 16), 3 .. 5 in LDS
-static int kind_of(int m, int n) {
-  if (m <= 16 && n <= 2048) return n <= 128 ? 0 : n <= 512 ? 1 : 2;
-  if (m > 64 || n > 65536) return -1;
+// How a matrix runs: -1 as tiles, 0 or 1 in one workgroup of that size
+static int kind_of(const nfi_ortho_item& q) {
+  const int m = std::min(q.rows, q.cols), n = std::max(q.rows, q.cols);
+  if (m <= 16 && n <= 2048) return 0;
+  if (m <= 16 || m > 64 || n > 65536) return -1;
   const int need = SmallShape(m, n).bytes();
-  for (int k = 0; k < 3; ++k)
-    if (need <= SMALL_SIZES[k]) return 3 + k;
-  return -1;
+  return need <= SMALL_SIZES[0] ? 0 : need <= SMALL_SIZES[1] ? 1 : -1;
 }
-static int kind_of(const nfi_ortho_item& q) { return kind_of(std::min(q.rows, q.cols), std::max(q.rows, q.cols)); }
+
+// the launches of a table's items, in the smallest table that holds them
+template <int N>
+static Table<N> smaller(const Table<ITEMS>& t) {
+  Table<N> r;
+  (Args&)r = t;
+  std::copy(t.item, t.item + std::min(t.items, N), r.item);
+  return r;
+}
+template <int N>
+static void launch_small(const Table<ITEMS>& a, int size, unsigned blocks, int steps, hipStream_t s) {
+  if (size == 0) ortho_small<SMALL_SIZES[0], N><<<blocks, SMALL_THREADS, 0, s>>>(smaller<N>(a), steps);
+  else ortho_small<SMALL_SIZES[1], N><<<blocks, SMALL_THREADS, 0, s>>>(smaller<N>(a), steps);
+}
+struct Grids {
+  int64_t chunks, starts, grams, tiles;
+};
+template <int N>
+static void launch_tiles(const Table<ITEMS>& a, const Grids& g, int steps, hipStream_t s) {
+  Table<N> t = smaller<N>(a);
+  ortho_norm<N><<<(unsigned)g.chunks, 256, 0, s>>>(t);
+  ortho_start<N><<<(unsigned)g.starts, 256, 0, s>>>(t);
+  for (int k = 0; k < steps; ++k) {
+    t.last = k == steps - 1;
+    ortho_gram<false, N><<<(unsigned)g.grams, 256, 0, s>>>(t);
+    ortho_gram<true, N><<<(unsigned)g.grams, 256, 0, s>>>(t);
+    ortho_apply<N><<<(unsigned)g.tiles, 256, 0, s>>>(t);
+    for (int i = 0; i < t.items; ++i) std::swap(t.item[i].x, t.item[i].y);
+  }
+}
 
 static int64_t item_bytes(const nfi_ortho_item& s) {
   const int m = std::min(s.rows, s.cols), n = std::max(s.rows, s.cols);
@@ -764,14 +896,22 @@ static int64_t item_bytes(const nfi_ortho_item& s) {
   return s.count * (2 * up(mp * np * 4) + 2 * up(mp * mp * 4)) + up(s.count * ((size + NORM_CHUNK - 1) / NORM_CHUNK) * 8);
 }
 
-// largest |s q(s^2)| and |q| over s in [0, top]
-static void bounds(float a, float b, float c, double top, double& x, double& q) {
+// largest |s q(s^2)| and |q| over s in [0, top], q(t) = a + b t + c t^2: at the ends or where a derivative is 0
+static void bounds(double a, double b, double c, double top, double& x, double& q) {
   x = q = 0.;
-  for (int k = 0; k <= 4096; ++k) {
-    const double s = top * k / 4096, t = s * s, v = a + t * (b + t * c);
-    x = std::max(x, std::fabs(s * v));
-    q = std::max(q, std::fabs(v));
-  }
+  auto at = [&](double t) {
+    if (!(t >= 0. && t <= top * top)) return;
+    const double v = std::fabs(a + t * (b + t * c));
+    x = std::max(x, std::sqrt(t) * v);
+    q = std::max(q, v);
+  };
+  at(0.);
+  at(top * top);
+  at(-b / (2. * c));
+  const double root = std::sqrt(9. * b * b - 20. * a * c);   // a + 3 b t + 5 c t^2 = 0
+  at((-3. * b + root) / (10. * c));
+  at((-3. * b - root) / (10. * c));
+  at(-a / (3. * b));
 }
 
 static int check(const nfi_ortho_args* p, double& most_x, double& most_q) {
@@ -792,7 +932,7 @@ static int check(const nfi_ortho_args* p, double& most_x, double& most_q) {
   most_x = 1.;
   most_q = 0.;
   for (int k = 0; k < p->steps; ++k) {
-    bounds(p->a, p->b, p->c, top * 1.0001, x, q);
+    bounds(p->a, p->b, p->c, top * 1.0001, x, q);   // (a division by 0 gives a point outside)
     most_x = std::max(most_x, x);
     most_q = std::max(most_q, q);
     top = x;
@@ -862,47 +1002,44 @@ int32_t nfi_ortho(const nfi_ortho_args* p, void* stream) {
     t.np = ceil_to(t.n, unit);
     return t;
   };
-  for (int kind = 0; kind < KINDS; ++kind) {
-    Args a = base;
+  // small matrices: in one launch if every compute unit gets one at most, else by size (two workgroups of the smaller
+  // for a unit)
+  int64_t counts[2] = {0, 0};
+  for (int i = 0; i < p->n_items; ++i)
+    if (kind_of(p->items[i]) >= 0) counts[kind_of(p->items[i])] += p->items[i].count;
+  const bool together = counts[0] + counts[1] <= 256 && counts[1] > 0;
+  for (int size = 0; size < 2; ++size) {
+    Table<ITEMS> a;
+    (Args&)a = base;
     int64_t blocks = 0;
     auto flush = [&]() {
-      if (a.items == 0) return;
-      const unsigned n = (unsigned)blocks;
-      if (kind == 0) ortho_rows16<1><<<n, 512, 0, s>>>(a, p->steps);
-      else if (kind == 1) ortho_rows16<4><<<n, 512, 0, s>>>(a, p->steps);
-      else if (kind == 2) ortho_rows16<16><<<n, 512, 0, s>>>(a, p->steps);
-      else if (kind == 3) ortho_small<SMALL_SIZES[0]><<<n, SMALL_THREADS, 0, s>>>(a, p->steps);
-      else if (kind == 4) ortho_small<SMALL_SIZES[1]><<<n, SMALL_THREADS, 0, s>>>(a, p->steps);
-      else ortho_small<SMALL_SIZES[2]><<<n, SMALL_THREADS, 0, s>>>(a, p->steps);
+      if (a.items == 1) launch_small<1>(a, size, (unsigned)blocks, p->steps, s);
+      else if (a.items > 0 && a.items <= 8) launch_small<8>(a, size, (unsigned)blocks, p->steps, s);
+      else if (a.items > 8) launch_small<ITEMS>(a, size, (unsigned)blocks, p->steps, s);
       a.items = 0;
       blocks = 0;
     };
     for (int i = 0; i < p->n_items; ++i) {
       const nfi_ortho_item& q = p->items[i];
-      if (kind_of(q) != kind) continue;
+      const int kind = kind_of(q);
+      if (kind < 0 || (together ? 1 : kind) != size) continue;
       a.item[a.items++] = item(q, 16);
       blocks += q.count;
       if (a.items == ITEMS) flush();
     }
     flush();
   }
-  Args a = base;
+  Table<ITEMS> a;
+  (Args&)a = base;
   unsigned char* work = (unsigned char*)p->work;
-  int64_t chunks = 0, starts = 0, grams = 0, tiles = 0;
+  Grids grids = {0, 0, 0, 0};
   auto flush = [&]() {
-    if (a.items == 0) return;
-    ortho_norm<<<(unsigned)chunks, 256, 0, s>>>(a);
-    ortho_start<<<(unsigned)starts, 256, 0, s>>>(a);
-    for (int k = 0; k < p->steps; ++k) {
-      a.last = k == p->steps - 1;
-      ortho_gram<false><<<(unsigned)grams, 256, 0, s>>>(a);
-      ortho_gram<true><<<(unsigned)grams, 256, 0, s>>>(a);
-      ortho_apply<<<(unsigned)tiles, 256, 0, s>>>(a);
-      for (int i = 0; i < a.items; ++i) std::swap(a.item[i].x, a.item[i].y);
-    }
-    a = base;
+    if (a.items == 1) launch_tiles<1>(a, grids, p->steps, s);
+    else if (a.items > 0 && a.items <= 8) launch_tiles<8>(a, grids, p->steps, s);
+    else if (a.items > 8) launch_tiles<ITEMS>(a, grids, p->steps, s);
+    a.items = 0;
     work = (unsigned char*)p->work;
-    chunks = starts = grams = tiles = 0;
+    grids = {0, 0, 0, 0};
   };
   for (int i = 0; i < p->n_items; ++i) {
     const nfi_ortho_item& q = p->items[i];
@@ -918,10 +1055,10 @@ int32_t nfi_ortho(const nfi_ortho_args* p, void* stream) {
     work += item_bytes(q);
     a.item[a.items++] = t;
     const int64_t mt = t.mp / TILE;
-    chunks += (int64_t)t.chunks * t.count;
-    starts += (int64_t)(t.mp / 64) * (t.np / 64) * t.count;
-    grams += mt * (mt + 1) / 2 * t.count;
-    tiles += mt * (t.np / TILE) * t.count;
+    grids.chunks += (int64_t)t.chunks * t.count;
+    grids.starts += (int64_t)(t.mp / 64) * (t.np / 64) * t.count;
+    grids.grams += mt * (mt + 1) / 2 * t.count;
+    grids.tiles += mt * (t.np / TILE) * t.count;
     if (a.items == ITEMS) flush();
   }
   flush();
