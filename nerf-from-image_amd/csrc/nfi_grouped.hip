@@ -79,81 +79,82 @@ __device__ __forceinline__ void store4(T* p, const float (&v)[4], int count) {
   }
 }
 
-// y (SLAB_B false: b = w[e], rows of K) and d x (SLAB_B true: a = dy, b = w[e] as slabs): rows of `a` by tiles
-template <class T, bool SLAB_B>
-__global__ void __launch_bounds__(256) grouped_rows(const GroupedArgs p) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * TILE_BYTES];
+// y (SLAB_B false: b = w[e], rows of K) and d x (SLAB_B true: a = dy, b = w[e] as slabs): rows of `a` by tiles of 128 x LB
+template <class T, bool SLAB_B, int LB>
+__global__ void __launch_bounds__(256, 2) grouped_rows(const GroupedArgs p) {
+  __shared__ __attribute__((aligned(16))) unsigned char s0[(TILE + LB) * STEP_BYTES], s1[(TILE + LB) * STEP_BYTES];
   const int64_t tile = blockIdx.x / p.col_tiles;
-  const int c0 = (int)(blockIdx.x % p.col_tiles) * TILE;
+  const int c0 = (int)(blockIdx.x % p.col_tiles) * LB;
   int64_t r0, r1;
   const int e = find_tile(p, tile, r0, r1);
   if (e < 0) return;
-  const int rows = (int)(r1 - r0), cols = min(TILE, p.n - c0);
-  f4v acc[4][4];
-#pragma unroll
-  for (int x = 0; x < 4; ++x)
-#pragma unroll
-    for (int y = 0; y < 4; ++y) acc[x][y] = f4v{0.f, 0.f, 0.f, 0.f};
+  const int rows = (int)(r1 - r0), cols = min(LB, p.n - c0);
+  Accumulate<T, 4, LB / 32, false> out;
+  out.clear();
   if (e < p.groups) {
     const unsigned char* b = p.b + e * p.sb + (SLAB_B ? (int64_t)c0 * (int)sizeof(T) : (int64_t)c0 * p.ldb);
-    tile_product<T, false, SLAB_B>(p.a + r0 * p.lda, p.lda, rows, b, p.ldb, cols, p.k, lds, acc);
+    tile_product<T, false, SLAB_B, TILE, LB>(p.a + r0 * p.lda, p.lda, rows, b, p.ldb, cols, p.k, s0, s1, out, false);
   }
   const int wave = threadIdx.x >> 6, i = lane_id() & 15, g = lane_id() >> 4;
 #pragma unroll
-  for (int y = 0; y < 4; ++y) {
-    const int n = (wave >> 1) * 64 + y * 16 + 4 * g;
+  for (int y = 0; y < LB / 32; ++y) {
+    const int n = (wave >> 1) * (LB / 2) + y * 16 + 4 * g;
     float bias[4] = {0.f, 0.f, 0.f, 0.f};
-    if (p.bias && e < p.groups)
-      for (int r = 0; r < 4; ++r)
-        if (n + r < cols) bias[r] = (float)((const T*)p.bias)[(int64_t)e * p.n + c0 + n + r];
+    if (p.bias && e < p.groups)   // (one after the other in flight: clamped, not skipped)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) bias[r] = (float)((const T*)p.bias)[(int64_t)e * p.n + c0 + min(n + r, cols - 1)];
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const int row = (wave & 1) * 64 + x * 16 + i;
       float v[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = acc[x][y][r] + bias[r];
+      for (int r = 0; r < 4; ++r) v[r] = out.acc[x][y][r] + bias[r];
       if (row < rows) store4<T>((T*)p.out + (r0 + row) * p.n + c0 + n, v, cols - n);
     }
   }
 }
 
-// d w[e] [N][K]: a = dy as slabs (its columns are the lines), b = x as slabs; blockIdx.y the group, .z the split
-template <class T>
-__global__ void __launch_bounds__(256) grouped_weights(const GroupedArgs p, int n_rows) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * TILE_BYTES];
+// d w[e] [N][K] and d b[e]: a = dy as slabs (its columns are the lines), b = x as slabs, tiles of L x L; blockIdx.y the group, .z the
+// split.  Partial results: part [split][group][N][K], then part_b [split][group][N].
+template <class T, int L>
+__global__ void __launch_bounds__(256, 2) grouped_weights(const GroupedArgs p, int n_rows, void* gb, float* part_b) {
+  __shared__ __attribute__((aligned(16))) unsigned char s0[2 * L * STEP_BYTES], s1[2 * L * STEP_BYTES];
   const int e = blockIdx.y;
-  const int m0 = (int)(blockIdx.x / p.col_tiles) * TILE, c0 = (int)(blockIdx.x % p.col_tiles) * TILE;
+  const int m0 = (int)(blockIdx.x / p.col_tiles) * L, c0 = (int)(blockIdx.x % p.col_tiles) * L;
   const int64_t s = offset_at(p.offsets, p.offsets64, e, p.rows), t = max(s, offset_at(p.offsets, p.offsets64, e + 1, p.rows));
   // pieces of whole steps
   constexpr int KSTEP = STEP_BYTES / sizeof(T);
   const int64_t piece = ((t - s + p.splits - 1) / p.splits + KSTEP - 1) / KSTEP * KSTEP;
   const int64_t r0 = min(t, s + blockIdx.z * piece), r1 = min(t, r0 + piece);
-  const int lines = min(TILE, n_rows - m0), cols = min(TILE, p.n - c0);
-  f4v acc[4][4];
-#pragma unroll
-  for (int x = 0; x < 4; ++x)
-#pragma unroll
-    for (int y = 0; y < 4; ++y) acc[x][y] = f4v{0.f, 0.f, 0.f, 0.f};
-  tile_product<T, true, true>(p.a + r0 * p.lda + m0 * (int64_t)sizeof(T), p.lda, lines, p.b + r0 * p.ldb + c0 * (int64_t)sizeof(T),
-                              p.ldb, cols, r1 - r0, lds, acc);
+  const int lines = min(L, n_rows - m0), cols = min(L, p.n - c0);
+  Accumulate<T, L / 32, L / 32, true> acc;
+  acc.clear();
+  const bool sums = gb != nullptr && c0 == 0;
+  tile_product<T, true, true, L, L>(p.a + r0 * p.lda + m0 * (int64_t)sizeof(T), p.lda, lines, p.b + r0 * p.ldb + c0 * (int64_t)sizeof(T),
+                                    p.ldb, cols, r1 - r0, s0, s1, acc, sums);
   const int wave = threadIdx.x >> 6, i = lane_id() & 15, g = lane_id() >> 4;
-  const int64_t matrix = (int64_t)n_rows * p.n;
+  const int64_t matrix = (int64_t)n_rows * p.n, place = (int64_t)blockIdx.z * p.groups + e;
 #pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    const int row = (wave & 1) * 64 + x * 16 + i;
+  for (int x = 0; x < L / 32; ++x) {
+    const int row = (wave & 1) * (L / 2) + x * 16 + i;
     if (row >= lines) continue;
+    if (sums && wave < 2 && g == 0) {
+      if (p.splits == 1) ((T*)gb)[(int64_t)e * n_rows + m0 + row] = (T)acc.sum[x][0];
+      else part_b[place * n_rows + m0 + row] = acc.sum[x][0];
+    }
+    if (p.out == nullptr) continue;
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      const int n = (wave >> 1) * 64 + y * 16 + 4 * g;
-      const float v[4] = {acc[x][y][0], acc[x][y][1], acc[x][y][2], acc[x][y][3]};
+    for (int y = 0; y < L / 32; ++y) {
+      const int n = (wave >> 1) * (L / 2) + y * 16 + 4 * g;
+      const float v[4] = {acc.acc[x][y][0], acc.acc[x][y][1], acc.acc[x][y][2], acc.acc[x][y][3]};
       const int64_t at = (int64_t)(m0 + row) * p.n + c0 + n;
       if (p.splits == 1) store4<T>((T*)p.out + e * matrix + at, v, cols - n);
-      else store4<float>(p.part + ((int64_t)blockIdx.z * p.groups + e) * matrix + at, v, cols - n);
+      else store4<float>(p.part + place * matrix + at, v, cols - n);
     }
   }
 }
 
-// d b[e]: 64 columns x 4 rows at a time; blockIdx.y the group, .z the split
+// d b[e] alone: 64 columns x 4 rows at a time; blockIdx.y the group, .z the split
 template <class T>
 __global__ void __launch_bounds__(256) grouped_bias(const GroupedArgs p) {
   __shared__ float lds[4][64];
@@ -175,25 +176,44 @@ __global__ void __launch_bounds__(256) grouped_bias(const GroupedArgs p) {
   }
 }
 
-// partial results summed in their order and rounded once
+// Partial results [splits][count] (and of a second array behind) summed in a fixed order and rounded once: 16 neighbours x 16
+// slices of the splits at a time
 template <class T>
-__global__ void __launch_bounds__(256) join_parts(const float* __restrict__ part, T* __restrict__ out, int64_t count, int splits) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= count) return;
+__global__ void __launch_bounds__(256) join_parts(const float* __restrict__ part, T* __restrict__ out, int64_t count,
+                                                  const float* __restrict__ part_b, T* __restrict__ out_b, int64_t count_b, int splits) {
+  __shared__ float lds[16][68];
+  int64_t at = (int64_t)blockIdx.x * 64 + (threadIdx.x & 15) * 4;
+  const int64_t first = (count + 63) / 64;   // (uniform) blocks of the first array
+  if (blockIdx.x >= first) {
+    at -= first * 64;
+    part = part_b;
+    out = out_b;
+    count = count_b;
+  }
+  const int slice = threadIdx.x >> 4, have = (int)min((int64_t)4, count - at);
   float v[4] = {0.f, 0.f, 0.f, 0.f};
-  const int have = (int)(count - i < 4 ? count - i : 4);
-  for (int s = 0; s < splits; ++s) {
-    const float* q = part + s * count + i;
-    if (have == 4) {
+  if (have == 4) {
+#pragma unroll 4
+    for (int s = slice; s < splits; s += 16) {
       float u[4];
-      load_piece<float, 4>(q, u);
+      load_piece<float, 4>(part + s * count + at, u);
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[r] += u[r];
-    } else {
-      for (int r = 0; r < have; ++r) v[r] += q[r];
     }
+  } else {
+    for (int s = slice; s < splits; s += 16)
+      for (int r = 0; r < have; ++r) v[r] += part[s * count + at + r];
   }
-  store4<T>(out + i, v, have);
+#pragma unroll
+  for (int r = 0; r < 4; ++r) lds_st_fenced(&lds[slice][(threadIdx.x & 15) * 4 + r], v[r]);
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  at += threadIdx.x - (int64_t)(threadIdx.x & 15) * 4;
+  if (at >= count) return;
+  float sum = 0.f;
+  const int used = splits < 16 ? splits : 16;
+  for (int k = 0; k < used; ++k) sum += lds[k][threadIdx.x];
+  out[at] = (T)sum;
 }
 
 // rows of `width` elements to rows of `padded`, zeros behind: a matrix whose rows are not aligned to 16 bytes
@@ -219,16 +239,35 @@ static inline int padded_width(int width, int es) { return (width * es + 15) / 1
 static inline bool rows_aligned(const void* p, int width, int es) { return ((uintptr_t)p & 15) == 0 && width * es % 16 == 0; }
 static inline int64_t up(int64_t v) { return (v + 255) / 256 * 256; }
 
-// The rows of a group are divided where the tiles alone are too few for 256 compute units with two workgroups
-// each; a piece keeps at least 256 rows of an average group
+// Tiles of the weights' gradients: 64 where a side is no larger (a 128 tile would be half empty)
+static int weight_tile(int n, int k) { return std::min(n, k) <= 64 ? 64 : TILE; }
+static int64_t tiles_of(int n, int k, int tile) { return (int64_t)((n + tile - 1) / tile) * ((k + tile - 1) / tile); }
+
+// The rows of a group are divided where the tiles alone are too few for 256 compute units with two workgroups (of 128 tiles) or
+// three (of 64) each; a piece keeps at least 128 rows of an average group
 static int weight_splits(int64_t rows, int groups, int n, int k) {
-  const int64_t tiles = (int64_t)groups * ((n + TILE - 1) / TILE) * ((k + TILE - 1) / TILE);
-  const int64_t want = 1024 / std::max<int64_t>(1, tiles), most = rows / groups / 256;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 64));
+  const int tile = weight_tile(n, k);
+  const int64_t tiles = groups * tiles_of(n, k, tile);
+  const int64_t want = (tile == TILE ? 512 : 768) / tiles, most = rows / groups / 128;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 256));
 }
 static int bias_splits(int64_t rows, int groups, int n) {
   const int64_t tiles = (int64_t)groups * ((n + 63) / 64);
   return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(1024 / tiles, rows / groups / 32), 64));
+}
+
+template <class T>
+static void launch_rows(GroupedArgs& p, bool slab, hipStream_t s) {
+  const int lb = p.n <= 64 ? 64 : TILE;   // (half of a 128 tile would be empty)
+  p.col_tiles = (p.n + lb - 1) / lb;
+  const unsigned tiles = (unsigned)(((p.rows + TILE - 1) / TILE + std::min<int64_t>(p.groups + 2, p.rows)) * p.col_tiles);
+  if (slab) {
+    if (lb == 64) grouped_rows<T, true, 64><<<tiles, 256, 0, s>>>(p);
+    else grouped_rows<T, true, TILE><<<tiles, 256, 0, s>>>(p);
+  } else {
+    if (lb == 64) grouped_rows<T, false, 64><<<tiles, 256, 0, s>>>(p);
+    else grouped_rows<T, false, TILE><<<tiles, 256, 0, s>>>(p);
+  }
 }
 
 template <class T>
@@ -258,9 +297,7 @@ static void forward(const nfi_grouped_args& a, hipStream_t s) {
   p.groups = a.groups;
   p.n = a.out_width;
   p.k = a.in_width;
-  p.col_tiles = (a.out_width + TILE - 1) / TILE;
-  const int64_t tiles = ((a.rows + TILE - 1) / TILE + std::min<int64_t>(a.groups + 2, a.rows)) * p.col_tiles;
-  grouped_rows<T, false><<<(unsigned)tiles, 256, 0, s>>>(p);
+  launch_rows<T>(p, false, s);
 }
 
 template <class T>
@@ -281,9 +318,7 @@ static void backward(const nfi_grouped_args& a, hipStream_t s) {
     p.out = a.gx;
     p.n = a.in_width;
     p.k = a.out_width;
-    p.col_tiles = (a.in_width + TILE - 1) / TILE;
-    const int64_t tiles = ((a.rows + TILE - 1) / TILE + std::min<int64_t>(a.groups + 2, a.rows)) * p.col_tiles;
-    grouped_rows<T, true><<<(unsigned)tiles, 256, 0, s>>>(p);
+    launch_rows<T>(p, true, s);
   }
   if (a.gw) {
     p.a = g;
@@ -291,16 +326,18 @@ static void backward(const nfi_grouped_args& a, hipStream_t s) {
     p.b = padded<T>(a.x, a.rows, a.in_width, work, p.ldb, s);
     p.out = a.gw;
     p.n = a.in_width;
-    p.col_tiles = (a.in_width + TILE - 1) / TILE;
+    const int tile = weight_tile(a.out_width, a.in_width);
+    p.col_tiles = (a.in_width + tile - 1) / tile;
     p.splits = weight_splits(a.rows, a.groups, a.out_width, a.in_width);
     p.part = (float*)work;
-    const int64_t count = (int64_t)a.groups * a.out_width * a.in_width;
-    if (p.splits > 1) work += up(count * 4 * p.splits);
-    grouped_weights<T><<<dim3((unsigned)((a.out_width + TILE - 1) / TILE * p.col_tiles), (unsigned)a.groups, (unsigned)p.splits), 256, 0, s>>>(
-        p, a.out_width);
-    if (p.splits > 1) join_parts<T><<<(unsigned)((count + 1023) / 1024), 256, 0, s>>>(p.part, (T*)a.gw, count, p.splits);
-  }
-  if (a.gb) {
+    const int64_t count = (int64_t)a.groups * a.out_width * a.in_width, count_b = a.gb ? (int64_t)a.groups * a.out_width : 0;
+    float* part_b = p.part + count * p.splits;
+    const dim3 grid((unsigned)tiles_of(a.out_width, a.in_width, tile), (unsigned)a.groups, (unsigned)p.splits);
+    if (tile == TILE) grouped_weights<T, TILE><<<grid, 256, 0, s>>>(p, a.out_width, a.gb, part_b);
+    else grouped_weights<T, 64><<<grid, 256, 0, s>>>(p, a.out_width, a.gb, part_b);
+    if (p.splits > 1)
+      join_parts<T><<<(unsigned)((count + 63) / 64 + (count_b + 63) / 64), 256, 0, s>>>(p.part, (T*)a.gw, count, part_b, (T*)a.gb, count_b, p.splits);
+  } else if (a.gb) {
     p.a = (const unsigned char*)a.gy;
     p.out = a.gb;
     p.n = a.out_width;
@@ -308,7 +345,7 @@ static void backward(const nfi_grouped_args& a, hipStream_t s) {
     p.part = (float*)work;
     const int64_t count = (int64_t)a.groups * a.out_width;
     grouped_bias<T><<<dim3((unsigned)((a.out_width + 63) / 64), (unsigned)a.groups, (unsigned)p.splits), 256, 0, s>>>(p);
-    if (p.splits > 1) join_parts<T><<<(unsigned)((count + 1023) / 1024), 256, 0, s>>>(p.part, (T*)a.gb, count, p.splits);
+    if (p.splits > 1) join_parts<T><<<(unsigned)((count + 63) / 64), 256, 0, s>>>(p.part, (T*)a.gb, count, p.part, (T*)a.gb, 0, p.splits);
   }
 }
 
@@ -321,7 +358,7 @@ static int check(const nfi_grouped_args* a, const char* what) {
   NFI_REQUIRE(a->in_width > 0 && a->in_width <= NFI_GROUPED_MAX_WIDTH && a->out_width > 0 && a->out_width <= NFI_GROUPED_MAX_WIDTH,
               "%s: widths %d -> %d (1 .. %d)", what, a->in_width, a->out_width, NFI_GROUPED_MAX_WIDTH);
   const int64_t widest = std::max(a->in_width, a->out_width);
-  NFI_REQUIRE(((a->rows + TILE - 1) / TILE + a->groups + 2) * ((widest + TILE - 1) / TILE) < (1ll << 31), "%s: too many tiles", what);
+  NFI_REQUIRE(((a->rows + TILE - 1) / TILE + a->groups + 2) * ((widest + 63) / 64) < (1ll << 31), "%s: too many tiles", what);
   return NFI_OK;
 }
 
@@ -353,9 +390,8 @@ int64_t nfi_grouped_backward_work_bytes(const nfi_grouped_args* a) {
   if (a->gw) {
     n += pad_bytes(a->x, a->rows, a->in_width, es);
     const int s = weight_splits(a->rows, a->groups, a->out_width, a->in_width);
-    if (s > 1) n += up((int64_t)a->groups * a->out_width * a->in_width * 4 * s);
-  }
-  if (a->gb) n += up((int64_t)a->groups * a->out_width * 4 * bias_splits(a->rows, a->groups, a->out_width));
+    if (s > 1) n += up((int64_t)a->groups * a->out_width * (a->in_width + (a->gb ? 1 : 0)) * 4 * s);
+  } else if (a->gb) n += up((int64_t)a->groups * a->out_width * 4 * bias_splits(a->rows, a->groups, a->out_width));
   return n;
 }
 

@@ -1,18 +1,21 @@
 // Tiles of a matrix product on the matrix cores, fed by loads that go straight to LDS (gfx950).
 //
-// An operand tile is 128 "lines" of 128 bytes of the contracted index (64 16-bit or 32 32-bit values),
-// 16 KB, in one of two layouts:
-//   lines   the operand's rows hold the contracted index contiguously: LDS [128 lines][8 pieces of 16 B],
-//           piece p of line r stored at p ^ (r & 7), so that the 16-byte reads of 8 lines use all banks
+// An operand tile is 64 or 128 "lines" of 128 bytes of the contracted index (64 16-bit or 32 32-bit values), 8 or 16 KB, in
+// one of two layouts:
+//   lines   the operand's rows hold the contracted index contiguously: LDS [lines][8 pieces of 16 B], piece p of line
+//           r stored at p ^ (r & 7), so that the 16-byte reads of 8 lines use all banks
 //   slabs   the contracted index runs over rows and the lines are columns (a transposed operand): LDS
-//           [64 or 32 rows][128 columns]; 16-bit fragments are read with the transposing LDS load, 32-bit
-//           ones word by word.  Pieces are exchanged by the row so that the rows of one read lie in
-//           different banks.
+//           [64 or 32 rows][columns]; 16-bit fragments are read with the transposing LDS load, 32-bit ones word by
+//           word.  Pieces are exchanged by the row so that the rows of one read lie in different banks.
 // Both give a lane the same contracted indices in the same order, so any two layouts meet in one product:
-// 16-bit: lane (i, g) = (l & 15, l >> 4) holds k = 32 sub + 8 g .. + 7;  32-bit: k = 16 sub + 4 g + s for
-// the s-th product of a sub-step.
+// 16-bit: lane (i, g) = (l & 15, l >> 4) holds k = 32 sub + 8 g .. + 7;  32-bit: k = 16 sub + 4 g .. + 3.
 // Loads go through a buffer descriptor whose range no lane out of the matrix falls into: such a lane's
 // offset is 2^31, and the hardware writes zeros.
+//
+// 32-bit values meet as three bf16 ones each, v = h + m + l (24 bits in 8 + 8 + 8, exactly), in six products l h + h l + m m +
+// m h + h m + h h on the bf16 matrix cores: 96 clocks of them for 32 contracted values against 256 of
+// v_mfma_f32_16x16x4_f32, and what is left out is at most 2^-24 of a product.  (An infinity, or a value that bf16 rounds to
+// one, leaves NaN: its parts m and l are no numbers.)
 #pragma once
 #include "nfi_learn.h"
 
@@ -43,24 +46,25 @@ __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, unsigned c
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, (int)offset, 0, 0, 0);
 }
 
-// The loads of one operand tile by a workgroup of 4 waves: 4 of 1 KB for each wave, at fixed offsets from
-// an address that moves by a step (lines: 128 bytes, slabs: a step's rows)
-template <class T, bool SLAB>
+// The loads of one operand tile of LINES lines by a workgroup of 4 waves: LINES / 32 of 1 KB for each wave, at fixed offsets
+// from an address that moves by a step (lines: 128 bytes, slabs: a step's rows)
+template <class T, bool SLAB, int LINES>
 struct TileLoad {
   static constexpr int KSTEP = STEP_BYTES / sizeof(T);
-  static constexpr int PIECES = SLAB ? TILE * (int)sizeof(T) / 16 : 8;   // 16-byte pieces of an LDS row
-  unsigned off[4];    // byte offset of each of this lane's pieces, NOWHERE out of the lines
-  int k[4];           // contracted byte (lines) or row (slabs) of the piece within the step
+  static constexpr int LOADS = LINES / 32;
+  static constexpr int PIECES = SLAB ? LINES * (int)sizeof(T) / 16 : 8;   // 16-byte pieces of an LDS row
+  unsigned off[LOADS];    // byte offset of each of this lane's pieces, NOWHERE out of the lines
+  int k[LOADS];           // contracted byte (lines) or row (slabs) of the piece within the step
 
-  static __device__ __forceinline__ int lds_row(int j) { return ((threadIdx.x >> 6) * 4 + j) * (64 / PIECES) + (lane_id() / PIECES); }
+  static __device__ __forceinline__ int lds_row(int j) { return ((threadIdx.x >> 6) * LOADS + j) * (64 / PIECES) + (lane_id() / PIECES); }
   static __device__ __forceinline__ int swizzle(int row) {
     if (!SLAB) return row & 7;
-    return sizeof(T) == 2 ? 2 * (row & 7) : 4 * ((row >> 2) & 3);
+    return sizeof(T) == 2 ? (2 * row) & (PIECES - 1) & 15 : 4 * ((row >> 2) & 3);
   }
   // `lines` valid lines (rows of the operand, or columns of a slab); ld: bytes between the operand's rows
   __device__ __forceinline__ void init(int lines, unsigned ld) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < LOADS; ++j) {
       const int row = lds_row(j), piece = (lane_id() & (PIECES - 1)) ^ swizzle(row);
       if (SLAB) {
         k[j] = row;
@@ -74,20 +78,16 @@ struct TileLoad {
   // left: contracted bytes (lines) or rows (slabs) that remain at this step
   __device__ __forceinline__ void issue(const void* base, unsigned char* lds, int left) const {
     const __amdgpu_buffer_rsrc_t r = descriptor(base);
-    unsigned char* dst = lds + (threadIdx.x >> 6) * 4096;
-    if (left >= (SLAB ? KSTEP : STEP_BYTES)) {
+    unsigned char* dst = lds + (threadIdx.x >> 6) * (LOADS * 1024);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) load_to_lds(r, dst + j * 1024, off[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) load_to_lds(r, dst + j * 1024, k[j] < left ? off[j] : NOWHERE);
-    }
+    for (int j = 0; j < LOADS; ++j) load_to_lds(r, dst + j * 1024, k[j] < left ? off[j] : NOWHERE);
   }
 };
 
-// Fragments of N 16-line blocks from line `line0`, for one sub-step
-template <class T, bool SLAB, int N>
+// Fragments of N 16-line blocks from line `line0`, for one sub-step, of a tile of LINES lines
+template <class T, bool SLAB, int LINES, int N>
 __device__ __forceinline__ void read_fragments(const unsigned char* lds, int line0, int sub, u4v (&f)[N]) {
+  typedef TileLoad<T, SLAB, LINES> L;
   const int i = lane_id() & 15, g = lane_id() >> 4;
   if constexpr (!SLAB) {
 #pragma unroll
@@ -105,7 +105,7 @@ __device__ __forceinline__ void read_fragments(const unsigned char* lds, int lin
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int row = r0 + 4 * h;
-        const unsigned char* p = lds + row * 256 + ((piece ^ (2 * (row & 7))) << 4) + half;
+        const unsigned char* p = lds + row * (L::PIECES * 16) + ((piece ^ L::swizzle(row)) << 4) + half;
         v[h] = __builtin_bit_cast(u2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*)p));
       }
       f[x] = u4v{v[0][0], v[0][1], v[1][0], v[1][1]};
@@ -117,7 +117,7 @@ __device__ __forceinline__ void read_fragments(const unsigned char* lds, int lin
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
         const int row = 16 * sub + 4 * g + s;   // (row >> 2) & 3 == g
-        f[x][s] = *reinterpret_cast<const unsigned*>(lds + row * 512 + (((col >> 2) ^ (4 * g)) << 4) + (col & 3) * 4);
+        f[x][s] = *reinterpret_cast<const unsigned*>(lds + row * (L::PIECES * 16) + (((col >> 2) ^ (4 * g)) << 4) + (col & 3) * 4);
       }
     }
   }
@@ -138,44 +138,150 @@ __device__ __forceinline__ f4v product(u4v b, u4v a, f4v acc) {
   }
 }
 
-// A 128 x 128 product tile by 4 waves of 64 x 64: steps over the contracted index, two stages of LDS (2 x 32
-// KB), the next step's loads in flight during a step's products.  `left` and the strides: TileLoad::issue.
-template <class T, bool SLAB_A, bool SLAB_B>
+// 8 32-bit values as three bf16 each (to nearest: each part's remainder is half a step of it, so that the products left out,
+// m l and l m, are 2^-25 of the whole)
+typedef float f2v __attribute__((ext_vector_type(2)));
+typedef __bf16 b2v __attribute__((ext_vector_type(2)));
+struct Thirds {
+  u4v h, m, l;
+  static __device__ __forceinline__ unsigned part(f2v& v) {
+    const unsigned p = __builtin_bit_cast(unsigned, __builtin_convertvector(v, b2v));
+    v[0] -= __uint_as_float(p << 16);
+    v[1] -= __uint_as_float(p & 0xffff0000u);
+    return p;
+  }
+  __device__ __forceinline__ void set(const u4v& v0, const u4v& v1) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      f2v v = k < 2 ? f2v{__uint_as_float(v0[2 * k]), __uint_as_float(v0[2 * k + 1])}
+                    : f2v{__uint_as_float(v1[2 * k - 4]), __uint_as_float(v1[2 * k - 3])};
+      h[k] = part(v);
+      m[k] = part(v);
+      l[k] = __builtin_bit_cast(unsigned, __builtin_convertvector(v, b2v));
+    }
+  }
+};
+__device__ __forceinline__ f4v product(const Thirds& b, const Thirds& a, f4v acc) {
+  acc = product<bf16_t>(b.l, a.h, acc);
+  acc = product<bf16_t>(b.h, a.l, acc);
+  acc = product<bf16_t>(b.m, a.m, acc);
+  acc = product<bf16_t>(b.m, a.h, acc);
+  acc = product<bf16_t>(b.h, a.m, acc);
+  return product<bf16_t>(b.h, a.h, acc);
+}
+
+// vmcnt(n), nothing else (n < 64)
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | ((N >> 4) << 14));
+}
+
+// A barrier alone: __syncthreads() also waits for every load on its way to LDS, those of the next step too
+__device__ __forceinline__ void bare_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// What is done with a step's fragments: acc[x][y] += a's block x, b's block y; with SUM also sum[x] += a's lines
+template <class T, int NA, int NB, bool SUM>
+struct Accumulate {
+  f4v acc[NA][NB], sum[NA];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int x = 0; x < NA; ++x) {
+      sum[x] = f4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int y = 0; y < NB; ++y) acc[x][y] = f4v{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  __device__ __forceinline__ void step(const u4v (&fa)[2][NA], const u4v (&fb)[2][NB], bool sums) {
+    if constexpr (sizeof(T) == 4) {
+      Thirds a[NA], b[NB];
+#pragma unroll
+      for (int x = 0; x < NA; ++x) a[x].set(fa[0][x], fa[1][x]);
+#pragma unroll
+      for (int y = 0; y < NB; ++y) b[y].set(fb[0][y], fb[1][y]);
+#pragma unroll
+      for (int x = 0; x < NA; ++x)
+#pragma unroll
+        for (int y = 0; y < NB; ++y) acc[x][y] = product(b[y], a[x], acc[x][y]);
+      if (SUM && sums) {
+        const unsigned one = 0x3f803f80u;
+        const u4v ones = {one, one, one, one};
+#pragma unroll
+        for (int x = 0; x < NA; ++x) {
+          sum[x] = product<bf16_t>(ones, a[x].l, sum[x]);
+          sum[x] = product<bf16_t>(ones, a[x].m, sum[x]);
+          sum[x] = product<bf16_t>(ones, a[x].h, sum[x]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int x = 0; x < NA; ++x)
+#pragma unroll
+          for (int y = 0; y < NB; ++y) acc[x][y] = product<T>(fb[sub][y], fa[sub][x], acc[x][y]);
+      if (SUM && sums) {
+        const unsigned one = TypeCode<T>::V == NFI_BF16 ? 0x3f803f80u : 0x3c003c00u;
+        const u4v ones = {one, one, one, one};
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+          for (int x = 0; x < NA; ++x) sum[x] = product<T>(ones, fa[sub][x], sum[x]);
+      }
+    }
+  }
+};
+
+// An LA x LB product tile by 4 waves of (LA / 2) x (LB / 2): steps over the contracted index through two stages of LDS, each of
+// (LA + LB) x 128 bytes.  A step's fragments go to registers at once, its stage is free after a barrier, and the loads of the step
+// after next are made into it while the step's products run: loads have a whole step to arrive.  (The stages are two variables of
+// their own: the compiler waits for all loads into the one that is read, and for no others.)
+template <class T, bool SLAB_A, bool SLAB_B, int LA, int LB, bool SUM>
 __device__ __forceinline__ void tile_product(const unsigned char* a, unsigned lda, int lines_a, const unsigned char* b, unsigned ldb,
-                                             int lines_b, int64_t contracted, unsigned char* lds, f4v (&acc)[4][4]) {
-  constexpr int KSTEP = STEP_BYTES / sizeof(T);
-  TileLoad<T, SLAB_A> la;
-  TileLoad<T, SLAB_B> lb;
+                                             int lines_b, int64_t contracted, unsigned char* s0, unsigned char* s1,
+                                             Accumulate<T, LA / 32, LB / 32, SUM>& out, bool sums) {
+  constexpr int KSTEP = STEP_BYTES / sizeof(T), NA = LA / 32, NB = LB / 32, LOADS = NA + NB;
+  TileLoad<T, SLAB_A, LA> la;
+  TileLoad<T, SLAB_B, LB> lb;
   la.init(lines_a, lda);
   lb.init(lines_b, ldb);
   const int64_t step_a = SLAB_A ? (int64_t)KSTEP * lda : STEP_BYTES, step_b = SLAB_B ? (int64_t)KSTEP * ldb : STEP_BYTES;
   const int steps = (int)((contracted + KSTEP - 1) / KSTEP);
-  const int wave = threadIdx.x >> 6, line_a = (wave & 1) * 64, line_b = (wave >> 1) * 64;
+  const int wave = threadIdx.x >> 6, line_a = (wave & 1) * (LA / 2), line_b = (wave >> 1) * (LB / 2);
+  // (a step behind the last reads nothing and clears its stage: every step waits for the same number of loads)
   auto issue = [&](int t, unsigned char* dst) {
     const int64_t k = contracted - (int64_t)t * KSTEP;
     const int left = (int)(k < KSTEP ? k : KSTEP);
     la.issue(a + t * step_a, dst, SLAB_A ? left : left * (int)sizeof(T));
-    lb.issue(b + t * step_b, dst + TILE_BYTES, SLAB_B ? left : left * (int)sizeof(T));
+    lb.issue(b + t * step_b, dst + LA * STEP_BYTES, SLAB_B ? left : left * (int)sizeof(T));
+    __builtin_amdgcn_sched_barrier(0);   // the waits count on this order of the steps' loads
   };
-  if (steps > 0) issue(0, lds);
-  for (int t = 0; t < steps; ++t) {
-    const unsigned char* cur = lds + (t & 1) * 2 * TILE_BYTES;
-    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's loads of step t are in LDS
-    __syncthreads();
-    u4v fa[2][4], fb[2][4];
+  auto step = [&](int t, unsigned char* cur) {
+    wait_loads<LOADS>();   // step t's loads are in LDS, those of step t + 1 may be on their way
+    bare_barrier();
+    u4v fa[2][NA], fb[2][NB];
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
-      read_fragments<T, SLAB_A, 4>(cur, line_a, sub, fa[sub]);
-      read_fragments<T, SLAB_B, 4>(cur + TILE_BYTES, line_b, sub, fb[sub]);
+      read_fragments<T, SLAB_A, LA, NA>(cur, line_a, sub, fa[sub]);
+      read_fragments<T, SLAB_B, LB, NB>(cur + LA * STEP_BYTES, line_b, sub, fb[sub]);
     }
-    if (t + 1 < steps) issue(t + 1, lds + ((t + 1) & 1) * 2 * TILE_BYTES);   // (last read before the barrier above)
-#pragma unroll
-    for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-#pragma unroll
-        for (int y = 0; y < 4; ++y) acc[x][y] = product<T>(fb[sub][y], fa[sub][x], acc[x][y]);
+    __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): this wave has read the step
+    bare_barrier();
+    issue(t + 2, cur);
+    out.step(fa, fb, sums);
+  };
+  issue(0, s0);
+  issue(1, s1);
+  int t = 0;
+  for (; t + 2 <= steps; t += 2) {
+    step(t, s0);
+    step(t + 1, s1);
   }
+  if (t < steps) step(t, s0);
+  wait_loads<0>();
 }
 
 }  // namespace learn

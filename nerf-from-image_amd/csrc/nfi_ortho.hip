@@ -226,7 +226,7 @@ __device__ __forceinline__ void read_pair_slab(const unsigned char* lds, int lin
 template <bool SLAB, bool SWAP>
 __device__ __forceinline__ void pair_product(const _Float16* a, unsigned lda, const _Float16* b, unsigned ldb, int k, unsigned char* lds,
                                              f4v (&acc)[4][4]) {
-  TileLoad<_Float16, false> la, lb;
+  TileLoad<_Float16, false, TILE> la, lb;
   PairSlab sb;
   la.init(TILE, lda);
   if (SLAB) sb.init(ldb);
@@ -251,9 +251,9 @@ __device__ __forceinline__ void pair_product(const _Float16* a, unsigned lda, co
     u4v fa[2][4], fb[2][4];
 #pragma unroll
     for (int plane = 0; plane < 2; ++plane) {
-      read_fragments<_Float16, false, 4>(cur, line_a, plane, fa[plane]);
+      read_fragments<_Float16, false, TILE, 4>(cur, line_a, plane, fa[plane]);
       if (SLAB) read_pair_slab<4>(cur + TILE_BYTES, line_b, plane, fb[plane]);
-      else read_fragments<_Float16, false, 4>(cur + TILE_BYTES, line_b, plane, fb[plane]);
+      else read_fragments<_Float16, false, TILE, 4>(cur + TILE_BYTES, line_b, plane, fb[plane]);
     }
     if (t + 1 < steps) issue(t + 1, lds + ((t + 1) & 1) * 2 * TILE_BYTES);
 #pragma unroll
