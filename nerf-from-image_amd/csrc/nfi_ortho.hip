@@ -32,8 +32,9 @@ struct Item {
   void* w;
   _Float16 *x, *y, *a, *q;    // workspace: X and the next X [mp][2 np], A and Q [mp][2 mp]
   double* sums;               // [count][chunks]
+  float* part;                // partial tiles of A or Q where the contracted index is split
   float scale;                // the step's factor of this matrix
-  int rows, cols, count, m, n, mp, np, chunks;
+  int rows, cols, count, m, n, mp, np, chunks, split_a, split_q;
 };
 
 struct Args {
@@ -59,7 +60,7 @@ template <int N, class F>
 __device__ __forceinline__ int locate(const Table<N>& p, int id, int& matrix, int& unit, F per) {
   for (int i = 0; i < p.items; ++i) {
     const int u = per(p.item[i]), all = u * p.item[i].count;
-    if (id < all) {
+    if (id < all) {   // (not for an item without units)
       matrix = id / u;
       unit = id - matrix * u;
       return i;
@@ -221,33 +222,34 @@ __device__ __forceinline__ void read_pair_slab(const unsigned char* lds, int lin
   }
 }
 
-// acc (a's lines by lane, b's by register) of a 128 x 128 tile; K a multiple of 32, everything inside the padding.
-// a: lines; b: lines, or (SLAB) rows of the contracted index; SWAP: the roles of lane and register exchanged
+// acc (a's lines by lane, b's by register) of a 128 x 128 tile over `steps` steps of 32; everything inside the padding.
+// a: lines; b: lines, or (SLAB) rows of the contracted index; SWAP: the roles of lane and register exchanged.  Two stages, loads
+// two steps ahead (tile_product in nfi_mm.h).
 template <bool SLAB, bool SWAP>
-__device__ __forceinline__ void pair_product(const _Float16* a, unsigned lda, const _Float16* b, unsigned ldb, int k, unsigned char* lds,
-                                             f4v (&acc)[4][4]) {
+__device__ __forceinline__ void pair_product(const _Float16* a, unsigned lda, const _Float16* b, unsigned ldb, int steps, unsigned char* s0,
+                                             unsigned char* s1, f4v (&acc)[4][4]) {
   TileLoad<_Float16, false, TILE> la, lb;
   PairSlab sb;
   la.init(TILE, lda);
   if (SLAB) sb.init(ldb);
   else lb.init(TILE, ldb);
   const int64_t step_b = SLAB ? (int64_t)32 * ldb : STEP_BYTES;
-  const int wave = threadIdx.x >> 6, line_a = (wave & 1) * 64, line_b = (wave >> 1) * 64, steps = k / 32;
+  const int wave = threadIdx.x >> 6, line_a = (wave & 1) * 64, line_b = (wave >> 1) * 64;
   const unsigned char *pa = (const unsigned char*)a, *pb = (const unsigned char*)b;
   auto issue = [&](int t, unsigned char* dst) {
+    t = min(t, steps - 1);   // (behind the last step that one again: every step waits for the same number of loads)
     la.issue(pa + (int64_t)t * STEP_BYTES, dst, STEP_BYTES);
     if (SLAB) sb.issue(pb + t * step_b, dst + TILE_BYTES);
     else lb.issue(pb + t * step_b, dst + TILE_BYTES, STEP_BYTES);
+    __builtin_amdgcn_sched_barrier(0);   // the waits count on this order of the steps' loads
   };
 #pragma unroll
   for (int x = 0; x < 4; ++x)
 #pragma unroll
     for (int y = 0; y < 4; ++y) acc[x][y] = f4v{0.f, 0.f, 0.f, 0.f};
-  issue(0, lds);
-  for (int t = 0; t < steps; ++t) {
-    const unsigned char* cur = lds + (t & 1) * 2 * TILE_BYTES;
-    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's loads of step t are in LDS
-    __syncthreads();
+  auto step = [&](int t, unsigned char* cur) {
+    wait_loads<8>();
+    bare_barrier();
     u4v fa[2][4], fb[2][4];
 #pragma unroll
     for (int plane = 0; plane < 2; ++plane) {
@@ -255,7 +257,9 @@ __device__ __forceinline__ void pair_product(const _Float16* a, unsigned lda, co
       if (SLAB) read_pair_slab<4>(cur + TILE_BYTES, line_b, plane, fb[plane]);
       else read_fragments<_Float16, false, TILE, 4>(cur + TILE_BYTES, line_b, plane, fb[plane]);
     }
-    if (t + 1 < steps) issue(t + 1, lds + ((t + 1) & 1) * 2 * TILE_BYTES);
+    __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): this wave has read the step
+    bare_barrier();
+    issue(t + 2, cur);
 #pragma unroll
     for (int pair = 0; pair < 3; ++pair)   // lo hi, hi lo, hi hi: the small ones first
 #pragma unroll
@@ -265,28 +269,38 @@ __device__ __forceinline__ void pair_product(const _Float16* a, unsigned lda, co
           const u4v va = fa[pair == 0][x], vb = fb[pair == 1][y];
           acc[x][y] = SWAP ? product<_Float16>(va, vb, acc[x][y]) : product<_Float16>(vb, va, acc[x][y]);
         }
+  };
+  issue(0, s0);
+  issue(1, s1);
+  int t = 0;
+  for (; t + 2 <= steps; t += 2) {
+    step(t, s0);
+    step(t + 1, s1);
   }
+  if (t < steps) step(t, s0);
+  wait_loads<0>();
 }
 
-// a 128 x 128 tile of a symmetric matrix in halves to (r0, c0), and mirrored to (c0, r0) off the diagonal
-__device__ __forceinline__ void store_symmetric(_Float16* d, int ld, int r0, int c0, const f4v (&v)[4][4], unsigned char* lds) {
+// a 128 x 128 tile of a symmetric matrix in halves to (r0, c0), and mirrored to (c0, r0) off the diagonal: the mirror goes
+// through LDS, rows 0 .. 63 of the tile in s0 and 64 .. 127 in s1
+__device__ __forceinline__ void store_symmetric(_Float16* d, int ld, int r0, int c0, const f4v (&v)[4][4], unsigned char* s0, unsigned char* s1) {
   const int wave = threadIdx.x >> 6, i = lane_id() & 15, g = lane_id() >> 4;
   const int la = (wave & 1) * 64, lb = (wave >> 1) * 64;
-  float* f = (float*)lds;
+  float *f0 = (float*)s0, *f1 = (float*)s1;
   __syncthreads();   // (the last step's fragments have been read)
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
-    const int row = la + 16 * x + i;
+    const int row = 16 * x + i;
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
       const int col = lb + 16 * y + 4 * g;
       const float u[4] = {v[x][y][0], v[x][y][1], v[x][y][2], v[x][y][3]};
       h4v hi, lo;
       split4(u, hi, lo);
-      _Float16* p = d + (int64_t)(r0 + row) * ld + half_at(c0 + col);
+      _Float16* p = d + (int64_t)(r0 + la + row) * ld + half_at(c0 + col);
       *reinterpret_cast<h4v*>(p) = hi;
       *reinterpret_cast<h4v*>(p + 32) = lo;
-      if (r0 != c0) lds_st_fenced(reinterpret_cast<f4v*>(f + row * 128 + (col ^ (((row >> 2) & 3) << 4))), v[x][y]);
+      if (r0 != c0) lds_st_fenced(reinterpret_cast<f4v*>((la ? f1 : f0) + row * 128 + (col ^ (((row >> 2) & 3) << 4))), v[x][y]);
     }
   }
   if (r0 == c0) return;
@@ -296,13 +310,13 @@ __device__ __forceinline__ void store_symmetric(_Float16* d, int ld, int r0, int
     const int row = la + 16 * x + i;   // a column of the tile
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
-      const int col = lb + 16 * y + 4 * g;
+      const int col = 16 * y + 4 * g;  // rows of the tile, of the half that lb names
       float u[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) u[r] = f[(col + r) * 128 + (row ^ ((((col + r) >> 2) & 3) << 4))];
+      for (int r = 0; r < 4; ++r) u[r] = (lb ? f1 : f0)[(col + r) * 128 + (row ^ ((((col + r) >> 2) & 3) << 4))];
       h4v hi, lo;
       split4(u, hi, lo);
-      _Float16* p = d + (int64_t)(c0 + row) * ld + half_at(r0 + col);
+      _Float16* p = d + (int64_t)(c0 + row) * ld + half_at(r0 + lb + col);
       *reinterpret_cast<h4v*>(p) = hi;
       *reinterpret_cast<h4v*>(p + 32) = lo;
     }
@@ -318,20 +332,12 @@ __device__ __forceinline__ void triangle(int unit, int& ti, int& tj) {
   tj = unit;
 }
 
-// A = X X^T (SQUARE false) or Q = a I + b A + c A A (SQUARE true), the tiles on and below the diagonal
-template <bool SQUARE, int N>
-__global__ void __launch_bounds__(256) ortho_gram(const Table<N> p) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * TILE_BYTES];
-  int matrix, unit, ti, tj;
-  const int it = locate(p, blockIdx.x, matrix, unit, [](const Item& t) { const int k = t.mp / TILE; return k * (k + 1) / 2; });
-  if (it < 0) return;
-  const Item& t = p.item[it];
-  triangle(unit, ti, tj);
-  const int k = SQUARE ? t.mp : t.np;
-  const _Float16* src = (SQUARE ? t.a : t.x) + (int64_t)matrix * t.mp * 2 * k;
-  const unsigned ld = 4u * k;
-  f4v acc[4][4];
-  pair_product<false, false>(src + (int64_t)ti * TILE * 2 * k, ld, src + (int64_t)tj * TILE * 2 * k, ld, k, lds, acc);
+__device__ __forceinline__ int lower_tiles(const Item& t) { const int k = t.mp / TILE; return k * (k + 1) / 2; }
+
+// The tile's sum scaled, or Q's other terms added, and stored
+template <bool SQUARE>
+__device__ __forceinline__ void finish_tile(const Args& p, const Item& t, int matrix, int ti, int tj, f4v (&acc)[4][4], unsigned char* s0,
+                                            unsigned char* s1) {
   const int wave = threadIdx.x >> 6, i = lane_id() & 15, g = lane_id() >> 4;
   const int r0 = ti * TILE, c0 = tj * TILE;
   if constexpr (!SQUARE) {
@@ -342,13 +348,14 @@ __global__ void __launch_bounds__(256) ortho_gram(const Table<N> p) {
       for (int y = 0; y < 4; ++y) acc[x][y] *= s;
   } else {
     const float s = p.c * p.up_q / (p.up_a * p.up_a), sb = p.b * p.up_q / p.up_a, sa = p.a * p.up_q;
+    const _Float16* src = t.a + (int64_t)matrix * t.mp * 2 * t.mp;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const int row = r0 + (wave & 1) * 64 + 16 * x + i;
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         const int col = c0 + (wave >> 1) * 64 + 16 * y + 4 * g;
-        const _Float16* q = src + (int64_t)row * 2 * k + half_at(col);
+        const _Float16* q = src + (int64_t)row * 2 * t.mp + half_at(col);
         const h4v hi = *reinterpret_cast<const h4v*>(q), lo = *reinterpret_cast<const h4v*>(q + 32);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -358,7 +365,60 @@ __global__ void __launch_bounds__(256) ortho_gram(const Table<N> p) {
       }
     }
   }
-  store_symmetric((SQUARE ? t.q : t.a) + (int64_t)matrix * t.mp * 2 * t.mp, 2 * t.mp, r0, c0, acc, lds);
+  store_symmetric((SQUARE ? t.q : t.a) + (int64_t)matrix * t.mp * 2 * t.mp, 2 * t.mp, r0, c0, acc, s0, s1);
+}
+
+// A = X X^T (SQUARE false) or Q = a I + b A + c A A (SQUARE true), the tiles on and below the diagonal, in `split` pieces of the
+// contracted index each
+template <bool SQUARE, int N>
+__global__ void __launch_bounds__(256, 2) ortho_gram(const Table<N> p) {
+  __shared__ __attribute__((aligned(16))) unsigned char s0[2 * TILE_BYTES], s1[2 * TILE_BYTES];
+  int matrix, unit, ti, tj;
+  const int it = locate(p, blockIdx.x, matrix, unit, [](const Item& t) { return lower_tiles(t) * (SQUARE ? t.split_q : t.split_a); });
+  if (it < 0) return;
+  const Item& t = p.item[it];
+  const int split = SQUARE ? t.split_q : t.split_a, tile = unit / split, piece = unit - tile * split;
+  triangle(tile, ti, tj);
+  const int k = SQUARE ? t.mp : t.np, steps = k / 32, k0 = steps * piece / split, k1 = steps * (piece + 1) / split;
+  const _Float16* src = (SQUARE ? t.a : t.x) + (int64_t)matrix * t.mp * 2 * k + (int64_t)k0 * 64;
+  const unsigned ld = 4u * k;
+  f4v acc[4][4];
+  pair_product<false, false>(src + (int64_t)ti * TILE * 2 * k, ld, src + (int64_t)tj * TILE * 2 * k, ld, k1 - k0, s0, s1, acc);
+  if (split == 1) {
+    finish_tile<SQUARE>(p, t, matrix, ti, tj, acc, s0, s1);
+    return;
+  }
+  f4v* part = (f4v*)(t.part + (((int64_t)matrix * lower_tiles(t) + tile) * split + piece) * (TILE * TILE)) + threadIdx.x;
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) part[(4 * x + y) * 256] = acc[x][y];
+}
+
+// the pieces of a tile summed in their order
+template <bool SQUARE, int N>
+__global__ void __launch_bounds__(256, 2) ortho_join(const Table<N> p) {
+  __shared__ __attribute__((aligned(16))) unsigned char s0[2 * TILE_BYTES], s1[2 * TILE_BYTES];
+  int matrix, tile, ti, tj;
+  const int it = locate(p, blockIdx.x, matrix, tile, [](const Item& t) { return (SQUARE ? t.split_q : t.split_a) > 1 ? lower_tiles(t) : 0; });
+  if (it < 0) return;
+  const Item& t = p.item[it];
+  const int split = SQUARE ? t.split_q : t.split_a;
+  triangle(tile, ti, tj);
+  const f4v* part = (const f4v*)(t.part + ((int64_t)matrix * lower_tiles(t) + tile) * split * (TILE * TILE)) + threadIdx.x;
+  f4v acc[4][4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) acc[x][y] = part[(4 * x + y) * 256];
+  for (int q = 1; q < split; ++q) {
+    part += TILE * TILE / 4;
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) acc[x][y] += part[(4 * x + y) * 256];
+  }
+  finish_tile<SQUARE>(p, t, matrix, ti, tj, acc, s0, s1);
 }
 
 // X' = Q X, or with `last` the weights' step (or the result)
@@ -380,8 +440,8 @@ __device__ __forceinline__ void put_update(const Args& p, const Item& t, int64_t
 }
 
 template <int N>
-__global__ void __launch_bounds__(256) ortho_apply(const Table<N> p) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * TILE_BYTES];
+__global__ void __launch_bounds__(256, 2) ortho_apply(const Table<N> p) {
+  __shared__ __attribute__((aligned(16))) unsigned char s0[2 * TILE_BYTES], s1[2 * TILE_BYTES];
   int matrix, unit;
   const int it = locate(p, blockIdx.x, matrix, unit, [](const Item& t) { return t.mp / TILE * (t.np / TILE); });
   if (it < 0) return;
@@ -396,7 +456,7 @@ __global__ void __launch_bounds__(256) ortho_apply(const Table<N> p) {
   const int64_t base = (int64_t)matrix * t.rows * t.cols;
   f4v acc[4][4];
   if (p.last && t.rows > t.cols) {   // (uniform) the turned matrix: a lane holds neighbours along X's rows
-    pair_product<true, true>(q, 4u * t.mp, x, 4u * t.np, t.mp, lds, acc);
+    pair_product<true, true>(q, 4u * t.mp, x, 4u * t.np, t.mp / 32, s0, s1, acc);
 #pragma unroll
     for (int xx = 0; xx < 4; ++xx)
 #pragma unroll
@@ -406,7 +466,7 @@ __global__ void __launch_bounds__(256) ortho_apply(const Table<N> p) {
       }
     return;
   }
-  pair_product<true, false>(q, 4u * t.mp, x, 4u * t.np, t.mp, lds, acc);
+  pair_product<true, false>(q, 4u * t.mp, x, 4u * t.np, t.mp / 32, s0, s1, acc);
   _Float16* d = t.y + (int64_t)matrix * t.mp * 2 * t.np;
 #pragma unroll
   for (int xx = 0; xx < 4; ++xx)
@@ -873,27 +933,70 @@ static void launch_small(const Table<ITEMS>& a, int size, unsigned blocks, int s
   else ortho_small<SMALL_SIZES[1], N><<<blocks, SMALL_THREADS, 0, s>>>(smaller<N>(a), steps);
 }
 struct Grids {
-  int64_t chunks, starts, grams, tiles;
+  int64_t chunks, starts, tiles;
 };
 template <int N>
 static void launch_tiles(const Table<ITEMS>& a, const Grids& g, int steps, hipStream_t s) {
   Table<N> t = smaller<N>(a);
+  int64_t grams = 0, squares = 0, join_a = 0, join_q = 0;
+  for (int i = 0; i < t.items; ++i) {
+    const Item& q = t.item[i];
+    const int64_t tiles = (int64_t)(q.mp / TILE) * (q.mp / TILE + 1) / 2 * q.count;
+    grams += tiles * q.split_a;
+    squares += tiles * q.split_q;
+    join_a += q.split_a > 1 ? tiles : 0;
+    join_q += q.split_q > 1 ? tiles : 0;
+  }
   ortho_norm<N><<<(unsigned)g.chunks, 256, 0, s>>>(t);
   ortho_start<N><<<(unsigned)g.starts, 256, 0, s>>>(t);
   for (int k = 0; k < steps; ++k) {
     t.last = k == steps - 1;
-    ortho_gram<false, N><<<(unsigned)g.grams, 256, 0, s>>>(t);
-    ortho_gram<true, N><<<(unsigned)g.grams, 256, 0, s>>>(t);
+    ortho_gram<false, N><<<(unsigned)grams, 256, 0, s>>>(t);
+    if (join_a) ortho_join<false, N><<<(unsigned)join_a, 256, 0, s>>>(t);
+    ortho_gram<true, N><<<(unsigned)squares, 256, 0, s>>>(t);
+    if (join_q) ortho_join<true, N><<<(unsigned)join_q, 256, 0, s>>>(t);
     ortho_apply<N><<<(unsigned)g.tiles, 256, 0, s>>>(t);
     for (int i = 0; i < t.items; ++i) std::swap(t.item[i].x, t.item[i].y);
   }
 }
 
+static int64_t padded_side(int v) { return ceil_to(v, TILE); }
+static int64_t lower_of(int64_t mp) { return (mp / TILE) * (mp / TILE + 1) / 2; }
+constexpr int MOST_SPLIT = 8;
+
 static int64_t item_bytes(const nfi_ortho_item& s) {
   const int m = std::min(s.rows, s.cols), n = std::max(s.rows, s.cols);
   if (kind_of(s) >= 0) return 0;
-  const int64_t mp = ceil_to(m, TILE), np = ceil_to(n, TILE), size = (int64_t)s.rows * s.cols;
+  const int64_t mp = padded_side(m), np = padded_side(n), size = (int64_t)s.rows * s.cols;
   return s.count * (2 * up(mp * np * 4) + 2 * up(mp * mp * 4)) + up(s.count * ((size + NORM_CHUNK - 1) / NORM_CHUNK) * 8);
+}
+
+// Tiles of A are few and long where matrices are wide: with fewer than the 256 compute units' one each, the contracted index is
+// divided so that two fit on every unit, in pieces of 12 steps at least (a shorter one costs more in the join).  The partial tiles
+// of A, and after them those of Q, lie from `part` on; returns their bytes.
+static int64_t choose_splits(Item* items, int count, unsigned char* part) {
+  int64_t tiles = 0, steps_a = 0, steps_q = 0;
+  for (int i = 0; i < count; ++i) {
+    const int64_t t = lower_of(items[i].mp) * items[i].count;
+    tiles += t;
+    steps_a += t * (items[i].np / 32);
+    steps_q += t * (items[i].mp / 32);
+  }
+  auto split = [&](int64_t all, int64_t own) {
+    if (tiles >= 256) return 1;
+    const int64_t piece = std::max<int64_t>(12, (all + 511) / 512);
+    return (int)std::min<int64_t>(MOST_SPLIT, std::max<int64_t>(1, own / piece));
+  };
+  int64_t used = 0;
+  for (int i = 0; i < count; ++i) {
+    Item& t = items[i];
+    t.split_a = split(steps_a, t.np / 32);
+    t.split_q = split(steps_q, t.mp / 32);
+    t.part = (float*)(part + used);
+    const int most = std::max(t.split_a, t.split_q);
+    if (most > 1) used += lower_of(t.mp) * t.count * TILE * TILE * 4 * most;
+  }
+  return used;
 }
 
 // largest |s q(s^2)| and |q| over s in [0, top], q(t) = a + b t + c t^2: at the ends or where a derivative is 0
@@ -954,12 +1057,22 @@ extern "C" {
 int64_t nfi_ortho_work_bytes(const nfi_ortho_item* items, int32_t n_items) {
   int64_t most = 0, sum = 0;
   int held = 0;
-  for (int i = 0; i < n_items; ++i) {
-    const int64_t b = item_bytes(items[i]);
-    if (b == 0) continue;
-    sum += b;
-    most = std::max(most, sum);
-    if (++held == ITEMS) held = 0, sum = 0;
+  Item table[ITEMS];
+  for (int i = 0; i <= n_items; ++i) {
+    const int64_t b = i < n_items ? item_bytes(items[i]) : 0;
+    if (b > 0) {
+      Item& t = table[held++];
+      t = {};
+      t.count = items[i].count;
+      t.mp = (int)padded_side(std::min(items[i].rows, items[i].cols));
+      t.np = (int)padded_side(std::max(items[i].rows, items[i].cols));
+      sum += b;
+    }
+    if (held == ITEMS || (i == n_items && held > 0)) {
+      most = std::max(most, sum + choose_splits(table, held, nullptr));
+      held = 0;
+      sum = 0;
+    }
   }
   return most;
 }
@@ -1032,14 +1145,15 @@ int32_t nfi_ortho(const nfi_ortho_args* p, void* stream) {
   Table<ITEMS> a;
   (Args&)a = base;
   unsigned char* work = (unsigned char*)p->work;
-  Grids grids = {0, 0, 0, 0};
+  Grids grids = {0, 0, 0};
   auto flush = [&]() {
+    choose_splits(a.item, a.items, work);   // (behind the last item)
     if (a.items == 1) launch_tiles<1>(a, grids, p->steps, s);
     else if (a.items > 0 && a.items <= 8) launch_tiles<8>(a, grids, p->steps, s);
     else if (a.items > 8) launch_tiles<ITEMS>(a, grids, p->steps, s);
     a.items = 0;
     work = (unsigned char*)p->work;
-    grids = {0, 0, 0, 0};
+    grids = {0, 0, 0};
   };
   for (int i = 0; i < p->n_items; ++i) {
     const nfi_ortho_item& q = p->items[i];
@@ -1057,7 +1171,6 @@ int32_t nfi_ortho(const nfi_ortho_args* p, void* stream) {
     const int64_t mt = t.mp / TILE;
     grids.chunks += (int64_t)t.chunks * t.count;
     grids.starts += (int64_t)(t.mp / 64) * (t.np / 64) * t.count;
-    grids.grams += mt * (mt + 1) / 2 * t.count;
     grids.tiles += mt * (t.np / TILE) * t.count;
     if (a.items == ITEMS) flush();
   }
