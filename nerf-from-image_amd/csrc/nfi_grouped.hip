@@ -21,8 +21,9 @@ struct GroupedArgs {
   int groups, n, k;                // the product's columns (of out) and contracted length
   unsigned lda, ldb;               // bytes between rows
   int64_t sb;                      // bytes between w's matrices
-  int offsets64, splits, col_tiles;
+  int offsets64, splits, col_tiles, row_tiles, by_xcd;
 };
+constexpr int BAND = 8;
 
 __device__ __forceinline__ int64_t offset_at(const void* p, int is64, int e, int64_t rows) {
   const int64_t v = is64 ? ((const int64_t*)p)[e] : (int64_t)((const int32_t*)p)[e];
@@ -83,8 +84,11 @@ __device__ __forceinline__ void store4(T* p, const float (&v)[4], int count) {
 template <class T, bool SLAB_B, int LB>
 __global__ void __launch_bounds__(256, 2) grouped_rows(const GroupedArgs p) {
   __shared__ __attribute__((aligned(16))) unsigned char s0[(TILE + LB) * STEP_BYTES], s1[(TILE + LB) * STEP_BYTES];
-  const int64_t tile = blockIdx.x / p.col_tiles;
-  const int c0 = (int)(blockIdx.x % p.col_tiles) * LB;
+  // bands of BAND row tiles, a band's rows first, so that what an XCD's compute units read at a time is a square of tiles
+  const unsigned unit = p.by_xcd ? xcd_order(blockIdx.x, gridDim.x) : blockIdx.x, band = unit / (BAND * p.col_tiles), in_band = unit - band * BAND * p.col_tiles;
+  const unsigned rows_of_band = min((unsigned)BAND, (unsigned)p.row_tiles - band * BAND);
+  const int64_t tile = band * BAND + in_band % rows_of_band;
+  const int c0 = (int)(in_band / rows_of_band) * LB;
   int64_t r0, r1;
   const int e = find_tile(p, tile, r0, r1);
   if (e < 0) return;
@@ -114,18 +118,18 @@ __global__ void __launch_bounds__(256, 2) grouped_rows(const GroupedArgs p) {
   }
 }
 
-// d w[e] [N][K] and d b[e]: a = dy as slabs (its columns are the lines), b = x as slabs, tiles of L x L; blockIdx.y the group, .z the
-// split.  Partial results: part [split][group][N][K], then part_b [split][group][N].
+// d w[e] [N][K] and d b[e]: a = dy as slabs (its columns are the lines), b = x as slabs, tiles of L x L.  Partial results: part [split][group][N][K], then part_b [split][group][N].
 template <class T, int L>
 __global__ void __launch_bounds__(256, 2) grouped_weights(const GroupedArgs p, int n_rows, void* gb, float* part_b) {
   __shared__ __attribute__((aligned(16))) unsigned char s0[2 * L * STEP_BYTES], s1[2 * L * STEP_BYTES];
-  const int e = blockIdx.y;
-  const int m0 = (int)(blockIdx.x / p.col_tiles) * L, c0 = (int)(blockIdx.x % p.col_tiles) * L;
+  const unsigned tile = blockIdx.x % p.row_tiles, place = blockIdx.x / p.row_tiles;   // place: split, group
+  const int e = (int)(place % p.groups), z = (int)(place / p.groups);
+  const int m0 = (int)(tile / p.col_tiles) * L, c0 = (int)(tile % p.col_tiles) * L;
   const int64_t s = offset_at(p.offsets, p.offsets64, e, p.rows), t = max(s, offset_at(p.offsets, p.offsets64, e + 1, p.rows));
   // pieces of whole steps
   constexpr int KSTEP = STEP_BYTES / sizeof(T);
   const int64_t piece = ((t - s + p.splits - 1) / p.splits + KSTEP - 1) / KSTEP * KSTEP;
-  const int64_t r0 = min(t, s + blockIdx.z * piece), r1 = min(t, r0 + piece);
+  const int64_t r0 = min(t, s + z * piece), r1 = min(t, r0 + piece);
   const int lines = min(L, n_rows - m0), cols = min(L, p.n - c0);
   Accumulate<T, L / 32, L / 32, true> acc;
   acc.clear();
@@ -133,14 +137,14 @@ __global__ void __launch_bounds__(256, 2) grouped_weights(const GroupedArgs p, i
   tile_product<T, true, true, L, L>(p.a + r0 * p.lda + m0 * (int64_t)sizeof(T), p.lda, lines, p.b + r0 * p.ldb + c0 * (int64_t)sizeof(T),
                                     p.ldb, cols, r1 - r0, s0, s1, acc, sums);
   const int wave = threadIdx.x >> 6, i = lane_id() & 15, g = lane_id() >> 4;
-  const int64_t matrix = (int64_t)n_rows * p.n, place = (int64_t)blockIdx.z * p.groups + e;
+  const int64_t matrix = (int64_t)n_rows * p.n;
 #pragma unroll
   for (int x = 0; x < L / 32; ++x) {
     const int row = (wave & 1) * (L / 2) + x * 16 + i;
     if (row >= lines) continue;
     if (sums && wave < 2 && g == 0) {
       if (p.splits == 1) ((T*)gb)[(int64_t)e * n_rows + m0 + row] = (T)acc.sum[x][0];
-      else part_b[place * n_rows + m0 + row] = acc.sum[x][0];
+      else part_b[(int64_t)place * n_rows + m0 + row] = acc.sum[x][0];
     }
     if (p.out == nullptr) continue;
 #pragma unroll
@@ -260,7 +264,12 @@ template <class T>
 static void launch_rows(GroupedArgs& p, bool slab, hipStream_t s) {
   const int lb = p.n <= 64 ? 64 : TILE;   // (half of a 128 tile would be empty)
   p.col_tiles = (p.n + lb - 1) / lb;
-  const unsigned tiles = (unsigned)(((p.rows + TILE - 1) / TILE + std::min<int64_t>(p.groups + 2, p.rows)) * p.col_tiles);
+  p.row_tiles = (int)((p.rows + TILE - 1) / TILE + std::min<int64_t>(p.groups + 2, p.rows));
+  // neighbouring tiles to an XCD where they share both operands (16 experts' 32,749 rows of 1024 -> 4096: 388 -> 374 us, back
+  // 364 -> 320); weights that a few rows read once, and single columns of tiles, go to all of them in turn (48 rows of 512 ->
+  // 2048: 19 -> 15 us)
+  p.by_xcd = p.col_tiles > 1 && p.rows / p.groups >= 2 * TILE;
+  const unsigned tiles = (unsigned)((int64_t)p.row_tiles * p.col_tiles);
   if (slab) {
     if (lb == 64) grouped_rows<T, true, 64><<<tiles, 256, 0, s>>>(p);
     else grouped_rows<T, true, TILE><<<tiles, 256, 0, s>>>(p);
@@ -332,7 +341,8 @@ static void backward(const nfi_grouped_args& a, hipStream_t s) {
     p.part = (float*)work;
     const int64_t count = (int64_t)a.groups * a.out_width * a.in_width, count_b = a.gb ? (int64_t)a.groups * a.out_width : 0;
     float* part_b = p.part + count * p.splits;
-    const dim3 grid((unsigned)tiles_of(a.out_width, a.in_width, tile), (unsigned)a.groups, (unsigned)p.splits);
+    p.row_tiles = (int)tiles_of(a.out_width, a.in_width, tile);   // (of one matrix)
+    const unsigned grid = (unsigned)((int64_t)p.row_tiles * a.groups * p.splits);
     if (tile == TILE) grouped_weights<T, TILE><<<grid, 256, 0, s>>>(p, a.out_width, a.gb, part_b);
     else grouped_weights<T, 64><<<grid, 256, 0, s>>>(p, a.out_width, a.gb, part_b);
     if (p.splits > 1)
@@ -359,6 +369,7 @@ static int check(const nfi_grouped_args* a, const char* what) {
               "%s: widths %d -> %d (1 .. %d)", what, a->in_width, a->out_width, NFI_GROUPED_MAX_WIDTH);
   const int64_t widest = std::max(a->in_width, a->out_width);
   NFI_REQUIRE(((a->rows + TILE - 1) / TILE + a->groups + 2) * ((widest + 63) / 64) < (1ll << 31), "%s: too many tiles", what);
+  NFI_REQUIRE(a->groups * tiles_of(a->out_width, a->in_width, weight_tile(a->out_width, a->in_width)) < (1ll << 31), "%s: too many tiles", what);
   return NFI_OK;
 }
 

@@ -170,6 +170,13 @@ __device__ __forceinline__ f4v product(const Thirds& b, const Thirds& a, f4v acc
   return product<bf16_t>(b.h, a.h, acc);
 }
 
+// Workgroups go to the 8 XCDs (each with an L2 of its own) in turn: the unit of work of workgroup b of n, such that
+// each XCD gets neighbouring units, which share operands
+__device__ __forceinline__ unsigned xcd_order(unsigned b, unsigned n) {
+  const unsigned x = b & 7, q = n >> 3, r = n & 7;
+  return x * q + min(x, r) + (b >> 3);
+}
+
 // vmcnt(n), nothing else (n < 64)
 template <int N>
 __device__ __forceinline__ void wait_loads() {

@@ -46,6 +46,7 @@ struct Args {
 // The launch's arguments: a kernel takes room for 1, 8 or 32 items (3.4 KB of arguments cost 10 us of a launch)
 template <int N>
 struct Table : Args {
+  int first[N];   // the launch's first unit of each item (behind the last: beyond any)
   Item item[N];
 };
 
@@ -55,19 +56,18 @@ __device__ __forceinline__ float typed_at(const void* p, int type, int64_t i) {
   return type == NFI_F32 ? ((const float*)p)[i] : type == NFI_BF16 ? (float)((const bf16_t*)p)[i] : (float)((const f16_t*)p)[i];
 }
 
-// Work unit `id` of a launch: the item, the matrix of its run, and the unit within it (per(item) units each)
+// Work unit `id` of a launch: the item, the matrix of its run, and the unit within it (per(item) units each).  (The first units
+// lie together and come with one or two loads; a walk over the items would wait for each.)
 template <int N, class F>
 __device__ __forceinline__ int locate(const Table<N>& p, int id, int& matrix, int& unit, F per) {
-  for (int i = 0; i < p.items; ++i) {
-    const int u = per(p.item[i]), all = u * p.item[i].count;
-    if (id < all) {   // (not for an item without units)
-      matrix = id / u;
-      unit = id - matrix * u;
-      return i;
-    }
-    id -= all;
-  }
-  return -1;
+  int it = 0;
+#pragma unroll
+  for (int k = 1; k < N; ++k) it += id >= p.first[k];
+  id -= p.first[it];
+  const int u = per(p.item[it]);
+  matrix = id / u;
+  unit = id - matrix * u;
+  return it;
 }
 
 // ---- momentum and norm -------------------------------------------------------------------------------------------
@@ -78,7 +78,6 @@ __global__ void __launch_bounds__(256) ortho_norm(const Table<N> p) {
   __shared__ double red[256];
   int matrix, chunk;
   const int i = locate(p, blockIdx.x, matrix, chunk, [](const Item& t) { return t.chunks; });
-  if (i < 0) return;
   const Item& t = p.item[i];
   const int64_t size = (int64_t)t.rows * t.cols, base = matrix * size;
   const int64_t e0 = (int64_t)chunk * NORM_CHUNK, e1 = min(e0 + NORM_CHUNK, size);
@@ -156,7 +155,6 @@ __global__ void __launch_bounds__(256) ortho_start(const Table<N> p) {
   __shared__ double red[256];
   int matrix, unit;
   const int i = locate(p, blockIdx.x, matrix, unit, [](const Item& t) { return t.mp / 64 * (t.np / 64); });
-  if (i < 0) return;
   const Item& t = p.item[i];
   const double inv = inverse_norm(t.sums + (int64_t)matrix * t.chunks, t.chunks, p.eps, red) * p.up_x;
   const int r0 = unit / (t.np / 64) * 64, c0 = unit % (t.np / 64) * 64;
@@ -197,11 +195,11 @@ struct PairSlab {
       off[j] = row * ld + (((lane_id() & 31) ^ (2 * (row & 7))) << 4);
     }
   }
-  __device__ __forceinline__ void issue(const void* base, unsigned char* lds) const {
+  __device__ __forceinline__ void issue(const void* base, unsigned char* lds, bool in) const {
     const __amdgpu_buffer_rsrc_t r = descriptor(base);
     unsigned char* dst = lds + (threadIdx.x >> 6) * 4096;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) load_to_lds(r, dst + j * 1024, off[j]);
+    for (int j = 0; j < 4; ++j) load_to_lds(r, dst + j * 1024, in ? off[j] : NOWHERE);
   }
 };
 
@@ -237,10 +235,10 @@ __device__ __forceinline__ void pair_product(const _Float16* a, unsigned lda, co
   const int wave = threadIdx.x >> 6, line_a = (wave & 1) * 64, line_b = (wave >> 1) * 64;
   const unsigned char *pa = (const unsigned char*)a, *pb = (const unsigned char*)b;
   auto issue = [&](int t, unsigned char* dst) {
-    t = min(t, steps - 1);   // (behind the last step that one again: every step waits for the same number of loads)
-    la.issue(pa + (int64_t)t * STEP_BYTES, dst, STEP_BYTES);
-    if (SLAB) sb.issue(pb + t * step_b, dst + TILE_BYTES);
-    else lb.issue(pb + t * step_b, dst + TILE_BYTES, STEP_BYTES);
+    const bool in = t < steps;   // (a step behind the last reads nothing: every step waits for the same number of loads)
+    la.issue(pa + (int64_t)t * STEP_BYTES, dst, in ? STEP_BYTES : 0);
+    if (SLAB) sb.issue(pb + t * step_b, dst + TILE_BYTES, in);
+    else lb.issue(pb + t * step_b, dst + TILE_BYTES, in ? STEP_BYTES : 0);
     __builtin_amdgcn_sched_barrier(0);   // the waits count on this order of the steps' loads
   };
 #pragma unroll
@@ -374,8 +372,7 @@ template <bool SQUARE, int N>
 __global__ void __launch_bounds__(256, 2) ortho_gram(const Table<N> p) {
   __shared__ __attribute__((aligned(16))) unsigned char s0[2 * TILE_BYTES], s1[2 * TILE_BYTES];
   int matrix, unit, ti, tj;
-  const int it = locate(p, blockIdx.x, matrix, unit, [](const Item& t) { return lower_tiles(t) * (SQUARE ? t.split_q : t.split_a); });
-  if (it < 0) return;
+  const int it = locate(p, xcd_order(blockIdx.x, gridDim.x), matrix, unit, [](const Item& t) { return lower_tiles(t) * (SQUARE ? t.split_q : t.split_a); });
   const Item& t = p.item[it];
   const int split = SQUARE ? t.split_q : t.split_a, tile = unit / split, piece = unit - tile * split;
   triangle(tile, ti, tj);
@@ -401,7 +398,6 @@ __global__ void __launch_bounds__(256, 2) ortho_join(const Table<N> p) {
   __shared__ __attribute__((aligned(16))) unsigned char s0[2 * TILE_BYTES], s1[2 * TILE_BYTES];
   int matrix, tile, ti, tj;
   const int it = locate(p, blockIdx.x, matrix, tile, [](const Item& t) { return (SQUARE ? t.split_q : t.split_a) > 1 ? lower_tiles(t) : 0; });
-  if (it < 0) return;
   const Item& t = p.item[it];
   const int split = SQUARE ? t.split_q : t.split_a;
   triangle(tile, ti, tj);
@@ -443,8 +439,7 @@ template <int N>
 __global__ void __launch_bounds__(256, 2) ortho_apply(const Table<N> p) {
   __shared__ __attribute__((aligned(16))) unsigned char s0[2 * TILE_BYTES], s1[2 * TILE_BYTES];
   int matrix, unit;
-  const int it = locate(p, blockIdx.x, matrix, unit, [](const Item& t) { return t.mp / TILE * (t.np / TILE); });
-  if (it < 0) return;
+  const int it = locate(p, xcd_order(blockIdx.x, gridDim.x), matrix, unit, [](const Item& t) { return t.mp / TILE * (t.np / TILE); });
   const Item& t = p.item[it];
   const int tr = unit % (t.mp / TILE), tc = unit / (t.mp / TILE);   // the tiles of a block of X's columns follow each other
   const int r0 = tr * TILE, c0 = tc * TILE;
@@ -893,7 +888,6 @@ __global__ void __launch_bounds__(SMALL_THREADS) ortho_small(const Table<N> p, i
   __shared__ double red[SMALL_WAVES];
   int matrix, unit;
   const int it = locate(p, blockIdx.x, matrix, unit, [](const Item&) { return 1; });
-  if (it < 0) return;
   const Item& t = p.item[it];
   if (t.m > 48) run_lds<4>(p, t, matrix, steps, lds, red);
   else if (t.m > 32) run_lds<3>(p, t, matrix, steps, lds, red);
@@ -919,7 +913,7 @@ static int kind_of(const nfi_ortho_item& q) {
   return need <= SMALL_SIZES[0] ? 0 : need <= SMALL_SIZES[1] ? 1 : -1;
 }
 
-// the launches of a table's items, in the smallest table that holds them
+// a table in the smallest size that holds its items
 template <int N>
 static Table<N> smaller(const Table<ITEMS>& t) {
   Table<N> r;
@@ -927,35 +921,40 @@ static Table<N> smaller(const Table<ITEMS>& t) {
   std::copy(t.item, t.item + std::min(t.items, N), r.item);
   return r;
 }
-template <int N>
-static void launch_small(const Table<ITEMS>& a, int size, unsigned blocks, int steps, hipStream_t s) {
-  if (size == 0) ortho_small<SMALL_SIZES[0], N><<<blocks, SMALL_THREADS, 0, s>>>(smaller<N>(a), steps);
-  else ortho_small<SMALL_SIZES[1], N><<<blocks, SMALL_THREADS, 0, s>>>(smaller<N>(a), steps);
-}
-struct Grids {
-  int64_t chunks, starts, tiles;
-};
-template <int N>
-static void launch_tiles(const Table<ITEMS>& a, const Grids& g, int steps, hipStream_t s) {
-  Table<N> t = smaller<N>(a);
-  int64_t grams = 0, squares = 0, join_a = 0, join_q = 0;
-  for (int i = 0; i < t.items; ++i) {
-    const Item& q = t.item[i];
-    const int64_t tiles = (int64_t)(q.mp / TILE) * (q.mp / TILE + 1) / 2 * q.count;
-    grams += tiles * q.split_a;
-    squares += tiles * q.split_q;
-    join_a += q.split_a > 1 ? tiles : 0;
-    join_q += q.split_q > 1 ? tiles : 0;
+// the items' first units, per(item) for each matrix; returns all
+template <int N, class F>
+static unsigned number_units(Table<N>& t, F per) {
+  int64_t all = 0;
+  for (int i = 0; i < N; ++i) {
+    t.first[i] = i < t.items ? (int)all : 0x7fffffff;
+    if (i < t.items) all += (int64_t)per(t.item[i]) * t.item[i].count;
   }
-  ortho_norm<N><<<(unsigned)g.chunks, 256, 0, s>>>(t);
-  ortho_start<N><<<(unsigned)g.starts, 256, 0, s>>>(t);
+  return (unsigned)all;
+}
+template <int N>
+static void launch_small(const Table<ITEMS>& a, int size, int steps, hipStream_t s) {
+  Table<N> t = smaller<N>(a);
+  const unsigned blocks = number_units(t, [](const Item&) { return 1; });
+  if (size == 0) ortho_small<SMALL_SIZES[0], N><<<blocks, SMALL_THREADS, 0, s>>>(t, steps);
+  else ortho_small<SMALL_SIZES[1], N><<<blocks, SMALL_THREADS, 0, s>>>(t, steps);
+}
+template <int N>
+static void launch_tiles(const Table<ITEMS>& a, int steps, hipStream_t s) {
+  Table<N> t = smaller<N>(a);
+  auto lower = [](const Item& q) { return (q.mp / TILE) * (q.mp / TILE + 1) / 2; };
+  auto launch = [&](auto kernel, auto per) {
+    const unsigned blocks = number_units(t, per);
+    if (blocks) kernel<<<blocks, 256, 0, s>>>(t);
+  };
+  launch(ortho_norm<N>, [](const Item& q) { return q.chunks; });
+  launch(ortho_start<N>, [](const Item& q) { return q.mp / 64 * (q.np / 64); });
   for (int k = 0; k < steps; ++k) {
     t.last = k == steps - 1;
-    ortho_gram<false, N><<<(unsigned)grams, 256, 0, s>>>(t);
-    if (join_a) ortho_join<false, N><<<(unsigned)join_a, 256, 0, s>>>(t);
-    ortho_gram<true, N><<<(unsigned)squares, 256, 0, s>>>(t);
-    if (join_q) ortho_join<true, N><<<(unsigned)join_q, 256, 0, s>>>(t);
-    ortho_apply<N><<<(unsigned)g.tiles, 256, 0, s>>>(t);
+    launch(ortho_gram<false, N>, [&](const Item& q) { return lower(q) * q.split_a; });
+    launch(ortho_join<false, N>, [&](const Item& q) { return q.split_a > 1 ? lower(q) : 0; });
+    launch(ortho_gram<true, N>, [&](const Item& q) { return lower(q) * q.split_q; });
+    launch(ortho_join<true, N>, [&](const Item& q) { return q.split_q > 1 ? lower(q) : 0; });
+    launch(ortho_apply<N>, [](const Item& q) { return q.mp / TILE * (q.np / TILE); });
     for (int i = 0; i < t.items; ++i) std::swap(t.item[i].x, t.item[i].y);
   }
 }
@@ -1124,20 +1123,17 @@ int32_t nfi_ortho(const nfi_ortho_args* p, void* stream) {
   for (int size = 0; size < 2; ++size) {
     Table<ITEMS> a;
     (Args&)a = base;
-    int64_t blocks = 0;
     auto flush = [&]() {
-      if (a.items == 1) launch_small<1>(a, size, (unsigned)blocks, p->steps, s);
-      else if (a.items > 0 && a.items <= 8) launch_small<8>(a, size, (unsigned)blocks, p->steps, s);
-      else if (a.items > 8) launch_small<ITEMS>(a, size, (unsigned)blocks, p->steps, s);
+      if (a.items == 1) launch_small<1>(a, size, p->steps, s);
+      else if (a.items > 0 && a.items <= 8) launch_small<8>(a, size, p->steps, s);
+      else if (a.items > 8) launch_small<ITEMS>(a, size, p->steps, s);
       a.items = 0;
-      blocks = 0;
     };
     for (int i = 0; i < p->n_items; ++i) {
       const nfi_ortho_item& q = p->items[i];
       const int kind = kind_of(q);
       if (kind < 0 || (together ? 1 : kind) != size) continue;
       a.item[a.items++] = item(q, 16);
-      blocks += q.count;
       if (a.items == ITEMS) flush();
     }
     flush();
@@ -1145,15 +1141,13 @@ int32_t nfi_ortho(const nfi_ortho_args* p, void* stream) {
   Table<ITEMS> a;
   (Args&)a = base;
   unsigned char* work = (unsigned char*)p->work;
-  Grids grids = {0, 0, 0};
   auto flush = [&]() {
     choose_splits(a.item, a.items, work);   // (behind the last item)
-    if (a.items == 1) launch_tiles<1>(a, grids, p->steps, s);
-    else if (a.items > 0 && a.items <= 8) launch_tiles<8>(a, grids, p->steps, s);
-    else if (a.items > 8) launch_tiles<ITEMS>(a, grids, p->steps, s);
+    if (a.items == 1) launch_tiles<1>(a, p->steps, s);
+    else if (a.items > 0 && a.items <= 8) launch_tiles<8>(a, p->steps, s);
+    else if (a.items > 8) launch_tiles<ITEMS>(a, p->steps, s);
     a.items = 0;
     work = (unsigned char*)p->work;
-    grids = {0, 0, 0};
   };
   for (int i = 0; i < p->n_items; ++i) {
     const nfi_ortho_item& q = p->items[i];
@@ -1168,10 +1162,6 @@ int32_t nfi_ortho(const nfi_ortho_args* p, void* stream) {
     t.chunks = (int)(((int64_t)q.rows * q.cols + NORM_CHUNK - 1) / NORM_CHUNK);
     work += item_bytes(q);
     a.item[a.items++] = t;
-    const int64_t mt = t.mp / TILE;
-    grids.chunks += (int64_t)t.chunks * t.count;
-    grids.starts += (int64_t)(t.mp / 64) * (t.np / 64) * t.count;
-    grids.tiles += mt * (t.np / TILE) * t.count;
     if (a.items == ITEMS) flush();
   }
   flush();
