@@ -35,20 +35,12 @@ __device__ __forceinline__ int64_t offset_at(const void* p, int is64, int e, int
 __device__ __forceinline__ int find_tile(const GroupedArgs& p, int64_t tile, int64_t& r0, int64_t& r1) {
   const int l = lane_id();
   int64_t before = 0;
-  const int64_t head = offset_at(p.offsets, p.offsets64, 0, p.rows), tail = offset_at(p.offsets, p.offsets64, p.groups, p.rows);
   for (int e0 = 0; e0 < p.groups + 2; e0 += 64) {
     // two runs of no group follow the last: the rows before the first group and behind the last
     const int e = e0 + l;
-    int64_t s = 0, t = 0;
-    if (e < p.groups) {
-      s = offset_at(p.offsets, p.offsets64, e, p.rows);
-      t = offset_at(p.offsets, p.offsets64, e + 1, p.rows);
-    } else if (e == p.groups) {
-      t = head;
-    } else if (e == p.groups + 1) {
-      s = tail;
-      t = p.rows;
-    }
+    int64_t s = e == p.groups ? 0 : offset_at(p.offsets, p.offsets64, min(e, p.groups), p.rows);
+    int64_t t = offset_at(p.offsets, p.offsets64, e < p.groups ? e + 1 : 0, p.rows);
+    if (e > p.groups) t = e == p.groups + 1 ? p.rows : 0;
     const int mine = t > s ? (int)((t - s + TILE - 1) / TILE) : 0;
     int incl = mine;
 #pragma unroll
@@ -83,6 +75,7 @@ __device__ __forceinline__ void store4(T* p, const float (&v)[4], int count) {
 // y (SLAB_B false: b = w[e], rows of K) and d x (SLAB_B true: a = dy, b = w[e] as slabs): rows of `a` by tiles of 128 x LB
 template <class T, bool SLAB_B, int LB>
 __global__ void __launch_bounds__(256, 2) grouped_rows(const GroupedArgs p) {
+  typedef Share<TILE, LB> S;
   __shared__ __attribute__((aligned(16))) unsigned char s0[(TILE + LB) * STEP_BYTES], s1[(TILE + LB) * STEP_BYTES];
   // bands of BAND row tiles, a band's rows first, so that what an XCD's compute units read at a time is a square of tiles
   const unsigned unit = p.by_xcd ? xcd_order(blockIdx.x, gridDim.x) : blockIdx.x, band = unit / (BAND * p.col_tiles), in_band = unit - band * BAND * p.col_tiles;
@@ -93,23 +86,23 @@ __global__ void __launch_bounds__(256, 2) grouped_rows(const GroupedArgs p) {
   const int e = find_tile(p, tile, r0, r1);
   if (e < 0) return;
   const int rows = (int)(r1 - r0), cols = min(LB, p.n - c0);
-  Accumulate<T, 4, LB / 32, false> out;
+  Accumulate<T, S::NA, S::NB, false> out;
   out.clear();
   if (e < p.groups) {
     const unsigned char* b = p.b + e * p.sb + (SLAB_B ? (int64_t)c0 * (int)sizeof(T) : (int64_t)c0 * p.ldb);
     tile_product<T, false, SLAB_B, TILE, LB>(p.a + r0 * p.lda, p.lda, rows, b, p.ldb, cols, p.k, s0, s1, out, false);
   }
-  const int wave = threadIdx.x >> 6, i = lane_id() & 15, g = lane_id() >> 4;
+  const int i = lane_id() & 15, g = lane_id() >> 4;
 #pragma unroll
-  for (int y = 0; y < LB / 32; ++y) {
-    const int n = (wave >> 1) * (LB / 2) + y * 16 + 4 * g;
+  for (int y = 0; y < S::NB; ++y) {
+    const int n = S::line_b() + y * 16 + 4 * g;
     float bias[4] = {0.f, 0.f, 0.f, 0.f};
     if (p.bias && e < p.groups)   // (one after the other in flight: clamped, not skipped)
 #pragma unroll
       for (int r = 0; r < 4; ++r) bias[r] = (float)((const T*)p.bias)[(int64_t)e * p.n + c0 + min(n + r, cols - 1)];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int row = (wave & 1) * 64 + x * 16 + i;
+    for (int x = 0; x < S::NA; ++x) {
+      const int row = S::line_a() + x * 16 + i;
       float v[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[r] = out.acc[x][y][r] + bias[r];
@@ -121,6 +114,7 @@ __global__ void __launch_bounds__(256, 2) grouped_rows(const GroupedArgs p) {
 // d w[e] [N][K] and d b[e]: a = dy as slabs (its columns are the lines), b = x as slabs, tiles of L x L.  Partial results: part [split][group][N][K], then part_b [split][group][N].
 template <class T, int L>
 __global__ void __launch_bounds__(256, 2) grouped_weights(const GroupedArgs p, int n_rows, void* gb, float* part_b) {
+  typedef Share<L, L> S;
   __shared__ __attribute__((aligned(16))) unsigned char s0[2 * L * STEP_BYTES], s1[2 * L * STEP_BYTES];
   const unsigned tile = blockIdx.x % p.row_tiles, place = blockIdx.x / p.row_tiles;   // place: split, group
   const int e = (int)(place % p.groups), z = (int)(place / p.groups);
@@ -131,25 +125,25 @@ __global__ void __launch_bounds__(256, 2) grouped_weights(const GroupedArgs p, i
   const int64_t piece = ((t - s + p.splits - 1) / p.splits + KSTEP - 1) / KSTEP * KSTEP;
   const int64_t r0 = min(t, s + z * piece), r1 = min(t, r0 + piece);
   const int lines = min(L, n_rows - m0), cols = min(L, p.n - c0);
-  Accumulate<T, L / 32, L / 32, true> acc;
+  Accumulate<T, S::NA, S::NB, true> acc;
   acc.clear();
   const bool sums = gb != nullptr && c0 == 0;
   tile_product<T, true, true, L, L>(p.a + r0 * p.lda + m0 * (int64_t)sizeof(T), p.lda, lines, p.b + r0 * p.ldb + c0 * (int64_t)sizeof(T),
                                     p.ldb, cols, r1 - r0, s0, s1, acc, sums);
-  const int wave = threadIdx.x >> 6, i = lane_id() & 15, g = lane_id() >> 4;
+  const int i = lane_id() & 15, g = lane_id() >> 4;
   const int64_t matrix = (int64_t)n_rows * p.n;
 #pragma unroll
-  for (int x = 0; x < L / 32; ++x) {
-    const int row = (wave & 1) * (L / 2) + x * 16 + i;
+  for (int x = 0; x < S::NA; ++x) {
+    const int row = S::line_a() + x * 16 + i;
     if (row >= lines) continue;
-    if (sums && wave < 2 && g == 0) {
+    if (sums && S::line_b() == 0 && g == 0) {
       if (p.splits == 1) ((T*)gb)[(int64_t)e * n_rows + m0 + row] = (T)acc.sum[x][0];
       else part_b[(int64_t)place * n_rows + m0 + row] = acc.sum[x][0];
     }
     if (p.out == nullptr) continue;
 #pragma unroll
-    for (int y = 0; y < L / 32; ++y) {
-      const int n = (wave >> 1) * (L / 2) + y * 16 + 4 * g;
+    for (int y = 0; y < S::NB; ++y) {
+      const int n = S::line_b() + y * 16 + 4 * g;
       const float v[4] = {acc.acc[x][y][0], acc.acc[x][y][1], acc.acc[x][y][2], acc.acc[x][y][3]};
       const int64_t at = (int64_t)(m0 + row) * p.n + c0 + n;
       if (p.splits == 1) store4<T>((T*)p.out + e * matrix + at, v, cols - n);
@@ -252,7 +246,7 @@ static int64_t tiles_of(int n, int k, int tile) { return (int64_t)((n + tile - 1
 static int weight_splits(int64_t rows, int groups, int n, int k) {
   const int tile = weight_tile(n, k);
   const int64_t tiles = groups * tiles_of(n, k, tile);
-  const int64_t want = (tile == TILE ? 512 : 768) / tiles, most = rows / groups / 128;
+  const int64_t want = (tile == 64 ? 768 : 512) / tiles, most = rows / groups / 128;
   return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 256));
 }
 static int bias_splits(int64_t rows, int groups, int n) {
@@ -260,9 +254,9 @@ static int bias_splits(int64_t rows, int groups, int n) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(1024 / tiles, rows / groups / 32), 64));
 }
 
-template <class T>
-static void launch_rows(GroupedArgs& p, bool slab, hipStream_t s) {
-  const int lb = p.n <= 64 ? 64 : TILE;   // (half of a 128 tile would be empty)
+template <class T, bool SLAB>
+static void launch_rows(GroupedArgs& p, hipStream_t s) {
+  const int lb = p.n <= 64 ? 64 : TILE;   // (64: half of a 128 tile would be empty)
   p.col_tiles = (p.n + lb - 1) / lb;
   p.row_tiles = (int)((p.rows + TILE - 1) / TILE + std::min<int64_t>(p.groups + 2, p.rows));
   // neighbouring tiles to an XCD where they share both operands (16 experts' 32,749 rows of 1024 -> 4096: 388 -> 374 us, back
@@ -270,13 +264,8 @@ static void launch_rows(GroupedArgs& p, bool slab, hipStream_t s) {
   // 2048: 19 -> 15 us)
   p.by_xcd = p.col_tiles > 1 && p.rows / p.groups >= 2 * TILE;
   const unsigned tiles = (unsigned)((int64_t)p.row_tiles * p.col_tiles);
-  if (slab) {
-    if (lb == 64) grouped_rows<T, true, 64><<<tiles, 256, 0, s>>>(p);
-    else grouped_rows<T, true, TILE><<<tiles, 256, 0, s>>>(p);
-  } else {
-    if (lb == 64) grouped_rows<T, false, 64><<<tiles, 256, 0, s>>>(p);
-    else grouped_rows<T, false, TILE><<<tiles, 256, 0, s>>>(p);
-  }
+  if (lb == 64) grouped_rows<T, SLAB, 64><<<tiles, 256, 0, s>>>(p);
+  else grouped_rows<T, SLAB, TILE><<<tiles, 256, 0, s>>>(p);
 }
 
 template <class T>
@@ -306,7 +295,7 @@ static void forward(const nfi_grouped_args& a, hipStream_t s) {
   p.groups = a.groups;
   p.n = a.out_width;
   p.k = a.in_width;
-  launch_rows<T>(p, false, s);
+  launch_rows<T, false>(p, s);
 }
 
 template <class T>
@@ -327,7 +316,7 @@ static void backward(const nfi_grouped_args& a, hipStream_t s) {
     p.out = a.gx;
     p.n = a.in_width;
     p.k = a.out_width;
-    launch_rows<T>(p, true, s);
+    launch_rows<T, true>(p, s);
   }
   if (a.gw) {
     p.a = g;
@@ -343,8 +332,8 @@ static void backward(const nfi_grouped_args& a, hipStream_t s) {
     float* part_b = p.part + count * p.splits;
     p.row_tiles = (int)tiles_of(a.out_width, a.in_width, tile);   // (of one matrix)
     const unsigned grid = (unsigned)((int64_t)p.row_tiles * a.groups * p.splits);
-    if (tile == TILE) grouped_weights<T, TILE><<<grid, 256, 0, s>>>(p, a.out_width, a.gb, part_b);
-    else grouped_weights<T, 64><<<grid, 256, 0, s>>>(p, a.out_width, a.gb, part_b);
+    if (tile == 64) grouped_weights<T, 64><<<grid, 256, 0, s>>>(p, a.out_width, a.gb, part_b);
+    else grouped_weights<T, TILE><<<grid, 256, 0, s>>>(p, a.out_width, a.gb, part_b);
     if (p.splits > 1)
       join_parts<T><<<(unsigned)((count + 63) / 64 + (count_b + 63) / 64), 256, 0, s>>>(p.part, (T*)a.gw, count, part_b, (T*)a.gb, count_b, p.splits);
   } else if (a.gb) {
@@ -369,7 +358,7 @@ static int check(const nfi_grouped_args* a, const char* what) {
               "%s: widths %d -> %d (1 .. %d)", what, a->in_width, a->out_width, NFI_GROUPED_MAX_WIDTH);
   const int64_t widest = std::max(a->in_width, a->out_width);
   NFI_REQUIRE(((a->rows + TILE - 1) / TILE + a->groups + 2) * ((widest + 63) / 64) < (1ll << 31), "%s: too many tiles", what);
-  NFI_REQUIRE(a->groups * tiles_of(a->out_width, a->in_width, weight_tile(a->out_width, a->in_width)) < (1ll << 31), "%s: too many tiles", what);
+  NFI_REQUIRE(a->groups * tiles_of(a->out_width, a->in_width, 64) < (1ll << 31), "%s: too many tiles", what);
   return NFI_OK;
 }
 

@@ -1,7 +1,7 @@
 // Tiles of a matrix product on the matrix cores, fed by loads that go straight to LDS (gfx950).
 //
-// An operand tile is 64 or 128 "lines" of 128 bytes of the contracted index (64 16-bit or 32 32-bit values), 8 or 16 KB, in
-// one of two layouts:
+// An operand tile is 64 or 128 "lines" of 128 bytes of the contracted index (64 16-bit or 32 32-bit values), in one of
+// two layouts:
 //   lines   the operand's rows hold the contracted index contiguously: LDS [lines][8 pieces of 16 B], piece p of line
 //           r stored at p ^ (r & 7), so that the 16-byte reads of 8 lines use all banks
 //   slabs   the contracted index runs over rows and the lines are columns (a transposed operand): LDS
@@ -46,7 +46,7 @@ __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, unsigned c
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, (int)offset, 0, 0, 0);
 }
 
-// The loads of one operand tile of LINES lines by a workgroup of 4 waves: LINES / 32 of 1 KB for each wave, at fixed offsets
+// The loads of one operand tile of LINES lines by a workgroup: LINES / 32 a wave, of 1 KB each, at fixed offsets
 // from an address that moves by a step (lines: 128 bytes, slabs: a step's rows)
 template <class T, bool SLAB, int LINES>
 struct TileLoad {
@@ -190,7 +190,15 @@ __device__ __forceinline__ void bare_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// What is done with a step's fragments: acc[x][y] += a's block x, b's block y; with SUM also sum[x] += a's lines
+// How four waves share an LA x LB product tile: two along a's lines, two along b's
+template <int LA, int LB>
+struct Share {
+  static constexpr int NA = LA / 32, NB = LB / 32;   // blocks of 16 lines of a wave
+  static __device__ __forceinline__ int line_a() { return ((threadIdx.x >> 6) & 1) * (LA / 2); }
+  static __device__ __forceinline__ int line_b() { return (threadIdx.x >> 7) * (LB / 2); }
+};
+
+// What is done with fragments: acc[x][y] += a's block x, b's block y; with SUM also sum[x] += a's lines
 template <class T, int NA, int NB, bool SUM>
 struct Accumulate {
   f4v acc[NA][NB], sum[NA];
@@ -202,62 +210,68 @@ struct Accumulate {
       for (int y = 0; y < NB; ++y) acc[x][y] = f4v{0.f, 0.f, 0.f, 0.f};
     }
   }
-  __device__ __forceinline__ void step(const u4v (&fa)[2][NA], const u4v (&fb)[2][NB], bool sums) {
-    if constexpr (sizeof(T) == 4) {
-      Thirds a[NA], b[NB];
+  // one sub-step of 16-bit values
+  __device__ __forceinline__ void add(const u4v (&fa)[NA], const u4v (&fb)[NB], bool sums) {
 #pragma unroll
-      for (int x = 0; x < NA; ++x) a[x].set(fa[0][x], fa[1][x]);
+    for (int x = 0; x < NA; ++x)
 #pragma unroll
-      for (int y = 0; y < NB; ++y) b[y].set(fb[0][y], fb[1][y]);
+      for (int y = 0; y < NB; ++y) acc[x][y] = product<T>(fb[y], fa[x], acc[x][y]);
+    if (SUM && sums) {
+      const unsigned one = TypeCode<T>::V == NFI_BF16 ? 0x3f803f80u : 0x3c003c00u;
+      const u4v ones = {one, one, one, one};
 #pragma unroll
-      for (int x = 0; x < NA; ++x)
+      for (int x = 0; x < NA; ++x) sum[x] = product<T>(ones, fa[x], sum[x]);
+    }
+  }
+  // a step of 32-bit values; the next block of a is cut into its parts while a block's products run
+  __device__ __forceinline__ void add32(const u4v (&fa)[2][NA], const u4v (&fb)[2][NB], bool sums) {
+    Thirds a[NA], b[NB];
 #pragma unroll
-        for (int y = 0; y < NB; ++y) acc[x][y] = product(b[y], a[x], acc[x][y]);
-      if (SUM && sums) {
-        const unsigned one = 0x3f803f80u;
-        const u4v ones = {one, one, one, one};
+    for (int y = 0; y < NB; ++y) b[y].set(fb[0][y], fb[1][y]);
+    a[0].set(fa[0][0], fa[1][0]);
 #pragma unroll
-        for (int x = 0; x < NA; ++x) {
-          sum[x] = product<bf16_t>(ones, a[x].l, sum[x]);
-          sum[x] = product<bf16_t>(ones, a[x].m, sum[x]);
-          sum[x] = product<bf16_t>(ones, a[x].h, sum[x]);
-        }
+    for (int x = 0; x < NA; ++x) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (x + 1 < NA) a[x + 1].set(fa[0][x + 1], fa[1][x + 1]);
+#pragma unroll
+      for (int y = 0; y < NB; ++y) acc[x][y] = product(b[y], a[x], acc[x][y]);
+#pragma unroll
+      for (int k = 0; k < 6 * NB; ++k) {   // a product, two other instructions, and so on
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
       }
-    } else {
+    }
+    if (SUM && sums) {
+      const unsigned one = 0x3f803f80u;
+      const u4v ones = {one, one, one, one};
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-        for (int x = 0; x < NA; ++x)
-#pragma unroll
-          for (int y = 0; y < NB; ++y) acc[x][y] = product<T>(fb[sub][y], fa[sub][x], acc[x][y]);
-      if (SUM && sums) {
-        const unsigned one = TypeCode<T>::V == NFI_BF16 ? 0x3f803f80u : 0x3c003c00u;
-        const u4v ones = {one, one, one, one};
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-          for (int x = 0; x < NA; ++x) sum[x] = product<T>(ones, fa[sub][x], sum[x]);
+      for (int x = 0; x < NA; ++x) {
+        sum[x] = product<bf16_t>(ones, a[x].l, sum[x]);
+        sum[x] = product<bf16_t>(ones, a[x].m, sum[x]);
+        sum[x] = product<bf16_t>(ones, a[x].h, sum[x]);
       }
     }
   }
 };
 
-// An LA x LB product tile by 4 waves of (LA / 2) x (LB / 2): steps over the contracted index through two stages of LDS, each of
-// (LA + LB) x 128 bytes.  A step's fragments go to registers at once, its stage is free after a barrier, and the loads of the step
-// after next are made into it while the step's products run: loads have a whole step to arrive.  (The stages are two variables of
-// their own: the compiler waits for all loads into the one that is read, and for no others.)
+// An LA x LB product tile: steps over the contracted index through two stages of LDS, each of (LA + LB) x 128 bytes.  A step's
+// fragments go to registers, its stage is free after a barrier, and the loads of the step after next are made into it while the
+// step's (last) products run: loads have a whole step to arrive.  (The stages are two variables of their own: the compiler waits
+// for all loads into the one that is read, and for no others.)
 template <class T, bool SLAB_A, bool SLAB_B, int LA, int LB, bool SUM>
 __device__ __forceinline__ void tile_product(const unsigned char* a, unsigned lda, int lines_a, const unsigned char* b, unsigned ldb,
                                              int lines_b, int64_t contracted, unsigned char* s0, unsigned char* s1,
-                                             Accumulate<T, LA / 32, LB / 32, SUM>& out, bool sums) {
-  constexpr int KSTEP = STEP_BYTES / sizeof(T), NA = LA / 32, NB = LB / 32, LOADS = NA + NB;
-  TileLoad<T, SLAB_A, LA> la;
-  TileLoad<T, SLAB_B, LB> lb;
+                                             Accumulate<T, Share<LA, LB>::NA, Share<LA, LB>::NB, SUM>& out, bool sums) {
+  typedef Share<LA, LB> S;
+  typedef TileLoad<T, SLAB_A, LA> LoadA;
+  typedef TileLoad<T, SLAB_B, LB> LoadB;
+  constexpr int KSTEP = STEP_BYTES / sizeof(T), NA = S::NA, NB = S::NB, LOADS = LoadA::LOADS + LoadB::LOADS;
+  LoadA la;
+  LoadB lb;
   la.init(lines_a, lda);
   lb.init(lines_b, ldb);
   const int64_t step_a = SLAB_A ? (int64_t)KSTEP * lda : STEP_BYTES, step_b = SLAB_B ? (int64_t)KSTEP * ldb : STEP_BYTES;
-  const int steps = (int)((contracted + KSTEP - 1) / KSTEP);
-  const int wave = threadIdx.x >> 6, line_a = (wave & 1) * (LA / 2), line_b = (wave >> 1) * (LB / 2);
+  const int steps = (int)((contracted + KSTEP - 1) / KSTEP), line_a = S::line_a(), line_b = S::line_b();
   // (a step behind the last reads nothing and clears its stage: every step waits for the same number of loads)
   auto issue = [&](int t, unsigned char* dst) {
     const int64_t k = contracted - (int64_t)t * KSTEP;
@@ -266,19 +280,25 @@ __device__ __forceinline__ void tile_product(const unsigned char* a, unsigned ld
     lb.issue(b + t * step_b, dst + LA * STEP_BYTES, SLAB_B ? left : left * (int)sizeof(T));
     __builtin_amdgcn_sched_barrier(0);   // the waits count on this order of the steps' loads
   };
+  auto read = [&](const unsigned char* cur, int sub, u4v (&fa)[NA], u4v (&fb)[NB]) {
+    read_fragments<T, SLAB_A, LA, NA>(cur, line_a, sub, fa);
+    read_fragments<T, SLAB_B, LB, NB>(cur + LA * STEP_BYTES, line_b, sub, fb);
+  };
   auto step = [&](int t, unsigned char* cur) {
     wait_loads<LOADS>();   // step t's loads are in LDS, those of step t + 1 may be on their way
     bare_barrier();
     u4v fa[2][NA], fb[2][NB];
-#pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-      read_fragments<T, SLAB_A, LA, NA>(cur, line_a, sub, fa[sub]);
-      read_fragments<T, SLAB_B, LB, NB>(cur + LA * STEP_BYTES, line_b, sub, fb[sub]);
-    }
+    read(cur, 0, fa[0], fb[0]);
+    read(cur, 1, fa[1], fb[1]);
     __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): this wave has read the step
     bare_barrier();
     issue(t + 2, cur);
-    out.step(fa, fb, sums);
+    if constexpr (sizeof(T) == 4) {
+      out.add32(fa, fb, sums);
+    } else {
+      out.add(fa[0], fb[0], sums);
+      out.add(fa[1], fb[1], sums);
+    }
   };
   issue(0, s0);
   issue(1, s1);
