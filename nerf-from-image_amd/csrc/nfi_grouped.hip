@@ -63,15 +63,6 @@ __device__ __forceinline__ int find_tile(const GroupedArgs& p, int64_t tile, int
   return -1;
 }
 
-template <class T>
-__device__ __forceinline__ void store4(T* p, const float (&v)[4], int count) {
-  if (count >= 4) {
-    store_piece<T, 4>(p, v);
-  } else {
-    for (int r = 0; r < count; ++r) p[r] = (T)v[r];
-  }
-}
-
 // y (SLAB_B false: b = w[e], rows of K) and d x (SLAB_B true: a = dy, b = w[e] as slabs): rows of `a` by tiles of 128 x LB
 template <class T, bool SLAB_B, int LB>
 __global__ void __launch_bounds__(256, 2) grouped_rows(const GroupedArgs p) {
@@ -92,23 +83,21 @@ __global__ void __launch_bounds__(256, 2) grouped_rows(const GroupedArgs p) {
     const unsigned char* b = p.b + e * p.sb + (SLAB_B ? (int64_t)c0 * (int)sizeof(T) : (int64_t)c0 * p.ldb);
     tile_product<T, false, SLAB_B, TILE, LB>(p.a + r0 * p.lda, p.lda, rows, b, p.ldb, cols, p.k, s0, s1, out, false);
   }
-  const int i = lane_id() & 15, g = lane_id() >> 4;
+  const int line_a = S::line_a(), line_b = S::line_b();
+  if constexpr (!SLAB_B) {
+    if (p.bias && e < p.groups) {
+      const int g = lane_id() >> 4;
 #pragma unroll
-  for (int y = 0; y < S::NB; ++y) {
-    const int n = S::line_b() + y * 16 + 4 * g;
-    float bias[4] = {0.f, 0.f, 0.f, 0.f};
-    if (p.bias && e < p.groups)   // (one after the other in flight: clamped, not skipped)
+      for (int y = 0; y < S::NB; ++y) {
+        f4v bias;   // (all in flight: clamped, not skipped)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) bias[r] = (float)((const T*)p.bias)[(int64_t)e * p.n + c0 + min(n + r, cols - 1)];
+        for (int r = 0; r < 4; ++r) bias[r] = (float)((const T*)p.bias)[(int64_t)e * p.n + c0 + min(line_b + y * 16 + 4 * g + r, cols - 1)];
 #pragma unroll
-    for (int x = 0; x < S::NA; ++x) {
-      const int row = S::line_a() + x * 16 + i;
-      float v[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = out.acc[x][y][r] + bias[r];
-      if (row < rows) store4<T>((T*)p.out + (r0 + row) * p.n + c0 + n, v, cols - n);
+        for (int x = 0; x < S::NA; ++x) out.acc[x][y] += bias;
+      }
     }
   }
+  store_part<T, S::NA, S::NB>(out.acc, S::room(s0, s1), (T*)p.out + (r0 + line_a) * p.n + c0 + line_b, p.n, rows - line_a, cols - line_b);
 }
 
 // d w[e] [N][K] and d b[e]: a = dy as slabs (its columns are the lines), b = x as slabs, tiles of L x L.  Partial results: part [split][group][N][K], then part_b [split][group][N].
@@ -130,26 +119,19 @@ __global__ void __launch_bounds__(256, 2) grouped_weights(const GroupedArgs p, i
   const bool sums = gb != nullptr && c0 == 0;
   tile_product<T, true, true, L, L>(p.a + r0 * p.lda + m0 * (int64_t)sizeof(T), p.lda, lines, p.b + r0 * p.ldb + c0 * (int64_t)sizeof(T),
                                     p.ldb, cols, r1 - r0, s0, s1, acc, sums);
-  const int i = lane_id() & 15, g = lane_id() >> 4;
-  const int64_t matrix = (int64_t)n_rows * p.n;
+  const int i = lane_id() & 15, g = lane_id() >> 4, line_a = S::line_a(), line_b = S::line_b();
+  if (sums && line_b == 0 && g == 0) {
 #pragma unroll
-  for (int x = 0; x < S::NA; ++x) {
-    const int row = S::line_a() + x * 16 + i;
-    if (row >= lines) continue;
-    if (sums && S::line_b() == 0 && g == 0) {
+    for (int x = 0; x < S::NA; ++x) {
+      const int row = line_a + x * 16 + i;
+      if (row >= lines) continue;
       if (p.splits == 1) ((T*)gb)[(int64_t)e * n_rows + m0 + row] = (T)acc.sum[x][0];
       else part_b[(int64_t)place * n_rows + m0 + row] = acc.sum[x][0];
     }
-    if (p.out == nullptr) continue;
-#pragma unroll
-    for (int y = 0; y < S::NB; ++y) {
-      const int n = S::line_b() + y * 16 + 4 * g;
-      const float v[4] = {acc.acc[x][y][0], acc.acc[x][y][1], acc.acc[x][y][2], acc.acc[x][y][3]};
-      const int64_t at = (int64_t)(m0 + row) * p.n + c0 + n;
-      if (p.splits == 1) store4<T>((T*)p.out + e * matrix + at, v, cols - n);
-      else store4<float>(p.part + place * matrix + at, v, cols - n);
-    }
   }
+  const int64_t matrix = (int64_t)n_rows * p.n, at = (int64_t)(m0 + line_a) * p.n + c0 + line_b;
+  if (p.splits == 1) store_part<T, S::NA, S::NB>(acc.acc, S::room(s0, s1), (T*)p.out + e * matrix + at, p.n, lines - line_a, cols - line_b);
+  else store_part<float, S::NA, S::NB>(acc.acc, S::room(s0, s1), p.part + place * matrix + at, p.n, lines - line_a, cols - line_b);
 }
 
 // d b[e] alone: 64 columns x 4 rows at a time; blockIdx.y the group, .z the split

@@ -196,6 +196,10 @@ struct Share {
   static constexpr int NA = LA / 32, NB = LB / 32;   // blocks of 16 lines of a wave
   static __device__ __forceinline__ int line_a() { return ((threadIdx.x >> 6) & 1) * (LA / 2); }
   static __device__ __forceinline__ int line_b() { return (threadIdx.x >> 7) * (LB / 2); }
+  // a wave's room for its part, of at most 4 bytes an element, in the stages of a product that has ended
+  static __device__ __forceinline__ unsigned char* room(unsigned char* s0, unsigned char* s1) {
+    return (threadIdx.x >> 7 ? s1 : s0) + ((threadIdx.x >> 6) & 1) * (LA / 2 * LB / 2 * 4);
+  }
 };
 
 // What is done with fragments: acc[x][y] += a's block x, b's block y; with SUM also sum[x] += a's lines
@@ -309,6 +313,59 @@ __device__ __forceinline__ void tile_product(const unsigned char* a, unsigned ld
   }
   if (t < steps) step(t, s0);
   wait_loads<0>();
+  bare_barrier();   // the stages are free: no wave reads, and no load is on its way
+}
+
+// A wave's part of a product tile to rows of `out` (ld elements apart; `rows` x `cols` of them from this wave's
+// corner are the matrix's).  A lane holds 4 columns of a row, 32 bytes of a row's line in a 16-bit store: the part is turned in
+// LDS first, where the wave has room for it, and leaves in pieces of 16 bytes, a row's one after the other (32,749 rows of
+// 1024 -> 4096: 410 -> EPI us).
+template <class O, int NA, int NB>
+__device__ __forceinline__ void store_part(const f4v (&acc)[NA][NB], unsigned char* lds, O* out, int64_t ld, int rows, int cols) {
+  constexpr int V = 16 / (int)sizeof(O), PIECES = NB * (int)sizeof(O), AT_ONCE = 64 / PIECES;   // pieces of a row; rows of a store
+  const int l = lane_id(), i = l & 15, g = l >> 4;
+#pragma unroll
+  for (int x = 0; x < NA; ++x)
+#pragma unroll
+    for (int y = 0; y < NB; ++y) {
+      const int row = 16 * x + i, byte = (16 * y + 4 * g) * (int)sizeof(O);
+      unsigned char* p = lds + row * (PIECES * 16) + (((byte >> 4) ^ (row & (PIECES - 1))) << 4) + (byte & 15);
+      const f4v v = acc[x][y];
+      if constexpr (sizeof(O) == 4) {
+        lds_st_fenced((f4v*)p, v);
+      } else {
+        O t[4] = {(O)v[0], (O)v[1], (O)v[2], (O)v[3]};
+        u2v u;
+        __builtin_memcpy(&u, t, 8);
+        lds_st_fenced((u2v*)p, u);
+      }
+    }
+  asm volatile("" ::: "memory");
+  const int piece = l & (PIECES - 1), row0 = l / PIECES, have = cols - piece * V;
+  constexpr int STORES = 16 * NA / AT_ONCE, GROUP = STORES < 8 ? STORES : 8;
+#pragma unroll
+  for (int j0 = 0; j0 < STORES; j0 += GROUP) {
+    u4v v[GROUP];
+#pragma unroll
+    for (int j = 0; j < GROUP; ++j) {
+      const int row = row0 + (j0 + j) * AT_ONCE;
+      v[j] = *reinterpret_cast<const u4v*>(lds + row * (PIECES * 16) + ((piece ^ (row & (PIECES - 1))) << 4));
+    }
+#pragma unroll
+    for (int j = 0; j < GROUP; ++j) {
+      const int row = row0 + (j0 + j) * AT_ONCE;
+      O* d = out + row * ld + piece * V;
+      if (row < rows && have >= V) {
+        __builtin_memcpy(d, &v[j], 16);
+      } else if (row < rows) {
+        O t[V];
+        __builtin_memcpy(t, &v[j], 16);
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+          if (k < have) d[k] = t[k];
+      }
+    }
+  }
 }
 
 }  // namespace learn

@@ -277,48 +277,68 @@ __device__ __forceinline__ void pair_product(const _Float16* a, unsigned lda, co
   }
   if (t < steps) step(t, s0);
   wait_loads<0>();
+  bare_barrier();   // the stages are free: no wave reads, and no load is on its way
 }
 
-// a 128 x 128 tile of a symmetric matrix in halves to (r0, c0), and mirrored to (c0, r0) off the diagonal: the mirror goes
-// through LDS, rows 0 .. 63 of the tile in s0 and 64 .. 127 in s1
-__device__ __forceinline__ void store_symmetric(_Float16* d, int ld, int r0, int c0, const f4v (&v)[4][4], unsigned char* s0, unsigned char* s1) {
-  const int wave = threadIdx.x >> 6, i = lane_id() & 15, g = lane_id() >> 4;
-  const int la = (wave & 1) * 64, lb = (wave >> 1) * 64;
-  float *f0 = (float*)s0, *f1 = (float*)s1;
-  __syncthreads();   // (the last step's fragments have been read)
+// a wave's 64 x 64 part of a tile in halves to rows of `ld` halves from d, turned in LDS on the way (store_part in nfi_mm.h): 256
+// bytes of a row at a time in place of 32 (X' of 512 x 4608, 24 of them: OLD -> NEW us)
+__device__ __forceinline__ void store_pairs(const f4v (&acc)[4][4], float scale, unsigned char* lds, _Float16* d, int64_t ld) {
+  const int l = lane_id(), i = l & 15, g = l >> 4;
 #pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    const int row = 16 * x + i;
+  for (int x = 0; x < 4; ++x)
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
-      const int col = lb + 16 * y + 4 * g;
-      const float u[4] = {v[x][y][0], v[x][y][1], v[x][y][2], v[x][y][3]};
+      const float v[4] = {acc[x][y][0] * scale, acc[x][y][1] * scale, acc[x][y][2] * scale, acc[x][y][3] * scale};
       h4v hi, lo;
-      split4(u, hi, lo);
-      _Float16* p = d + (int64_t)(r0 + la + row) * ld + half_at(c0 + col);
-      *reinterpret_cast<h4v*>(p) = hi;
-      *reinterpret_cast<h4v*>(p + 32) = lo;
-      if (r0 != c0) lds_st_fenced(reinterpret_cast<f4v*>((la ? f1 : f0) + row * 128 + (col ^ (((row >> 2) & 3) << 4))), v[x][y]);
+      split4(v, hi, lo);
+      const int row = 16 * x + i, col = 16 * y + 4 * g, piece = half_at(col) >> 3;   // of 8 halves; lo: 4 pieces on
+      unsigned char* q = lds + row * 256 + (col & 4) * 2;
+      lds_st_fenced((h4v*)(q + ((piece ^ i) << 4)), hi);
+      lds_st_fenced((h4v*)(q + (((piece + 4) ^ i) << 4)), lo);
     }
-  }
-  if (r0 == c0) return;
-  __syncthreads();
+  asm volatile("" ::: "memory");
 #pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    const int row = la + 16 * x + i;   // a column of the tile
+  for (int j0 = 0; j0 < 16; j0 += 8) {
+    u4v v[8];
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      const int col = 16 * y + 4 * g;  // rows of the tile, of the half that lb names
-      float u[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) u[r] = (lb ? f1 : f0)[(col + r) * 128 + (row ^ ((((col + r) >> 2) & 3) << 4))];
-      h4v hi, lo;
-      split4(u, hi, lo);
-      _Float16* p = d + (int64_t)(c0 + row) * ld + half_at(r0 + lb + col);
-      *reinterpret_cast<h4v*>(p) = hi;
-      *reinterpret_cast<h4v*>(p + 32) = lo;
+    for (int j = 0; j < 8; ++j) {
+      const int row = 4 * (j0 + j) + g;
+      v[j] = *reinterpret_cast<const u4v*>(lds + row * 256 + ((i ^ (row & 15)) << 4));
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) *reinterpret_cast<u4v*>(d + (4 * (j0 + j) + g) * ld + 8 * i) = v[j];
   }
+}
+
+// a wave's 64 x 64 part, turned
+__device__ __forceinline__ void turn_part(f4v (&v)[4][4], unsigned char* lds) {
+  const int i = lane_id() & 15, g = lane_id() >> 4;
+  float* f = (float*)lds;
+  auto at = [](int row, int col) { return row * 64 + (col ^ (((row >> 2) & 3) << 4) ^ ((row & 3) << 2)); };
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) lds_st_fenced(reinterpret_cast<f4v*>(f + at(16 * x + i, 16 * y + 4 * g)), v[x][y]);
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[x][y][r] = f[at(16 * y + 4 * g + r, 16 * x + i)];
+  asm volatile("" ::: "memory");
+}
+
+// a 128 x 128 tile of a symmetric matrix in halves to (r0, c0), and mirrored to (c0, r0) off the diagonal
+__device__ __forceinline__ void store_symmetric(_Float16* d, int ld, int r0, int c0, f4v (&v)[4][4], unsigned char* s0, unsigned char* s1) {
+  typedef Share<TILE, TILE> S;
+  unsigned char* room = S::room(s0, s1);
+  r0 += S::line_a();
+  c0 += S::line_b();
+  store_pairs(v, 1.f, room, d + (int64_t)r0 * ld + half_at(c0), ld);
+  if (r0 / TILE == c0 / TILE) return;
+  turn_part(v, room);
+  store_pairs(v, 1.f, room, d + (int64_t)c0 * ld + half_at(r0), ld);
 }
 
 __device__ __forceinline__ void triangle(int unit, int& ti, int& tj) {
@@ -424,7 +444,13 @@ __device__ __forceinline__ void put_update(const Args& p, const Item& t, int64_t
   for (int r = 0; r < 4; ++r) v[r] = acc[r] * s;
   if (p.update) {
     const float step = p.step * t.scale;
-    for (int r = 0; r < count; ++r) v[r] = fmaf(p.keep, typed_at(t.w, p.w_type, at + r), -step * v[r]);
+    if (p.w_type == NFI_F32 && count == 4) {
+      float w[4];
+      load_piece<float, 4>((const float*)t.w + at, w);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = fmaf(p.keep, w[r], -step * v[r]);
+    } else
+      for (int r = 0; r < count; ++r) v[r] = fmaf(p.keep, typed_at(t.w, p.w_type, at + r), -step * v[r]);
   }
   if (p.w_type == NFI_F32) {
     if (count == 4) store_piece<float, 4>((float*)t.w + at, v);
@@ -462,23 +488,17 @@ __global__ void __launch_bounds__(256, 2) ortho_apply(const Table<N> p) {
     return;
   }
   pair_product<true, false>(q, 4u * t.mp, x, 4u * t.np, t.mp / 32, s0, s1, acc);
-  _Float16* d = t.y + (int64_t)matrix * t.mp * 2 * t.np;
+  if (p.last) {
 #pragma unroll
-  for (int xx = 0; xx < 4; ++xx)
+    for (int xx = 0; xx < 4; ++xx)
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      const int row = r0 + la + 16 * xx + i, col = c0 + lb + 16 * y + 4 * g;
-      if (p.last) {
+      for (int y = 0; y < 4; ++y) {
+        const int row = r0 + la + 16 * xx + i, col = c0 + lb + 16 * y + 4 * g;
         if (row < t.m && col < t.n) put_update(p, t, base + (int64_t)row * t.cols + col, acc[xx][y], s, min(4, t.n - col));
-      } else {
-        const float v[4] = {acc[xx][y][0] * down, acc[xx][y][1] * down, acc[xx][y][2] * down, acc[xx][y][3] * down};
-        h4v hi, lo;
-        split4(v, hi, lo);
-        _Float16* o = d + (int64_t)row * 2 * t.np + half_at(col);
-        *reinterpret_cast<h4v*>(o) = hi;
-        *reinterpret_cast<h4v*>(o + 32) = lo;
       }
-    }
+    return;
+  }
+  store_pairs(acc, down, Share<TILE, TILE>::room(s0, s1), t.y + ((int64_t)matrix * t.mp + r0 + la) * 2 * t.np + half_at(c0 + lb), 2 * t.np);
 }
 
 // ---- small matrices ----------------------------------------------------------------------------------------------------
