@@ -24,7 +24,10 @@ namespace nfi {
 namespace learn {
 
 constexpr int PARAMS = 5;       // d weight, d bias, d next_weight, d next_bias, d gate
-constexpr int BLOCKS = 512;     // workgroups of the backward (two for each of 256 compute units)
+
+// Workgroups of the backward: two for each of 256 compute units, three where a row's four waves meet twice a row and wait
+// (16,384 rows of 1024 bf16: 66 -> 58 us; 131,072 rows of 64 in one wave each lose, 31 -> 35)
+__host__ inline int blocks_of(int width) { return width > 512 && width <= 1024 ? 768 : 512; }
 
 // sum over TPR lanes (a power of two up to 64), in every one of them
 template <int TPR>
@@ -80,6 +83,18 @@ struct Row {
   __device__ __forceinline__ void load(const void* p, int64_t at, int width) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) load_piece<T, V>((const T*)p + at + col(c, width), v[c]);
+  }
+  // the same in two steps: the bits, and later their values
+  struct Bits { T t[NC][V]; };
+  static __device__ __forceinline__ void load_bits(Bits& b, const void* p, int64_t at, int width) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) __builtin_memcpy(b.t[c], (const T*)p + at + col(c, width), sizeof(T) * V);
+  }
+  __device__ __forceinline__ void set(const Bits& b) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[c][j] = (float)b.t[c][j];
   }
   __device__ __forceinline__ void load_param(const void* p, int type, int64_t at, int width, float fill) {
     if (p == nullptr) {
@@ -203,16 +218,17 @@ struct Plan {
 // (a gate for each row alone needs no sum)
 __host__ inline int64_t summed_groups(int64_t rows, int64_t groups, bool affine) { return groups > 0 && (groups < rows || affine) ? groups : 1; }
 
-__host__ inline Plan make_plan(int64_t rows, int64_t groups, bool affine, int slots) {
+__host__ inline Plan make_plan(int64_t rows, int64_t groups, bool affine, int width, int slots) {
   Plan p;
+  const int64_t blocks = blocks_of(width);
   const int64_t g = summed_groups(rows, groups, affine);
   p.rows_per_gate = rows / g;
-  const int64_t want = std::max<int64_t>(1, BLOCKS / g);
+  const int64_t want = std::max<int64_t>(1, blocks / g);
   const int64_t most = (p.rows_per_gate + slots - 1) / slots;
   p.splits = (int)std::min(want, most);
   p.rows_per_split = (p.rows_per_gate + p.splits - 1) / p.splits;
   p.segments = g * p.splits;
-  p.per = p.splits > 1 ? 1 : (p.segments + BLOCKS - 1) / BLOCKS;
+  p.per = p.splits > 1 ? 1 : (p.segments + blocks - 1) / blocks;
   p.blocks = (int)((p.segments + p.per - 1) / p.per);
   return p;
 }
@@ -264,28 +280,60 @@ __global__ void __launch_bounds__((TPR > 256 ? TPR : 256)) resnorm_bwd(const nfi
       acc[0][c][j] = acc[1][c][j] = acc[2][c][j] = acc[3][c][j] = 0.f;
       accg[c][j] = 0.f;
     }
+  // up to one piece of 16 bytes a lane there are registers for the next row's bits, which arrive while a row is worked on, and for the
+  // parameters that the rows share (16,384 rows of 1024 bf16, together: 88 -> 58 us)
+  constexpr bool AHEAD = NC * R::V * (int)sizeof(T) <= 16;
+  const bool keep = AHEAD && !a.affine_groups;
+  R gate, w, b, w2;
+  auto load_params = [&](int64_t at) {
+    w.load_param(a.weight, a.param_dtype, at, width, 1.f);
+    b.load_param(a.bias, a.param_dtype, at, width, 0.f);
+    if (a.gy) w2.load_param(a.next_weight, a.param_dtype, at, width, 1.f);
+  };
+  if (keep) load_params(0);
   const int64_t last = min((int64_t)(blockIdx.x + 1) * p.per, p.segments);
   for (int64_t seg = (int64_t)blockIdx.x * p.per; seg < last; ++seg) {
     const int64_t gi = seg / p.splits, piece = seg - gi * p.splits;
     const int64_t r0 = gi * p.rows_per_gate + piece * p.rows_per_split;
     const int64_t r1 = min(r0 + p.rows_per_split, (gi + 1) * p.rows_per_gate);
-    for (int64_t row = r0 + threadIdx.x / TPR; row < r1; row += R::SLOTS) {
+    const bool keep_gate = AHEAD && a.gate && !row_gate;
+    if (keep_gate) gate.load_param(a.gate, a.gate_dtype, gi * width, width, 1.f);
+    typename R::Bits bh, bres, bg, bgy;
+    float4 next_st;
+    auto ahead = [&](int64_t row) {
       const int64_t at = row * width;
-      R h, res, g, gy, gate, w;
-      h.load(a.h, at, width);
-      if (a.residual) res.load(a.residual, at, width);
-      if (a.gx) g.load(a.gx, at, width);
-      if (a.gy) gy.load(a.gy, at, width);
-      if (a.gate) gate.load_param(a.gate, a.gate_dtype, (row_gate ? row : gi) * width, width, 1.f);
-      const int64_t param_at = a.affine_groups ? gi * width : 0;
-      w.load_param(a.weight, a.param_dtype, param_at, width, 1.f);
-      R b;
-      b.load_param(a.bias, a.param_dtype, param_at, width, 0.f);
-      const float4 st = *reinterpret_cast<const float4*>(a.stats + 4 * row);
+      R::load_bits(bh, a.h, at, width);
+      if (a.residual) R::load_bits(bres, a.residual, at, width);
+      if (a.gx) R::load_bits(bg, a.gx, at, width);
+      if (a.gy) R::load_bits(bgy, a.gy, at, width);
+      next_st = *reinterpret_cast<const float4*>(a.stats + 4 * row);
+    };
+    const int64_t mine = r0 + threadIdx.x / TPR;
+    if (AHEAD && mine < r1) ahead(mine);
+    for (int64_t row = mine; row < r1; row += R::SLOTS) {
+      const int64_t at = row * width;
+      R h, res, g, gy;
+      if constexpr (!AHEAD) {
+        R none;   // (nothing is carried from row to row)
+        gate = w = b = w2 = none;
+        h.load(a.h, at, width);
+        if (a.residual) res.load(a.residual, at, width);
+        if (a.gx) g.load(a.gx, at, width);
+        if (a.gy) gy.load(a.gy, at, width);
+        next_st = *reinterpret_cast<const float4*>(a.stats + 4 * row);
+      } else {
+        h.set(bh);
+        if (a.residual) res.set(bres);
+        if (a.gx) g.set(bg);
+        if (a.gy) gy.set(bgy);
+      }
+      const float4 st = next_st;
+      if (AHEAD && row + R::SLOTS < r1) ahead(row + R::SLOTS);
+      if (a.gate && !keep_gate) gate.load_param(a.gate, a.gate_dtype, (row_gate ? row : gi) * width, width, 1.f);
+      if (!keep) load_params(a.affine_groups ? gi * width : 0);
       // h becomes n, res becomes v (the gated value is scale (res + gate v))
       float s[2] = {0.f, 0.f};
-      R w2;
-      if (a.gy) w2.load_param(a.next_weight, a.param_dtype, param_at, width, 1.f);
+      R m2, &m_of = AHEAD ? m2 : w2;   // (w2 is not needed again, but for the next row)
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -306,7 +354,7 @@ __global__ void __launch_bounds__((TPR > 256 ? TPR : 256)) resnorm_bwd(const nfi
             acc[3][c][j] += q;
             const float qw = q * w2.v[c][j];
             gy.v[c][j] = qw;
-            w2.v[c][j] = m;   // (w2 is not needed again)
+            m_of.v[c][j] = m;
             s[0] += ok ? qw : 0.f;
             s[1] += ok ? qw * m : 0.f;
           }
@@ -319,7 +367,7 @@ __global__ void __launch_bounds__((TPR > 256 ? TPR : 256)) resnorm_bwd(const nfi
         for (int c = 0; c < NC; ++c)
 #pragma unroll
           for (int j = 0; j < R::V; ++j) {
-            const float q = st.w * (gy.v[c][j] - s[0] - w2.v[c][j] * s[1]);
+            const float q = st.w * (gy.v[c][j] - s[0] - m_of.v[c][j] * s[1]);
             g.v[c][j] = a.gx ? g.v[c][j] + q : q;
           }
       }
@@ -425,44 +473,67 @@ __global__ void __launch_bounds__(1024) resnorm_join(const nfi_resnorm_args a, c
   }
 }
 
-template <class T, int V, int TPR, int NC, bool EXACT>
+enum Way { BOTH, FORWARD, BACKWARD };
+
+template <class T, int V, int TPR, int NC, bool EXACT, Way WAY>
 static void launch(const nfi_resnorm_args& a, bool backward, hipStream_t s) {
   typedef Row<T, V, TPR, NC, EXACT> R;
-  if (!backward) {
-    const int64_t need = (a.rows + R::SLOTS - 1) / R::SLOTS;
-    resnorm_fwd<T, V, TPR, NC, EXACT><<<(unsigned)std::min<int64_t>(need, 8192), R::BLK, 0, s>>>(a);
-    return;
+  if constexpr (WAY != BACKWARD) {
+    if (!backward) {
+      const int64_t need = (a.rows + R::SLOTS - 1) / R::SLOTS;
+      resnorm_fwd<T, V, TPR, NC, EXACT><<<(unsigned)std::min<int64_t>(need, 8192), R::BLK, 0, s>>>(a);
+      return;
+    }
   }
-  const Plan p = make_plan(a.rows, a.groups, a.affine_groups, R::SLOTS);
+  if constexpr (WAY == FORWARD) return;
+  else {
+  const Plan p = make_plan(a.rows, a.groups, a.affine_groups, a.width, R::SLOTS);
   resnorm_bwd<T, V, TPR, NC, EXACT><<<(unsigned)p.blocks, R::BLK, 0, s>>>(a, p);
   const bool params = (a.dweight || a.dbias || a.dnext_weight || a.dnext_bias) && (p.splits > 1 || !a.affine_groups);
   const bool gate = a.dgate && (a.groups < a.rows || a.affine_groups) && p.splits > 1;
-  const bool each = gate || (params && a.affine_groups);   // (a group's own sums: fewer than BLOCKS groups)
+  const bool each = gate || (params && a.affine_groups);   // (a group's own sums: fewer groups than workgroups)
   if (params || gate)
     resnorm_join<<<dim3((unsigned)((a.width + 15) / 16), gate ? 5 : 4, (unsigned)(each ? a.groups : 1)), 1024, 0, s>>>(a, p);
+  }
 }
 
-template <class T, int TPR, int NC>
+template <class T, int V, int TPR, int NC, Way WAY = BOTH>
 static void pick_exact(const nfi_resnorm_args& a, bool backward, hipStream_t s) {
-  constexpr int V = 16 / sizeof(T);
-  if (a.width == TPR * NC * V) launch<T, V, TPR, NC, true>(a, backward, s);
-  else launch<T, V, TPR, NC, false>(a, backward, s);
+  if (a.width == TPR * NC * V) launch<T, V, TPR, NC, true, WAY>(a, backward, s);
+  else launch<T, V, TPR, NC, false, WAY>(a, backward, s);
 }
 
 template <class T>
 static void dispatch(const nfi_resnorm_args& a, bool backward, hipStream_t s) {
   constexpr int V = 16 / sizeof(T);
   const int n = (a.width + V - 1) / V;
-  if (a.width < V) launch<T, 1, 8, 1, false>(a, backward, s);   // (a piece does not fit into the row)
-  else if (n <= 8) pick_exact<T, 8, 1>(a, backward, s);
-  else if (n <= 16) pick_exact<T, 16, 1>(a, backward, s);
-  else if (n <= 32) pick_exact<T, 32, 1>(a, backward, s);
-  else if (n <= 64) pick_exact<T, 64, 1>(a, backward, s);
-  else if (n <= 128) pick_exact<T, 64, 2>(a, backward, s);
-  else if (n <= 256) pick_exact<T, 256, 1>(a, backward, s);
-  else if (n <= 512) pick_exact<T, 256, 2>(a, backward, s);
-  else if (n <= 1024) pick_exact<T, 512, 2>(a, backward, s);
-  else if constexpr (sizeof(T) == 4) pick_exact<T, 512, 4>(a, backward, s);
+  if (a.width < V) launch<T, 1, 8, 1, false, BOTH>(a, backward, s);   // (a piece does not fit into the row)
+  else if (n <= 8) pick_exact<T, V, 8, 1>(a, backward, s);
+  else if (n <= 16) pick_exact<T, V, 16, 1>(a, backward, s);
+  else if (n <= 32) pick_exact<T, V, 32, 1>(a, backward, s);
+  else if (n <= 64) pick_exact<T, V, 64, 1>(a, backward, s);
+  else if constexpr (sizeof(T) == 2) {
+    // the backward of wide 16-bit rows: a lane's registers hold a row's four tensors, so few elements to a lane, in more waves
+    // (16,384 rows of 1024: two pieces of 8 in one wave 83 us, one of 4 in four waves 57; 4096 rows of 4096: two of 8 in four
+    // waves 104 us, one in eight 54); the forward holds less, and wants the wider loads (30 us, and 37)
+    if (n <= 128) {
+      if (backward) pick_exact<T, 4, 256, 1, BACKWARD>(a, backward, s);
+      else pick_exact<T, V, 64, 2, FORWARD>(a, backward, s);
+    } else if (n <= 256) {
+      pick_exact<T, V, 256, 1>(a, backward, s);
+    } else if (n <= 512) {
+      if (backward) pick_exact<T, V, 512, 1, BACKWARD>(a, backward, s);
+      else pick_exact<T, V, 256, 2, FORWARD>(a, backward, s);
+    } else {
+      pick_exact<T, V, 512, 2>(a, backward, s);
+    }
+  } else {
+    if (n <= 128) pick_exact<T, V, 64, 2>(a, backward, s);
+    else if (n <= 256) pick_exact<T, V, 256, 1>(a, backward, s);
+    else if (n <= 512) pick_exact<T, V, 256, 2>(a, backward, s);
+    else if (n <= 1024) pick_exact<T, V, 512, 2>(a, backward, s);
+    else pick_exact<T, V, 512, 4>(a, backward, s);
+  }
 }
 
 static int check(const nfi_resnorm_args* a, const char* what) {
@@ -494,7 +565,7 @@ int64_t nfi_resnorm_work_bytes(int64_t rows, int64_t groups, int32_t affine_grou
   if (rows <= 0 || groups < 0 || width <= 0) return 0;
   // (the plan's workgroups, whatever number of rows one holds)
   const int64_t g = summed_groups(rows, groups, affine_groups != 0);
-  const int64_t blocks = g >= BLOCKS ? BLOCKS : g * std::max<int64_t>(1, BLOCKS / g);
+  const int64_t most = blocks_of(width), blocks = g >= most ? most : g * std::max<int64_t>(1, most / g);
   return blocks * PARAMS * (int64_t)width * 4;
 }
 
