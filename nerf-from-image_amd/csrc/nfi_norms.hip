@@ -25,9 +25,10 @@ namespace learn {
 
 constexpr int PARAMS = 5;       // d weight, d bias, d next_weight, d next_bias, d gate
 
-// Workgroups of the backward: two for each of 256 compute units, three where a row's four waves meet twice a row and wait
-// (16,384 rows of 1024 bf16: 66 -> 58 us; 131,072 rows of 64 in one wave each lose, 31 -> 35)
-__host__ inline int blocks_of(int width) { return width > 512 && width <= 1024 ? 768 : 512; }
+// Workgroups of the backward, as many as 256 compute units hold at a time: two each; three where a row's four waves meet twice a
+// row and wait (16,384 rows of 1024 bf16: 66 -> 58 us; 131,072 rows of 64, a wave each, lose by it, 31 -> 35); one of eight
+// waves where a row is wider, whose partial results cost most (2048 rows of 8192 bf16: 117 us in place of 143)
+__host__ inline int blocks_of(int width) { return width <= 512 ? 512 : width <= 1024 ? 768 : width <= 2048 ? 512 : 256; }
 
 // sum over TPR lanes (a power of two up to 64), in every one of them
 template <int TPR>
@@ -282,7 +283,7 @@ __global__ void __launch_bounds__((TPR > 256 ? TPR : 256)) resnorm_bwd(const nfi
     }
   // up to one piece of 16 bytes a lane there are registers for the next row's bits, which arrive while a row is worked on, and for the
   // parameters that the rows share (16,384 rows of 1024 bf16, together: 88 -> 58 us)
-  constexpr bool AHEAD = NC * R::V * (int)sizeof(T) <= 16;
+  constexpr bool AHEAD = NC * R::V * (int)sizeof(T) <= 16 && TPR < 1024;
   const bool keep = AHEAD && !a.affine_groups;
   R gate, w, b, w2;
   auto load_params = [&](int64_t at) {
@@ -446,29 +447,31 @@ __global__ void __launch_bounds__((TPR > 256 ? TPR : 256)) resnorm_bwd(const nfi
   if (gate_sum && p.splits > 1) slots_sum<R, TPR, NC>(accg, lds, width, [&](int col, float v) { part[4 * width + col] = v; });
 }
 
-// The workgroups' partials summed in their order, 16 columns x 64 slices of workgroups at a time: blockIdx.y the
+// The workgroups' partials summed in their order, COLS columns x 1024 / COLS slices of workgroups at a time: blockIdx.y the
 // parameter (4: the gate), blockIdx.z the group (its own workgroups), or 0 for parameters of all rows
+template <int COLS>
 __global__ void __launch_bounds__(1024) resnorm_join(const nfi_resnorm_args a, const Plan p) {
-  __shared__ float lds[64][17];
+  constexpr int SLICES = 1024 / COLS;
+  __shared__ float lds[SLICES][COLS + 1];
   const int which = blockIdx.y;
   void* out = which == 0 ? a.dweight : which == 1 ? a.dbias : which == 2 ? a.dnext_weight : which == 3 ? a.dnext_bias : a.dgate;
   const bool grouped = which == 4 || a.affine_groups;
   const int64_t gi = blockIdx.z;
   if (out == nullptr || (!grouped && gi > 0) || (grouped && p.splits == 1)) return;
   const int first = grouped ? (int)(gi * p.splits) : 0, count = grouped ? p.splits : p.blocks;
-  const int col = blockIdx.x * 16 + (threadIdx.x & 15), slice = threadIdx.x >> 4;
+  const int col = blockIdx.x * COLS + (threadIdx.x & (COLS - 1)), slice = threadIdx.x / COLS;
   float s = 0.f;
   if (col < a.width) {
     const float* q = a.work + ((int64_t)first * PARAMS + which) * a.width + col;
 #pragma unroll 8
-    for (int k = slice; k < count; k += 64) s += q[(int64_t)k * PARAMS * a.width];
+    for (int k = slice; k < count; k += SLICES) s += q[(int64_t)k * PARAMS * a.width];
   }
-  lds[slice][threadIdx.x & 15] = s;
+  lds[slice][threadIdx.x & (COLS - 1)] = s;
   __syncthreads();
   if (slice == 0 && col < a.width) {
     float t = 0.f;
-#pragma unroll 16
-    for (int k = 0; k < 64; ++k) t += lds[k][threadIdx.x & 15];
+#pragma unroll
+    for (int k = 0; k < SLICES; ++k) t += lds[k][threadIdx.x & (COLS - 1)];
     store_typed(out, which < 4 ? a.param_dtype : a.gate_dtype, gi * a.width + col, t);
   }
 }
@@ -492,8 +495,13 @@ static void launch(const nfi_resnorm_args& a, bool backward, hipStream_t s) {
   const bool params = (a.dweight || a.dbias || a.dnext_weight || a.dnext_bias) && (p.splits > 1 || !a.affine_groups);
   const bool gate = a.dgate && (a.groups < a.rows || a.affine_groups) && p.splits > 1;
   const bool each = gate || (params && a.affine_groups);   // (a group's own sums: fewer groups than workgroups)
-  if (params || gate)
-    resnorm_join<<<dim3((unsigned)((a.width + 15) / 16), gate ? 5 : 4, (unsigned)(each ? a.groups : 1)), 1024, 0, s>>>(a, p);
+  if (params || gate) {
+    // (few columns need every slice, many want whole lines: 256 partial results of 8192 columns, 37 -> 13 us)
+    const int cols = a.width >= 512 ? 64 : 16;
+    const dim3 grid((unsigned)((a.width + cols - 1) / cols), gate ? 5 : 4, (unsigned)(each ? a.groups : 1));
+    if (cols == 64) resnorm_join<64><<<grid, 1024, 0, s>>>(a, p);
+    else resnorm_join<16><<<grid, 1024, 0, s>>>(a, p);
+  }
   }
 }
 
@@ -515,7 +523,7 @@ static void dispatch(const nfi_resnorm_args& a, bool backward, hipStream_t s) {
   else if constexpr (sizeof(T) == 2) {
     // the backward of wide 16-bit rows: a lane's registers hold a row's four tensors, so few elements to a lane, in more waves
     // (16,384 rows of 1024: two pieces of 8 in one wave 83 us, one of 4 in four waves 57; 4096 rows of 4096: two of 8 in four
-    // waves 104 us, one in eight 54); the forward holds less, and wants the wider loads (30 us, and 37)
+    // waves 101 us, one in eight 49; 2048 rows of 8192: two in eight 117, one in sixteen 79); the forward holds less, and wants the wider loads (30 us, and 37)
     if (n <= 128) {
       if (backward) pick_exact<T, 4, 256, 1, BACKWARD>(a, backward, s);
       else pick_exact<T, V, 64, 2, FORWARD>(a, backward, s);
@@ -525,14 +533,16 @@ static void dispatch(const nfi_resnorm_args& a, bool backward, hipStream_t s) {
       if (backward) pick_exact<T, V, 512, 1, BACKWARD>(a, backward, s);
       else pick_exact<T, V, 256, 2, FORWARD>(a, backward, s);
     } else {
-      pick_exact<T, V, 512, 2>(a, backward, s);
+      if (backward) pick_exact<T, V, 1024, 1, BACKWARD>(a, backward, s);
+      else pick_exact<T, V, 512, 2, FORWARD>(a, backward, s);
     }
   } else {
     if (n <= 128) pick_exact<T, V, 64, 2>(a, backward, s);
     else if (n <= 256) pick_exact<T, V, 256, 1>(a, backward, s);
     else if (n <= 512) pick_exact<T, V, 256, 2>(a, backward, s);
     else if (n <= 1024) pick_exact<T, V, 512, 2>(a, backward, s);
-    else pick_exact<T, V, 512, 4>(a, backward, s);
+    else if (backward) pick_exact<T, V, 1024, 2, BACKWARD>(a, backward, s);   // (2048 rows of 8192: four pieces in eight waves 179 us, two in sixteen 127)
+    else pick_exact<T, V, 512, 4, FORWARD>(a, backward, s);
   }
 }
 
