@@ -64,11 +64,19 @@ class Muon(torch.optim.Optimizer):
         _check('Muon', steps, coefficients, eps)
         super().__init__(params, dict(lr=lr, momentum=momentum, weight_decay=weight_decay, nesterov=nesterov, steps=steps,
                                       coefficients=tuple(coefficients), eps=eps, batched=batched))
-        for group in self.param_groups:
-            for p in group['params']:
-                if p.dim() < 2:
-                    raise ValueError(f'Muon: parameters of two or more dimensions are wanted, not {tuple(p.shape)} '
-                                     '(biases and gains belong to another optimiser)')
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        params = self.param_groups[-1]['params']
+        bad = next((p for p in params if p.dim() < 2), None)
+        twice = len({id(p) for p in params}) < len(params)
+        if bad is None and not twice:
+            return
+        self.param_groups.pop()
+        if bad is not None:
+            raise ValueError(f'Muon: parameters of two or more dimensions are wanted, not {tuple(bad.shape)} '
+                             '(biases and gains belong to another optimiser)')
+        raise ValueError('Muon: a parameter twice in a group (all steps of a group are taken at a time)')
 
     @torch.no_grad()
     def step(self, closure=None):

@@ -151,3 +151,24 @@ def test_ortho_work_is_that_of_the_largest_launch():
     assert bytes_of([(200, 300, 1)] * 32) >= 32 * plain
     assert bytes_of([(200, 300, 1)] * 33) == bytes_of([(200, 300, 1)] * 32)
     assert bytes_of([(128, 128, 1)] * 32 + [(2000, 3000, 1)]) == bytes_of([(2000, 3000, 1)])
+
+
+def test_muon_refuses_vectors_and_repeated_parameters():
+    """In the constructor and for groups that come later; a refused group is not kept."""
+    from nfi import optim
+    a, b = (torch.nn.Parameter(torch.zeros(3, 4)) for _ in range(2))
+    vector = torch.nn.Parameter(torch.zeros(4))
+    with pytest.raises(ValueError, match='two or more dimensions'):
+        optim.Muon([a, vector])
+    with pytest.raises(ValueError, match='twice'), pytest.warns(UserWarning):
+        optim.Muon([a, a])
+    o = optim.Muon([a])
+    with pytest.raises(ValueError, match='two or more dimensions'):
+        o.add_param_group({'params': [vector]})
+    with pytest.raises(ValueError, match='twice'), pytest.warns(UserWarning):
+        o.add_param_group({'params': [b, b]})
+    with pytest.raises(ValueError):
+        o.add_param_group({'params': [a]})
+    assert len(o.param_groups) == 1
+    o.add_param_group({'params': [b], 'lr': 0.5})
+    assert len(o.param_groups) == 2 and o.param_groups[1]['lr'] == 0.5
