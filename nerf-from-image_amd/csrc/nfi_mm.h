@@ -319,7 +319,7 @@ __device__ __forceinline__ void tile_product(const unsigned char* a, unsigned ld
 // A wave's part of a product tile to rows of `out` (ld elements apart; `rows` x `cols` of them from this wave's
 // corner are the matrix's).  A lane holds 4 columns of a row, 32 bytes of a row's line in a 16-bit store: the part is turned in
 // LDS first, where the wave has room for it, and leaves in pieces of 16 bytes, a row's one after the other (32,749 rows of
-// 1024 -> 4096: 410 -> EPI us).
+// 1024 -> 4096 in bf16: 410 -> 365 us).
 template <class O, int NA, int NB>
 __device__ __forceinline__ void store_part(const f4v (&acc)[NA][NB], unsigned char* lds, O* out, int64_t ld, int rows, int cols) {
   constexpr int V = 16 / (int)sizeof(O), PIECES = NB * (int)sizeof(O), AT_ONCE = 64 / PIECES;   // pieces of a row; rows of a store
