@@ -144,6 +144,25 @@ def test_values_and_gradients(case, dtype):
         assert err <= e * float(b.norm()) * (dtype != torch.float32) + (64 + rows / 16) * U * amp * max(total, float(b.norm())) + 1e-30, (name, err, float(b.norm()))
 
 
+MANY = [  # more rows than workgroups, so that each takes several; no kink, whose side the last bit decides
+    (1700, 320, True, 17, 'layer', 'layer', 1.0, True),
+    (1600, 520, True, 1600, 'rms', 'layer', 1.0, True),
+    (2100, 1000, True, 7, 'layer', 'rms', 1.0, True),
+    (1601, 1024, True, 1, 'rms', 'rms', 1.0, True),
+    (1500, 1024, False, 750, 'layer', None, 1.0, True),
+    (1100, 2000, True, 2, 'layer', 'layer', 1.0, True),
+    (600, 4096, True, 4, 'rms', 'rms', 1.0, True),
+    (555, 4100, True, 5, 'layer', 'layer', 1.0, True),
+    (530, 8192, True, 1, 'rms', 'layer', 1.0, True),
+]
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('case', MANY, ids=lambda c: f'{c[0]}x{c[1]}')
+def test_many_rows_of_a_workgroup(case, dtype):
+    test_values_and_gradients(case, dtype)
+
+
 def test_gradient_against_differences():
     """Central differences of the 32-bit outputs' scalar product: step 2^-6, truncation ~ step^2, rounding ~ u / step."""
     p = inputs(6, 40, torch.float32, 3, True, 3)
