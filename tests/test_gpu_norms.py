@@ -229,6 +229,31 @@ def test_parameters_of_groups(rows, groups, width, gate):
     assert torch.equal(some[0], got[keys.index('bias')]) and torch.equal(some[1], got[keys.index('next_weight')])
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('rows,groups,width', [(1600, 800, 1000), (800, 2, 1024), (6, 3, 4096), (260, 260, 5000), (520, 4, 8192), (1600, 4, 320)])
+def test_parameters_of_groups_of_wide_rows(rows, groups, width, dtype):
+    """The same where a row takes a workgroup, beside 16-bit rows too (the parameters 32-bit, their gradients unrounded)."""
+    g = torch.Generator(device=DEV).manual_seed(rows + width)
+
+    def rnd(*shape, shift=0.0, dt=torch.float32):
+        return (torch.randn(shape, device=DEV, generator=g) * 0.3 + shift).to(dt).requires_grad_()
+    p = {'h': rnd(rows, width, dt=dtype), 'residual': rnd(rows, width, dt=dtype), 'gate': rnd(groups, width, shift=1),
+         'weight': rnd(groups, width, shift=1), 'bias': rnd(groups, width), 'next_weight': rnd(groups, width, shift=1),
+         'next_bias': rnd(groups, width)}
+    p64 = {k: v.detach().double().requires_grad_() for k, v in p.items()}
+    spread = {k: (v if k in ('h', 'residual', 'gate') else v.repeat_interleave(rows // groups, 0)) for k, v in p64.items()}
+    x, y = run(p, 'layer', 'rms', 1.0, 0.7)
+    rx, ry = formula(spread, 'layer', 'rms', 1.0, 0.7)
+    near(x.detach(), rx.detach(), dtype, 8)
+    near(y.detach(), ry.detach(), dtype, 32)
+    gx, gy = (torch.randn((rows, width), device=DEV, generator=g).to(dtype) for _ in range(2))
+    got = torch.autograd.grad([x, y], list(p.values()), [gx, gy])
+    ref = torch.autograd.grad([rx, ry], list(p64.values()), [gx.double(), gy.double()])
+    for k, a, b in zip(p, got, ref):
+        e = torch.finfo(a.dtype).eps / 2 if a.dtype != torch.float32 else 0.0
+        assert float((a.double() - b).norm()) <= (e + (64 + rows / 16) * U * 16) * float(b.norm()), k
+
+
 def test_refusals():
     h = torch.zeros((6, 8), device=DEV)
     w = torch.ones((8,), device=DEV)
