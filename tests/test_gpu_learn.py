@@ -115,3 +115,52 @@ def test_inversion_with_orthogonalised_latent_steps(graph):
     cfg.latent_update = 'sgd'
     with pytest.raises(ValueError, match='latent_update'):
         inversion.invert(gen, d['target'], d['cam0'], d['focal0'], d['w_init'], cfg)
+
+
+def test_two_graphs_and_eager_calls_take_turns():
+    """Two captured runs of all three operators (products whose rows are split, a norm with its gradients, an update in
+    tiles), replayed in turn on two streams and between eager calls: each leaves what it left alone."""
+    from nfi import grouped, norms
+
+    def setup(seed):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+
+        def rnd(*shape):
+            return torch.randn(shape, device=DEV, generator=g)
+        x, w, gy = rnd(3001, 200).requires_grad_(), (rnd(3, 136, 200) * 0.1).requires_grad_(), rnd(3001, 136)
+        gate, weight, bias = (rnd(136).requires_grad_() for _ in range(3))
+        offsets = torch.tensor([0, 1200 + seed, 1200 + seed, 2990], device=DEV, dtype=torch.int32)
+
+        def step():
+            h = grouped.grouped_linear(x, w, offsets)
+            y = norms.residual_norm(h, None, gate, weight, bias, slope=0.2)
+            grads = torch.autograd.grad(y, [x, w, gate, weight, bias], gy)
+            return [y.detach(), *grads, optim.orthogonalize(grads[1])]
+        return x, step
+
+    runs = [setup(1), setup(2)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _, step in runs:
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs, held = [], []
+    for _, step in runs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held.append(step())
+        graphs.append(graph)
+    for turn in range(4):
+        with torch.no_grad():
+            for x, _ in runs:
+                x.mul_(0.9)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graphs[turn % 2].replay()
+        graphs[1 - turn % 2].replay()
+        torch.cuda.synchronize()
+        for (_, step), h in zip(runs, held):
+            assert all(torch.equal(a, b) for a, b in zip(h, step()))
+        torch.cuda.synchronize()
