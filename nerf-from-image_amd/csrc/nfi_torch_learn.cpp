@@ -350,6 +350,7 @@ void muon_step(at::TensorList params, at::TensorList grads, at::TensorList momen
   // everything is checked before anything is changed
   std::vector<Tensor> g(n);
   std::vector<int64_t> lot(n);
+  std::vector<char> done(n, 0);
   for (size_t i = 0; i < n; ++i) {
     const Tensor &p = params[i], &m = momenta[i];
     on_device(what, p);
@@ -358,13 +359,16 @@ void muon_step(at::TensorList params, at::TensorList grads, at::TensorList momen
     TORCH_CHECK(p.dim() >= 2 && p.is_contiguous() && !grads[i].is_sparse(), what, ": dense gradients and contiguous parameters are wanted");
     TORCH_CHECK(grads[i].sizes() == p.sizes() && m.sizes() == p.sizes() && m.is_contiguous() && m.scalar_type() == torch::kFloat, what,
                 ": a 32-bit momentum and a gradient of the parameter's shape ", p.sizes(), " are wanted");
-    const int64_t cols = batched ? p.size(-1) : p.numel() / p.size(0), rows = batched ? p.size(-2) : p.size(0);
-    TORCH_CHECK_VALUE(rows <= NFI_ORTHO_MAX_SIDE && cols <= NFI_ORTHO_MAX_SIDE, what, ": sides of 1 to ", NFI_ORTHO_MAX_SIDE, " are wanted, not ",
-                      rows, " x ", cols);
+    if (p.numel() == 0) {   // (nothing to update, and no sizes to divide by)
+      done[i] = 1;
+      continue;
+    }
+    const int64_t cols = batched ? p.size(-1) : p.numel() / p.size(0), rows = batched ? p.size(-2) : p.size(0), count = p.numel() / (rows * cols);
+    TORCH_CHECK_VALUE(rows <= NFI_ORTHO_MAX_SIDE && cols <= NFI_ORTHO_MAX_SIDE && count < (1ll << 31), what, ": sides of 1 to ", NFI_ORTHO_MAX_SIDE,
+                      " are wanted, not ", count, " of ", rows, " x ", cols);
     lot[i] = (p.device().index() * 3 + type_code(p, what)) * 3 + type_code(grads[i], what);
     g[i] = grads[i].contiguous();
   }
-  std::vector<char> done(n, 0);
   for (size_t i = 0; i < n; ++i) {   // one call for each device and pair of types
     if (done[i]) continue;
     std::vector<nfi_ortho_item> items;

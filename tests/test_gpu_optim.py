@@ -267,3 +267,24 @@ def test_two_wide_bf16_matrices_repeat_and_stay_as_near_as_32_bit_products():
     own = optim.orthogonalize(v)
     assert torch.equal(own.bfloat16(), first)
     near(own, v, torch.float32)
+
+
+def step_op(params, grads, momenta, batched=False, lr=0.1):
+    from nfi import torch_ops
+    torch_ops.op('muon_step')(params, grads, momenta, batched, lr, 0.9, 0.0, True, 5, *optim.QUINTIC, 1e-7)
+
+
+def test_the_step_operator_leaves_empty_parameters_alone():
+    """torch.ops.nfi.muon_step, as a C++ or TorchScript caller reaches it: a parameter without values divides nothing, and
+    the others of its call are stepped."""
+    for batched, shapes in ((False, [(0, 3), (3, 0), (0, 0), (4, 0, 3)]), (True, [(2, 0, 4), (0, 3, 4), (2, 3, 0)])):
+        empty = [torch.zeros(s, device=DEV) for s in shapes]
+        step_op(empty, [torch.zeros_like(t) for t in empty], [torch.zeros_like(t) for t in empty], batched)
+        w, g = torch.ones((6, 8), device=DEV), torch.randn((6, 8), device=DEV)
+        m = torch.zeros_like(w)
+        want, want_m = reference_step(w, g, m, 0.1, 0.9, 0.0, True)
+        params = empty[:1] + [w] + empty[1:]
+        step_op(params, [torch.zeros_like(t) if t is not w else g for t in params], [torch.zeros_like(t) if t is not w else m for t in params], batched)
+        # (the update's own error times lr, see above, and W's roundings; M is G itself)
+        assert float((w.double() - want).norm()) <= 0.1 * 341 * 8 * 2.0 ** -22 * 6 ** 0.5 + 4 * 2.0 ** -24 * float(want.norm())
+        assert torch.equal(m, g) and float((m.double() - want_m).abs().max()) == 0
