@@ -99,7 +99,7 @@ typedef struct nfi_ortho_item {
  * rows <= cols (else of the transposed matrix);  then w = X, or with update w <- (1 - decay) w - step
  * scale X.  Products are held to 32-bit accuracy for every type, and the result is rounded once.  `items` is
  * host memory, read during the call.  A polynomial under which singular values leave [0, 64) is refused.
- * work: nfi_ortho_work_bytes, or NULL where that is 0. */
+ * work: nfi_ortho_work_bytes (-1 for items that nfi_ortho refuses by their sizes), or NULL where that is 0. */
 typedef struct nfi_ortho_args {
   const nfi_ortho_item* items;
   void* work;

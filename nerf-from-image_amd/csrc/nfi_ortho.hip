@@ -1040,19 +1040,25 @@ static void bounds(double a, double b, double c, double top, double& x, double& 
   at(-a / (3. * b));
 }
 
+static int check_items(const nfi_ortho_item* items, int n_items) {
+  for (int i = 0; i < n_items; ++i) {
+    const nfi_ortho_item& s = items[i];
+    NFI_REQUIRE(s.rows > 0 && s.cols > 0 && s.count > 0 && s.rows <= NFI_ORTHO_MAX_SIDE && s.cols <= NFI_ORTHO_MAX_SIDE,
+                "ortho: matrix %d is %d x %d x %d (sides 1 .. %d)", i, s.count, s.rows, s.cols, NFI_ORTHO_MAX_SIDE);
+    const int64_t tr = (s.rows + TILE - 1) / TILE, tc = (s.cols + TILE - 1) / TILE;
+    NFI_REQUIRE(4 * tr * tc * s.count < (1ll << 26), "ortho: matrix %d is too large", i);
+  }
+  return NFI_OK;
+}
+
 static int check(const nfi_ortho_args* p, double& most_x, double& most_q) {
   NFI_REQUIRE(p && p->items && p->n_items > 0, "ortho: no matrices");
   NFI_REQUIRE(type_ok(p->g_type) && type_ok(p->w_type), "ortho: bad type");
   NFI_REQUIRE(p->steps >= 1 && p->steps <= 64, "ortho: %d steps (1 .. 64)", p->steps);
   NFI_REQUIRE(p->eps > 0.f && std::isfinite(p->eps), "ortho: eps %g", (double)p->eps);
-  for (int i = 0; i < p->n_items; ++i) {
-    const nfi_ortho_item& s = p->items[i];
-    NFI_REQUIRE(s.rows > 0 && s.cols > 0 && s.count > 0 && s.rows <= NFI_ORTHO_MAX_SIDE && s.cols <= NFI_ORTHO_MAX_SIDE,
-                "ortho: matrix %d is %d x %d x %d (sides 1 .. %d)", i, s.count, s.rows, s.cols, NFI_ORTHO_MAX_SIDE);
-    const int64_t tr = (s.rows + TILE - 1) / TILE, tc = (s.cols + TILE - 1) / TILE;
-    NFI_REQUIRE(4 * tr * tc * s.count < (1ll << 26), "ortho: matrix %d is too large", i);
-    NFI_REQUIRE(s.g && s.w, "ortho: null tensor");
-  }
+  const int e = check_items(p->items, p->n_items);
+  if (e) return e;
+  for (int i = 0; i < p->n_items; ++i) NFI_REQUIRE(p->items[i].g && p->items[i].w, "ortho: null tensor");
   // the iterates stay bounded under this polynomial
   double top = 1., x, q;
   most_x = 1.;
@@ -1078,6 +1084,7 @@ using namespace nfi::learn;
 extern "C" {
 
 int64_t nfi_ortho_work_bytes(const nfi_ortho_item* items, int32_t n_items) {
+  if (check_items(items, n_items) != NFI_OK) return -1;
   int64_t most = 0, sum = 0;
   int held = 0;
   Item table[ITEMS];

@@ -298,13 +298,18 @@ Tensor grouped_linear(const Tensor& x, const Tensor& w, const Tensor& offsets, c
 
 // ---- orthogonalised updates ------------------------------------------------------------------------------------------
 
-void ortho(const std::vector<nfi_ortho_item>& items, nfi_ortho_args a, const Tensor& like) {
+int64_t ortho_bytes(const std::vector<nfi_ortho_item>& items) {
+  const int64_t n = nfi_ortho_work_bytes(items.data(), (int32_t)items.size());
+  if (n < 0) check(-1, "nfi_ortho_work_bytes");
+  return n;
+}
+
+void ortho(const std::vector<nfi_ortho_item>& items, nfi_ortho_args a, const Tensor& work, void* stream) {
   a.items = items.data();
   a.n_items = (int32_t)items.size();
-  a.work_bytes = nfi_ortho_work_bytes(a.items, a.n_items);
-  const Tensor work = bytes(a.work_bytes, like);
   a.work = ptr(work);
-  check(nfi_ortho(&a, stream_of(like)), "nfi_ortho");
+  a.work_bytes = work.defined() ? work.numel() : 0;
+  check(nfi_ortho(&a, stream), "nfi_ortho");
 }
 
 Tensor orthogonalize(const Tensor& u, int64_t steps, double ca, double cb, double cc, double eps) {
@@ -327,7 +332,7 @@ Tensor orthogonalize(const Tensor& u, int64_t steps, double ca, double cb, doubl
   a.eps = (float)eps;
   std::vector<nfi_ortho_item> items(1);
   items[0] = {src.data_ptr(), nullptr, out.data_ptr(), (int32_t)rows, (int32_t)cols, (int32_t)count, 1.f};
-  ortho(items, a, u);
+  ortho(items, a, bytes(ortho_bytes(items), u), stream_of(u));
   return out;
 }
 
@@ -347,10 +352,16 @@ void muon_step(at::TensorList params, at::TensorList grads, at::TensorList momen
   a.b = (float)cb;
   a.c = (float)cc;
   a.eps = (float)eps;
-  // everything is checked before anything is changed
+  // everything is checked, and every buffer is had, before anything is changed: one call for each device and pair of types (a
+  // polynomial that is refused is the same for all of them, and the first call says so)
+  struct Lot {
+    int64_t kind;
+    std::vector<nfi_ortho_item> items;
+    std::vector<size_t> of;
+    Tensor work;
+  };
   std::vector<Tensor> g(n);
-  std::vector<int64_t> lot(n);
-  std::vector<char> done(n, 0);
+  std::vector<Lot> lots;
   for (size_t i = 0; i < n; ++i) {
     const Tensor &p = params[i], &m = momenta[i];
     on_device(what, p);
@@ -359,35 +370,34 @@ void muon_step(at::TensorList params, at::TensorList grads, at::TensorList momen
     TORCH_CHECK(p.dim() >= 2 && p.is_contiguous() && !grads[i].is_sparse(), what, ": dense gradients and contiguous parameters are wanted");
     TORCH_CHECK(grads[i].sizes() == p.sizes() && m.sizes() == p.sizes() && m.is_contiguous() && m.scalar_type() == torch::kFloat, what,
                 ": a 32-bit momentum and a gradient of the parameter's shape ", p.sizes(), " are wanted");
-    if (p.numel() == 0) {   // (nothing to update, and no sizes to divide by)
-      done[i] = 1;
-      continue;
-    }
+    const int64_t kind = (p.device().index() * 3 + type_code(p, what)) * 3 + type_code(grads[i], what);
+    if (p.numel() == 0) continue;   // (nothing to update, and no sizes to divide by)
     const int64_t cols = batched ? p.size(-1) : p.numel() / p.size(0), rows = batched ? p.size(-2) : p.size(0), count = p.numel() / (rows * cols);
     TORCH_CHECK_VALUE(rows <= NFI_ORTHO_MAX_SIDE && cols <= NFI_ORTHO_MAX_SIDE && count < (1ll << 31), what, ": sides of 1 to ", NFI_ORTHO_MAX_SIDE,
                       " are wanted, not ", count, " of ", rows, " x ", cols);
-    lot[i] = (p.device().index() * 3 + type_code(p, what)) * 3 + type_code(grads[i], what);
     g[i] = grads[i].contiguous();
+    size_t l = 0;
+    while (l < lots.size() && lots[l].kind != kind) ++l;
+    if (l == lots.size()) lots.push_back({kind, {}, {}, Tensor()});
+    lots[l].items.push_back({g[i].data_ptr(), m.data_ptr(), p.data_ptr(), (int32_t)rows, (int32_t)cols, (int32_t)count,
+                             (float)std::sqrt(std::max(1.0, (double)rows / (double)cols))});
+    lots[l].of.push_back(i);
   }
-  for (size_t i = 0; i < n; ++i) {   // one call for each device and pair of types
-    if (done[i]) continue;
-    std::vector<nfi_ortho_item> items;
-    items.reserve(n - i);
-    for (size_t j = i; j < n; ++j) {
-      if (done[j] || lot[j] != lot[i]) continue;
-      done[j] = 1;
-      const Tensor& p = params[j];
-      const int64_t rows = batched ? p.size(-2) : p.size(0), cols = batched ? p.size(-1) : p.numel() / p.size(0);
-      items.push_back({g[j].data_ptr(), momenta[j].data_ptr(), p.data_ptr(), (int32_t)rows, (int32_t)cols, (int32_t)(p.numel() / (rows * cols)),
-                       (float)std::sqrt(std::max(1.0, (double)rows / (double)cols))});
-      // what is cached by a tensor's version is out of date
-      p.unsafeGetTensorImpl()->bump_version();
-      momenta[j].unsafeGetTensorImpl()->bump_version();
+  for (Lot& l : lots) {
+    const Tensor& p = params[l.of[0]];
+    const c10::DeviceGuard guard(p.device());
+    l.work = bytes(ortho_bytes(l.items), p);
+  }
+  for (Lot& l : lots) {
+    const Tensor& p = params[l.of[0]];
+    const c10::DeviceGuard guard(p.device());
+    a.w_type = type_code(p, what);
+    a.g_type = type_code(g[l.of[0]], what);
+    ortho(l.items, a, l.work, stream_of(p));
+    for (size_t i : l.of) {   // what is cached by a tensor's version is out of date
+      params[i].unsafeGetTensorImpl()->bump_version();
+      momenta[i].unsafeGetTensorImpl()->bump_version();
     }
-    const c10::DeviceGuard guard(params[i].device());
-    a.w_type = type_code(params[i], what);
-    a.g_type = type_code(g[i], what);
-    ortho(items, a, params[i]);
   }
 }
 

@@ -288,3 +288,22 @@ def test_the_step_operator_leaves_empty_parameters_alone():
         # (the update's own error times lr, see above, and W's roundings; M is G itself)
         assert float((w.double() - want).norm()) <= 0.1 * 341 * 8 * 2.0 ** -22 * 6 ** 0.5 + 4 * 2.0 ** -24 * float(want.norm())
         assert torch.equal(m, g) and float((m.double() - want_m).abs().max()) == 0
+
+
+def test_a_refused_matrix_stops_the_step_before_anything_changes():
+    """One call steps the 32-bit parameters, another the 16-bit ones: a matrix that the second refuses leaves the first's
+    weights, momenta and versions as they were, and so does a polynomial."""
+    def tensors(dtype, *shape):
+        return torch.ones(shape, device=DEV, dtype=dtype), torch.ones(shape, device=DEV, dtype=dtype), torch.zeros(shape, device=DEV)
+    w, g, m = tensors(torch.float32, 6, 8)
+    # 2^24 matrices of one value: too many for a call
+    many, many_g, many_m = tensors(torch.bfloat16, 1 << 24, 1, 1)
+    bw, bg, bm = w[None], g[None], m[None]
+    versions = w._version, m._version
+    with pytest.raises(RuntimeError, match='too large'):
+        step_op([bw, many], [bg, many_g], [bm, many_m], batched=True)
+    from nfi import torch_ops
+    with pytest.raises(RuntimeError, match='polynomial'):
+        torch_ops.op('muon_step')([w, many[:3, 0]], [g, many_g[:3, 0]], [m, many_m[:3, 0]], False, 0.1, 0.9, 0.0, True, 5, 9.0, 9.0, 9.0, 1e-7)
+    assert torch.equal(w, torch.ones_like(w)) and float(m.abs().max()) == 0 and (w._version, m._version) == versions
+    assert float((many - 1).abs().max()) == 0 and float(many_m.abs().max()) == 0

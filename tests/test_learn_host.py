@@ -172,3 +172,13 @@ def test_muon_refuses_vectors_and_repeated_parameters():
     assert len(o.param_groups) == 1
     o.add_param_group({'params': [b], 'lr': 0.5})
     assert len(o.param_groups) == 2 and o.param_groups[1]['lr'] == 0.5
+
+
+def test_ortho_work_refuses_what_the_call_refuses():
+    """A caller of several calls in a row can size them all, and hears of a refused matrix, before the first one runs."""
+    lib = _lib.load()
+    for shape, word in (((0, 4, 1), b'sides'), ((4, 262145, 1), b'sides'), ((4, 4, 0), b'sides'), ((4, 4, 1 << 24), b'too large'),
+                        ((262144, 262144, 4), b'too large')):
+        arr = (_lib.NfiOrthoItem * 2)(_lib.NfiOrthoItem(16, None, 16, 200, 300, 1, 1.0), _lib.NfiOrthoItem(16, None, 16, *shape, 1.0))
+        assert lib.nfi_ortho_work_bytes(arr, 2) == -1 and word in lib.nfi_last_error(), shape
+    assert lib.nfi_ortho_work_bytes(arr, 1) > 0
