@@ -55,7 +55,8 @@ class Muon(torch.optim.Optimizer):
 
     M (state 'momentum_buffer') is 32-bit for every type of parameter; gradients and parameters are float32, bfloat16 or
     float16, contiguous.  All matrices of a group of equal types go through one call; lr and the other numbers are read
-    when step() is called (a captured graph keeps those of its capture)."""
+    when step() is called (a captured graph keeps those of its capture).  The first step of a parameter makes its momentum, and
+    is refused in a capture, where every replay would make it anew: take one step before."""
 
     def __init__(self, params: Iterable, lr: float = 0.02, momentum: float = 0.95, weight_decay: float = 0.0, nesterov: bool = True,
                  steps: int = 5, coefficients: Sequence[float] = QUINTIC, eps: float = 1e-7, batched: bool = False):
@@ -84,23 +85,28 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        op = _op('muon_step')
+        calls = []
         for group in self.param_groups:
             params, grads, momenta = [], [], []
             for p in group['params']:
                 g = p.grad
                 if g is None or p.numel() == 0:
                     continue
-                state = self.state[p]
-                m = state.get('momentum_buffer')
+                m = self.state[p].get('momentum_buffer') if p in self.state else None
                 if m is None:
-                    m = state['momentum_buffer'] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError('Muon: the first step of a parameter makes its momentum, and in a graph every replay would '
+                                           'clear it again: take one step before the capture')
+                    m = self.state[p]['momentum_buffer'] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
                 params.append(p)
                 grads.append(g)
                 momenta.append(m)
             if params:
-                op(params, grads, momenta, group['batched'], group['lr'], group['momentum'], group['weight_decay'], group['nesterov'],
-                   group['steps'], *group['coefficients'], group['eps'])
+                calls.append((group, params, grads, momenta))
+        op = _op('muon_step')
+        for group, params, grads, momenta in calls:
+            op(params, grads, momenta, group['batched'], group['lr'], group['momentum'], group['weight_decay'], group['nesterov'],
+               group['steps'], *group['coefficients'], group['eps'])
         return loss
 
     def load_state_dict(self, state_dict):

@@ -307,3 +307,31 @@ def test_a_refused_matrix_stops_the_step_before_anything_changes():
         torch_ops.op('muon_step')([w, many[:3, 0]], [g, many_g[:3, 0]], [m, many_m[:3, 0]], False, 0.1, 0.9, 0.0, True, 5, 9.0, 9.0, 9.0, 1e-7)
     assert torch.equal(w, torch.ones_like(w)) and float(m.abs().max()) == 0 and (w._version, m._version) == versions
     assert float((many - 1).abs().max()) == 0 and float(many_m.abs().max()) == 0
+
+
+def test_the_first_step_is_refused_in_a_capture():
+    """And taken eagerly behind it, from where the parameter was; then the capture works."""
+    p = torch.nn.Parameter(torch.ones((20, 30), device=DEV))
+    p.grad = torch.randn((20, 30), device=DEV)
+    opt = optim.Muon([p], lr=0.1)
+    optim.orthogonalize(p.grad)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match='before the capture'):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    torch.cuda.synchronize()
+    assert torch.equal(p.detach(), torch.ones_like(p)) and 'momentum_buffer' not in opt.state.get(p, {})
+    opt.step()
+    q = torch.nn.Parameter(p.detach().clone())
+    q.grad = p.grad
+    other = optim.Muon([q], lr=0.1)
+    other.load_state_dict(copy.deepcopy(opt.state_dict()))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        other.step()
+        assert torch.equal(p, q)

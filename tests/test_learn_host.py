@@ -182,3 +182,24 @@ def test_ortho_work_refuses_what_the_call_refuses():
         arr = (_lib.NfiOrthoItem * 2)(_lib.NfiOrthoItem(16, None, 16, 200, 300, 1, 1.0), _lib.NfiOrthoItem(16, None, 16, *shape, 1.0))
         assert lib.nfi_ortho_work_bytes(arr, 2) == -1 and word in lib.nfi_last_error(), shape
     assert lib.nfi_ortho_work_bytes(arr, 1) > 0
+
+
+def test_muon_refuses_a_first_step_in_a_capture(monkeypatch):
+    """Before any parameter is stepped, those of earlier groups too, and without leaving a momentum behind."""
+    a, b = (torch.nn.Parameter(torch.ones(3, 4)) for _ in range(2))
+    o = optim.Muon([{'params': [a]}, {'params': [b]}])
+    o.state[a]['momentum_buffer'] = torch.zeros(3, 4)
+    a.grad, b.grad = torch.ones(3, 4), torch.ones(3, 4)
+    stepped = []
+    monkeypatch.setattr(optim, '_op', lambda name: lambda params, *rest: stepped.extend(params))
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+    with pytest.raises(RuntimeError, match='before the capture'):
+        o.step()
+    assert not stepped and 'momentum_buffer' not in o.state.get(b, {})
+    b.grad = None
+    o.step()                     # (a parameter without a gradient has no part in it)
+    assert stepped == [a]
+    b.grad = torch.ones(3, 4)
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: False)
+    o.step()
+    assert stepped == [a, a, b] and float(o.state[b]['momentum_buffer'].abs().max()) == 0
