@@ -89,15 +89,18 @@ class ViewDirectionMapperBank(torch.nn.Module):
                              eps=layers[0].eps)
 
     def forward(self, viewdir: torch.Tensor, mapper_of_image: torch.Tensor) -> torch.Tensor:
-        """viewdir [images, rays, 3], mapper_of_image [images] int64 on the device, not decreasing -> [images, rays, 32]."""
+        """viewdir [images, rays, 3], mapper_of_image [images] int64 on the device, in any order -> [images, rays, 32]."""
         images, rays = viewdir.shape[:2]
         if mapper_of_image.shape != (images,) or mapper_of_image.dtype != torch.int64:
             raise ValueError(f'mapper_of_image [{images}] int64 is wanted, not {tuple(mapper_of_image.shape)} {mapper_of_image.dtype}')
+        # the products want a mapper's rows side by side: the images are brought into their mappers' order, and back
+        image, order = torch.sort(mapper_of_image, stable=True)
         ends = torch.arange(len(self.mappers) + 1, device=viewdir.device)
-        offsets = torch.searchsorted(mapper_of_image.contiguous(), ends) * rays
-        x = F.leaky_relu(self._linear('fc0', viewdir.reshape(images * rays, 3), offsets), 0.2)
+        offsets = torch.searchsorted(image, ends) * rays
+        x = F.leaky_relu(self._linear('fc0', viewdir.index_select(0, order).reshape(images * rays, 3), offsets), 0.2)
         for a, b in ((1, 2), (3, 4)):
-            h = self._norm(f'norm{a}', self._linear(f'fc{a}', x, offsets), mapper_of_image)
-            x = self._norm(f'norm{b}', self._linear(f'fc{b}', h, offsets), mapper_of_image, shortcut=x)
+            h = self._norm(f'norm{a}', self._linear(f'fc{a}', x, offsets), image)
+            x = self._norm(f'norm{b}', self._linear(f'fc{b}', h, offsets), image, shortcut=x)
         x = F.leaky_relu(self._linear('fc5', x, offsets), 0.2)
-        return self._linear('fc6', x, offsets).view(images, rays, -1)
+        x = self._linear('fc6', x, offsets).view(images, rays, -1)
+        return x.index_select(0, torch.argsort(order))

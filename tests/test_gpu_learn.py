@@ -164,3 +164,26 @@ def test_two_graphs_and_eager_calls_take_turns():
         for (_, step), h in zip(runs, held):
             assert all(torch.equal(a, b) for a, b in zip(h, step()))
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize('which', [[1, 0, 1], [3, 0, 2, 0, 1]])
+def test_bank_takes_images_in_any_order(which):
+    """Each image's rows and gradients are those of the same images in their mappers' order, bit for bit (a row's sums
+    do not depend on its place; the weights' gradients are summed over the same rows in the same order)."""
+    b = bank(4)
+    v = torch.nn.functional.normalize(torch.randn((len(which), 70, 3), device=DEV), dim=-1)
+    g = torch.randn((len(which), 70, 32), device=DEV)
+    image = torch.tensor(which, device=DEV)
+    order = torch.tensor(sorted(range(len(which)), key=lambda i: which[i]), device=DEV)
+    params = [p for k, p in b.named_parameters() if 'output' not in k]
+    results = []
+    for pick in (slice(None), order):
+        leaf = v[pick].clone().requires_grad_()
+        x = b(leaf, image[pick])
+        results.append([x.detach(), *torch.autograd.grad(x, [leaf] + params, g[pick])])
+    (x, gv, *gp), (xs, gvs, *gps) = results
+    assert torch.equal(x[order], xs) and torch.equal(gv[order], gvs)
+    assert all(torch.equal(p, q) for p, q in zip(gp, gps))
+    for i, m in enumerate(which):
+        ref = viewdir_trunk(copy.deepcopy(b.mappers[m]).double(), v[i].double().unsqueeze(-2)).squeeze(-2)
+        assert float((x[i].double() - ref).abs().max()) <= 2 ** 9 * U * max(1.0, float(ref.abs().max())), i

@@ -203,3 +203,42 @@ def test_muon_refuses_a_first_step_in_a_capture(monkeypatch):
     monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: False)
     o.step()
     assert stepped == [a, a, b] and float(o.state[b]['momentum_buffer'].abs().max()) == 0
+
+
+@pytest.fixture
+def plain_bank(monkeypatch):
+    """A bank of three mappers on the CPU, its two operators in torch."""
+    from nfi import viewdir
+
+    def linear(x, weight, offsets, bias=None):
+        y = x.new_zeros((x.shape[0], weight.shape[1]))
+        for e in range(weight.shape[0]):
+            r = slice(int(offsets[e]), int(offsets[e + 1]))
+            y[r] = x[r] @ weight[e].t() + (0 if bias is None else bias[e])
+        return y
+
+    def norm(h, residual, gate, weight, bias, *, slope, scale, eps):
+        assert weight.shape[0] >= 1
+        n = torch.nn.functional.layer_norm(h, h.shape[-1:], eps=eps).view(weight.shape[0], -1, h.shape[-1])
+        u = torch.nn.functional.leaky_relu(n * weight[:, None] + bias[:, None], slope).view(h.shape)
+        return scale * (u + (0 if residual is None else residual))
+
+    monkeypatch.setattr(viewdir, 'grouped_linear', linear)
+    monkeypatch.setattr(viewdir, 'residual_norm', norm)
+    torch.manual_seed(0)
+    mappers = [viewdir.ViewDirectionMapper(10) for _ in range(3)]
+    for m in mappers:
+        for k in range(1, 5):
+            with torch.no_grad():
+                getattr(m, f'norm{k}').weight.add_(torch.randn(64) * 0.1)
+                getattr(m, f'norm{k}').bias.add_(torch.randn(64) * 0.1)
+    return viewdir.ViewDirectionMapperBank(mappers)
+
+
+@pytest.mark.parametrize('which', [[0, 1, 2], [1, 0, 1], [2, 2, 0, 1], [1]])
+def test_bank_gives_each_image_its_own_mapper(plain_bank, which):
+    from nfi.viewdir import viewdir_trunk
+    v = torch.nn.functional.normalize(torch.randn((len(which), 5, 3)), dim=-1)
+    x = plain_bank(v, torch.tensor(which))
+    for i, m in enumerate(which):
+        torch.testing.assert_close(x[i], viewdir_trunk(plain_bank.mappers[m], v[i].unsqueeze(-2)).squeeze(-2), rtol=1e-5, atol=1e-5)
