@@ -89,7 +89,8 @@ class ViewDirectionMapperBank(torch.nn.Module):
                              eps=layers[0].eps)
 
     def forward(self, viewdir: torch.Tensor, mapper_of_image: torch.Tensor) -> torch.Tensor:
-        """viewdir [images, rays, 3], mapper_of_image [images] int64 on the device, in any order -> [images, rays, 32]."""
+        """viewdir [images, rays, 3], mapper_of_image [images] int64 on the device, in any order -> [images, rays, 32]; zeros,
+        and no gradients, for an image whose number is none of a mapper (it is not read on the host)."""
         images, rays = viewdir.shape[:2]
         if mapper_of_image.shape != (images,) or mapper_of_image.dtype != torch.int64:
             raise ValueError(f'mapper_of_image [{images}] int64 is wanted, not {tuple(mapper_of_image.shape)} {mapper_of_image.dtype}')
@@ -97,6 +98,7 @@ class ViewDirectionMapperBank(torch.nn.Module):
         image, order = torch.sort(mapper_of_image, stable=True)
         ends = torch.arange(len(self.mappers) + 1, device=viewdir.device)
         offsets = torch.searchsorted(image, ends) * rays
+        image = image.clamp(0, len(self.mappers) - 1)   # (the products leave such images' rows out)
         x = F.leaky_relu(self._linear('fc0', viewdir.index_select(0, order).reshape(images * rays, 3), offsets), 0.2)
         for a, b in ((1, 2), (3, 4)):
             h = self._norm(f'norm{a}', self._linear(f'fc{a}', x, offsets), image)

@@ -187,3 +187,21 @@ def test_bank_takes_images_in_any_order(which):
     for i, m in enumerate(which):
         ref = viewdir_trunk(copy.deepcopy(b.mappers[m]).double(), v[i].double().unsqueeze(-2)).squeeze(-2)
         assert float((x[i].double() - ref).abs().max()) <= 2 ** 9 * U * max(1.0, float(ref.abs().max())), i
+
+
+def test_bank_leaves_out_images_of_no_mapper():
+    """They give zeros and no gradients; the others, and every parameter's gradient, are what they are without them."""
+    b = bank(3)
+    v = torch.nn.functional.normalize(torch.randn((5, 40, 3), device=DEV), dim=-1)
+    g = torch.randn((5, 40, 32), device=DEV)
+    which = torch.tensor([2, -1, 0, 3, 2], device=DEV)
+    keep = torch.tensor([0, 2, 4], device=DEV)
+    params = [p for k, p in b.named_parameters() if 'output' not in k]
+    leaf, alone = v.clone().requires_grad_(), v[keep].clone().requires_grad_()
+    x, y = b(leaf, which), b(alone, which[keep])
+    gv, *gp = torch.autograd.grad(x, [leaf] + params, g)
+    gw, *gq = torch.autograd.grad(y, [alone] + params, g[keep])
+    assert torch.equal(x[keep], y) and torch.equal(gv[keep], gw)
+    assert float(x[[1, 3]].detach().abs().max()) == 0 and float(gv[[1, 3]].abs().max()) == 0
+    # (sums over the same rows; zeros of the rows left out may stand between them)
+    assert all(float((p - q).abs().max()) <= 2 ** 8 * U * float(q.abs().max()) + 1e-12 for p, q in zip(gp, gq))

@@ -242,3 +242,13 @@ def test_bank_gives_each_image_its_own_mapper(plain_bank, which):
     x = plain_bank(v, torch.tensor(which))
     for i, m in enumerate(which):
         torch.testing.assert_close(x[i], viewdir_trunk(plain_bank.mappers[m], v[i].unsqueeze(-2)).squeeze(-2), rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize('which', [[3, 1, 0], [-1, 2, -5], [7]])
+def test_bank_leaves_out_images_of_no_mapper(plain_bank, which):
+    from nfi.viewdir import viewdir_trunk
+    v = torch.nn.functional.normalize(torch.randn((len(which), 5, 3)), dim=-1)
+    x = plain_bank(v, torch.tensor(which))
+    for i, m in enumerate(which):
+        want = viewdir_trunk(plain_bank.mappers[m], v[i].unsqueeze(-2)).squeeze(-2) if 0 <= m < 3 else torch.zeros(5, 32)
+        torch.testing.assert_close(x[i], want, rtol=1e-5, atol=1e-5)
