@@ -70,11 +70,35 @@ class ViewDirectionMapperBank(torch.nn.Module):
     """Several mappers' trunks over one batch of rays: image b's rays go through mapper `mapper_of_image[b]` (a batch that
     mixes categories, each with a mapper of its own).  The layers are viewdir_trunk's, all mappers in each launch: grouped
     products (nfi.grouped) and one fused norm, activation and shortcut for each (nfi.norms), the norms' weights taken image
-    by image.  Gradients reach the mappers' own parameters and viewdir."""
+    by image.  Gradients reach the mappers' own parameters and viewdir.  The mappers are alike but for their parameters' values:
+    others are refused."""
 
     def __init__(self, mappers):
         super().__init__()
         self.mappers = torch.nn.ModuleList(mappers)
+        if len(self.mappers) == 0:
+            raise ValueError('ViewDirectionMapperBank: no mappers')
+        first = self._form(self.mappers[0])
+        for i, m in enumerate(self.mappers):
+            if self._form(m) != first:
+                a, b = next((x, y) for x, y in zip(self._form(m), first) if x != y)
+                raise ValueError(f'ViewDirectionMapperBank: mapper {i} differs from the first, {a} from {b}')
+
+    @staticmethod
+    def _form(mapper):
+        """What all mappers of a bank share: shapes, gains, and the norms' and the activation's constants."""
+        form = [('relu', type(mapper.relu).__name__, getattr(mapper.relu, 'negative_slope', None))]
+        for name in (f'fc{i}' for i in range(7)):
+            m = getattr(mapper, name)
+            form.append((name, tuple(m.weight.shape), m.weight_gain, m.bias is None or m.bias_gain))
+        for name in (f'norm{i}' for i in range(1, 5)):
+            m = getattr(mapper, name)
+            if m.weight is None or m.bias is None:
+                raise ValueError(f'ViewDirectionMapperBank: {name} has no weight or no bias')
+            form.append((name, tuple(m.weight.shape), m.eps))
+        if form[0] != ('relu', 'LeakyReLU', 0.2):
+            raise ValueError(f'ViewDirectionMapperBank: LeakyReLU(0.2) is wanted, not {mapper.relu}')
+        return form
 
     def _linear(self, name, x, offsets):
         layers = [getattr(m, name) for m in self.mappers]

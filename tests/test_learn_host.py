@@ -252,3 +252,24 @@ def test_bank_leaves_out_images_of_no_mapper(plain_bank, which):
     for i, m in enumerate(which):
         want = viewdir_trunk(plain_bank.mappers[m], v[i].unsqueeze(-2)).squeeze(-2) if 0 <= m < 3 else torch.zeros(5, 32)
         torch.testing.assert_close(x[i], want, rtol=1e-5, atol=1e-5)
+
+
+def test_bank_refuses_mappers_that_differ():
+    """In a gain, a bias, a norm's eps, a slope or a width: one launch takes the first mapper's for all."""
+    from nfi.viewdir import ViewDirectionMapper, ViewDirectionMapperBank
+
+    def change(f):
+        m = ViewDirectionMapper(10)
+        f(m)
+        return m
+
+    for f, word in ((lambda m: setattr(m.fc2, 'weight_gain', 0.5), 'fc2'), (lambda m: setattr(m.fc5, 'bias_gain', 0.5), 'fc5'),
+                    (lambda m: setattr(m.fc0, 'bias', None), 'fc0'), (lambda m: setattr(m.norm3, 'eps', 1e-6), 'norm3'),
+                    (lambda m: setattr(m.relu, 'negative_slope', 0.1), 'LeakyReLU'),
+                    (lambda m: setattr(m, 'relu', torch.nn.ReLU()), 'LeakyReLU'), (lambda m: setattr(m.norm1, 'bias', None), 'norm1'),
+                    (lambda m: setattr(m, 'fc6', type(m.fc6)(64, 16)), 'fc6')):
+        with pytest.raises(ValueError, match=word):
+            ViewDirectionMapperBank([ViewDirectionMapper(10), change(f)])
+    with pytest.raises(ValueError, match='no mappers'):
+        ViewDirectionMapperBank([])
+    ViewDirectionMapperBank([ViewDirectionMapper(10), ViewDirectionMapper(4)])   # (the output layers are not the bank's)
