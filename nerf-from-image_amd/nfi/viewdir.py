@@ -90,7 +90,7 @@ class ViewDirectionMapperBank(torch.nn.Module):
         form = [('relu', type(mapper.relu).__name__, getattr(mapper.relu, 'negative_slope', None))]
         for name in (f'fc{i}' for i in range(7)):
             m = getattr(mapper, name)
-            form.append((name, tuple(m.weight.shape), m.weight_gain, m.bias is None or m.bias_gain))
+            form.append((name, tuple(m.weight.shape), m.weight_gain, None if m.bias is None else m.bias_gain))
         for name in (f'norm{i}' for i in range(1, 5)):
             m = getattr(mapper, name)
             if m.weight is None or m.bias is None:
