@@ -118,6 +118,8 @@ class ViewDirectionMapperBank(torch.nn.Module):
         images, rays = viewdir.shape[:2]
         if mapper_of_image.shape != (images,) or mapper_of_image.dtype != torch.int64:
             raise ValueError(f'mapper_of_image [{images}] int64 is wanted, not {tuple(mapper_of_image.shape)} {mapper_of_image.dtype}')
+        if images * rays == 0:   # (an empty result with its graph: rows of groups are at least one)
+            return viewdir_trunk(self.mappers[0], viewdir.unsqueeze(-2)).squeeze(-2)
         # the products want a mapper's rows side by side: the images are brought into their mappers' order, and back
         image, order = torch.sort(mapper_of_image, stable=True)
         ends = torch.arange(len(self.mappers) + 1, device=viewdir.device)

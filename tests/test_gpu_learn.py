@@ -205,3 +205,13 @@ def test_bank_leaves_out_images_of_no_mapper():
     assert float(x[[1, 3]].detach().abs().max()) == 0 and float(gv[[1, 3]].abs().max()) == 0
     # (sums over the same rows; zeros of the rows left out may stand between them)
     assert all(float((p - q).abs().max()) <= 2 ** 8 * U * float(q.abs().max()) + 1e-12 for p, q in zip(gp, gq))
+
+
+@pytest.mark.parametrize('images,rays', [(0, 5), (3, 0)])
+def test_bank_of_an_empty_batch(images, rays):
+    b = bank(2)
+    v = torch.zeros((images, rays, 3), device=DEV, requires_grad=True)
+    x = b(v, torch.zeros((images,), device=DEV, dtype=torch.int64))
+    assert x.shape == (images, rays, 32)
+    gv, gw = torch.autograd.grad(x.sum(), [v, b.mappers[0].fc1.weight])
+    assert gv.shape == v.shape and float(gw.abs().max()) == 0

@@ -273,3 +273,12 @@ def test_bank_refuses_mappers_that_differ():
     with pytest.raises(ValueError, match='no mappers'):
         ViewDirectionMapperBank([])
     ViewDirectionMapperBank([ViewDirectionMapper(10), ViewDirectionMapper(4)])   # (the output layers are not the bank's)
+
+
+@pytest.mark.parametrize('images,rays', [(0, 5), (3, 0), (0, 0)])
+def test_bank_of_an_empty_batch(plain_bank, images, rays):
+    v = torch.zeros((images, rays, 3), requires_grad=True)
+    x = plain_bank(v, torch.zeros((images,), dtype=torch.int64))
+    assert x.shape == (images, rays, 32)
+    gv, gw = torch.autograd.grad(x.sum(), [v, plain_bank.mappers[0].fc1.weight])
+    assert gv.shape == v.shape and float(gw.abs().max()) == 0
