@@ -85,27 +85,45 @@ __global__ void __launch_bounds__(256, 2) grouped_rows(const GroupedArgs p) {
   const int e = find_tile(p, tile, r0, r1);
   if (e < 0) return;
   const int rows = (int)(r1 - r0), cols = min(LB, p.n - c0);
-  Accumulate<T, S::NA, S::NB, false> out;
-  out.clear();
-  if (e < p.groups) {
-    const unsigned char* b = p.b + e * p.sb + (SLAB_B ? (int64_t)c0 * (int)sizeof(T) : (int64_t)c0 * p.ldb);
-    tile_product<T, false, SLAB_B, TILE, LB>(p.a + r0 * p.lda, p.lda, rows, b, p.ldb, cols, p.k, s0, s1, out, false);
-  }
+  const unsigned char* b = p.b + min(e, p.groups - 1) * p.sb + (SLAB_B ? (int64_t)c0 * (int)sizeof(T) : (int64_t)c0 * p.ldb);
   const int line_a = S::line_a(), line_b = S::line_b();
-  if constexpr (!SLAB_B) {
-    if (p.bias && e < p.groups) {
-      const int g = lane_id() >> 4;
+  T* corner = (T*)p.out + (r0 + line_a) * p.n + c0 + line_b;
+  Accumulate<T, S::NA, S::NB, false> out;
+  auto add_bias = [&]() {
+    if constexpr (!SLAB_B) {
+      if (p.bias && e < p.groups) {
+        const int g = lane_id() >> 4;
 #pragma unroll
-      for (int y = 0; y < S::NB; ++y) {
-        f4v bias;   // (all in flight: clamped, not skipped)
+        for (int y = 0; y < S::NB; ++y) {
+          f4v bias;   // (all in flight: clamped, not skipped)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) bias[r] = (float)((const T*)p.bias)[(int64_t)e * p.n + c0 + min(line_b + y * 16 + 4 * g + r, cols - 1)];
+          for (int r = 0; r < 4; ++r) bias[r] = (float)((const T*)p.bias)[(int64_t)e * p.n + c0 + min(line_b + y * 16 + 4 * g + r, cols - 1)];
 #pragma unroll
-        for (int x = 0; x < S::NA; ++x) out.acc[x][y] += bias;
+          for (int x = 0; x < S::NA; ++x) out.acc[x][y] += bias;
+        }
       }
     }
+  };
+  out.clear();
+  const bool live = e < p.groups;
+  if (live) tile_product<T, false, SLAB_B, TILE, LB, sizeof(T) == 4>(p.a + r0 * p.lda, p.lda, rows, b, p.ldb, cols, p.k, s0, s1, out, false);
+  bool again = false;
+  unsigned long long which = 0;
+  unsigned lines;
+  if constexpr (sizeof(T) == 4) {
+    again = live && any_wave(out.overflowed(), s0);
+    if (again) out.broken(which, lines);
   }
-  store_part<T, S::NA, S::NB>(out.acc, S::room(s0, s1), (T*)p.out + (r0 + line_a) * p.n + c0 + line_b, p.n, rows - line_a, cols - line_b);
+  add_bias();
+  store_part<T, S::NA, S::NB>(out.acc, S::room(s0, s1), corner, p.n, rows - line_a, cols - line_b);
+  if constexpr (sizeof(T) == 4) {
+    if (!again) return;
+    __syncthreads();   // (the stages are free of what was stored)
+    out.clear();
+    tile_product<T, false, SLAB_B, TILE, LB, false>(p.a + r0 * p.lda, p.lda, rows, b, p.ldb, cols, p.k, s0, s1, out, false);
+    add_bias();
+    store_broken(out.acc, which, corner, p.n, rows - line_a, cols - line_b);
+  }
 }
 
 // d w[e] [N][K] and d b[e]: a = dy as slabs (its columns are the lines), b = x as slabs, tiles of L x L.  Partial results: part [split][group][N][K], then part_b [split][group][N].
@@ -125,21 +143,39 @@ __global__ void __launch_bounds__(256, 2) grouped_weights(const GroupedArgs p, i
   Accumulate<T, S::NA, S::NB, true> acc;
   acc.clear();
   const bool sums = gb != nullptr && c0 == 0;
-  tile_product<T, true, true, L, L>(p.a + r0 * p.lda + m0 * (int64_t)sizeof(T), p.lda, lines, p.b + r0 * p.ldb + c0 * (int64_t)sizeof(T),
-                                    p.ldb, cols, r1 - r0, s0, s1, acc, sums);
+  const unsigned char *pa = p.a + r0 * p.lda + m0 * (int64_t)sizeof(T), *pb = p.b + r0 * p.ldb + c0 * (int64_t)sizeof(T);
+  tile_product<T, true, true, L, L, sizeof(T) == 4>(pa, p.lda, lines, pb, p.ldb, cols, r1 - r0, s0, s1, acc, sums);
   const int i = lane_id() & 15, g = lane_id() >> 4, line_a = S::line_a(), line_b = S::line_b();
-  if (sums && line_b == 0 && g == 0) {
-#pragma unroll
-    for (int x = 0; x < S::NA; ++x) {
-      const int row = line_a + x * 16 + i;
-      if (row >= lines) continue;
-      if (p.splits == 1) ((T*)gb)[(int64_t)e * n_rows + m0 + row] = (T)acc.sum[x][0];
-      else part_b[(int64_t)place * n_rows + m0 + row] = acc.sum[x][0];
-    }
+  bool again = false;
+  unsigned long long which = 0;
+  unsigned which_lines = 0;
+  if constexpr (sizeof(T) == 4) {
+    again = any_wave(acc.overflowed(), s0);
+    if (again) acc.broken(which, which_lines);
   }
+  auto put_sums = [&](unsigned of) {
+    if (sums && line_b == 0 && g == 0) {
+#pragma unroll
+      for (int x = 0; x < S::NA; ++x) {
+        const int row = line_a + x * 16 + i;
+        if (row >= lines || !(of >> x & 1)) continue;
+        if (p.splits == 1) ((T*)gb)[(int64_t)e * n_rows + m0 + row] = (T)acc.sum[x][0];
+        else part_b[(int64_t)place * n_rows + m0 + row] = acc.sum[x][0];
+      }
+    }
+  };
+  put_sums(~0u);
   const int64_t matrix = (int64_t)n_rows * p.n, at = (int64_t)(m0 + line_a) * p.n + c0 + line_b;
   if (p.splits == 1) store_part<T, S::NA, S::NB>(acc.acc, S::room(s0, s1), (T*)p.out + e * matrix + at, p.n, lines - line_a, cols - line_b);
   else store_part<float, S::NA, S::NB>(acc.acc, S::room(s0, s1), p.part + place * matrix + at, p.n, lines - line_a, cols - line_b);
+  if constexpr (sizeof(T) == 4) {
+    if (!again) return;
+    __syncthreads();   // (the stages are free of what was stored)
+    acc.clear();
+    tile_product<T, true, true, L, L, false>(pa, p.lda, lines, pb, p.ldb, cols, r1 - r0, s0, s1, acc, sums);
+    put_sums(which_lines);
+    store_broken(acc.acc, which, p.splits == 1 ? (float*)p.out + e * matrix + at : p.part + place * matrix + at, p.n, lines - line_a, cols - line_b);
+  }
 }
 
 // d b[e] alone: 64 columns x 4 rows at a time; blockIdx.y the group, .z the split

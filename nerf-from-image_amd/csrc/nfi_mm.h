@@ -14,8 +14,8 @@
 //
 // 32-bit values meet as three bf16 ones each, v = h + m + l (24 bits in 8 + 8 + 8, exactly), in six products l h + h l + m m +
 // m h + h m + h h on the bf16 matrix cores: 96 clocks of them for 32 contracted values against 256 of
-// v_mfma_f32_16x16x4_f32, and what is left out is at most 2^-24 of a product.  (An infinity, or a value that bf16 rounds to
-// one, leaves NaN: its parts m and l are no numbers.)
+// v_mfma_f32_16x16x4_f32, and what is left out is at most 2^-24 of a product.  An infinity, or a value that bf16 rounds to
+// one, has parts that are no numbers: sums that do not come out finite are taken again in 32-bit products (any_wave).
 #pragma once
 #include "nfi_learn.h"
 
@@ -214,14 +214,14 @@ struct Accumulate {
       for (int y = 0; y < NB; ++y) acc[x][y] = f4v{0.f, 0.f, 0.f, 0.f};
     }
   }
-  // one sub-step of 16-bit values
+  // one sub-step, of 16-bit values or in 32-bit products
   __device__ __forceinline__ void add(const u4v (&fa)[NA], const u4v (&fb)[NB], bool sums) {
 #pragma unroll
     for (int x = 0; x < NA; ++x)
 #pragma unroll
       for (int y = 0; y < NB; ++y) acc[x][y] = product<T>(fb[y], fa[x], acc[x][y]);
     if (SUM && sums) {
-      const unsigned one = TypeCode<T>::V == NFI_BF16 ? 0x3f803f80u : 0x3c003c00u;
+      const unsigned one = TypeCode<T>::V == NFI_F32 ? 0x3f800000u : TypeCode<T>::V == NFI_BF16 ? 0x3f803f80u : 0x3c003c00u;
       const u4v ones = {one, one, one, one};
 #pragma unroll
       for (int x = 0; x < NA; ++x) sum[x] = product<T>(ones, fa[x], sum[x]);
@@ -256,13 +256,41 @@ struct Accumulate {
       }
     }
   }
+  // is a sum of this lane not finite?
+  __device__ __forceinline__ bool overflowed() const {
+    float z = 0.f;   // (a number times 0, added: 0, or no number)
+#pragma unroll
+    for (int x = 0; x < NA; ++x) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (SUM) z = fmaf(sum[x][r], 0.f, z);
+#pragma unroll
+        for (int y = 0; y < NB; ++y) z = fmaf(acc[x][y][r], 0.f, z);
+      }
+    }
+    return z != 0.f;
+  }
+  // which of them (bit 4 (NB x + y) + r), and which of its lines' sums (bit x)
+  __device__ __forceinline__ void broken(unsigned long long& which, unsigned& lines) const {
+    static_assert(NA * NB * 4 <= 64, "a bit for each sum");
+    which = 0;
+    lines = 0;
+#pragma unroll
+    for (int x = 0; x < NA; ++x) {
+      if (SUM) lines |= (unsigned)!(fabsf(sum[x][0]) < INFINITY) << x;
+#pragma unroll
+      for (int y = 0; y < NB; ++y)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) which |= (unsigned long long)!(fabsf(acc[x][y][r]) < INFINITY) << (4 * (NB * x + y) + r);
+    }
+  }
 };
 
 // An LA x LB product tile: steps over the contracted index through two stages of LDS, each of (LA + LB) x 128 bytes.  A step's
 // fragments go to registers, its stage is free after a barrier, and the loads of the step after next are made into it while the
 // step's (last) products run: loads have a whole step to arrive.  (The stages are two variables of their own: the compiler waits
 // for all loads into the one that is read, and for no others.)
-template <class T, bool SLAB_A, bool SLAB_B, int LA, int LB, bool SUM>
+template <class T, bool SLAB_A, bool SLAB_B, int LA, int LB, bool PARTS, bool SUM>
 __device__ __forceinline__ void tile_product(const unsigned char* a, unsigned lda, int lines_a, const unsigned char* b, unsigned ldb,
                                              int lines_b, int64_t contracted, unsigned char* s0, unsigned char* s1,
                                              Accumulate<T, Share<LA, LB>::NA, Share<LA, LB>::NB, SUM>& out, bool sums) {
@@ -297,7 +325,7 @@ __device__ __forceinline__ void tile_product(const unsigned char* a, unsigned ld
     __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): this wave has read the step
     bare_barrier();
     issue(t + 2, cur);
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (PARTS) {   // (of 32-bit values)
       out.add32(fa, fb, sums);
     } else {
       out.add(fa[0], fb[0], sums);
@@ -314,6 +342,19 @@ __device__ __forceinline__ void tile_product(const unsigned char* a, unsigned ld
   if (t < steps) step(t, s0);
   wait_loads<0>();
   bare_barrier();   // the stages are free: no wave reads, and no load is on its way
+}
+
+// Has any wave of the workgroup, behind its product, a sum that is not finite?  (32-bit values in parts: an infinity's are no
+// numbers.  The sums that are finite stay, and keep their bits whatever another row holds; the others are taken again in 32-bit
+// products and stored over them.  The test costs less than 1 % of a tile of 512 contracted values.)
+__device__ __forceinline__ bool any_wave(bool mine, unsigned char* free_stage) {
+  int* votes = (int*)free_stage;
+  const bool wave = __ballot(mine) != 0;
+  if (lane_id() == 0) votes[threadIdx.x >> 6] = wave;
+  __syncthreads();
+  const bool any = (votes[0] | votes[1] | votes[2] | votes[3]) != 0;
+  __syncthreads();
+  return any;
 }
 
 // A wave's part of a product tile to rows of `out` (ld elements apart; `rows` x `cols` of them from this wave's
@@ -366,6 +407,21 @@ __device__ __forceinline__ void store_part(const f4v (&acc)[NA][NB], unsigned ch
       }
     }
   }
+}
+
+// The sums of `which` (Accumulate::broken) alone, to the same places
+template <int NA, int NB>
+__device__ __forceinline__ void store_broken(const f4v (&acc)[NA][NB], unsigned long long which, float* out, int64_t ld, int rows, int cols) {
+  const int i = lane_id() & 15, g = lane_id() >> 4;
+#pragma unroll
+  for (int x = 0; x < NA; ++x)
+#pragma unroll
+    for (int y = 0; y < NB; ++y)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = 16 * x + i, col = 16 * y + 4 * g + r;
+        if ((which >> (4 * (NB * x + y) + r) & 1) && row < rows && col < cols) out[row * ld + col] = acc[x][y][r];
+      }
 }
 
 }  // namespace learn

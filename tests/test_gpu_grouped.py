@@ -198,3 +198,47 @@ def test_captured_and_replayed():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(held, step()))
+
+
+def alike(got, ref, dtype):
+    """The same infinities and the same places without a number as the formula in 64 bits; the rest within the tolerance."""
+    value, mags, length = ref
+    got64 = got.double()
+    assert torch.equal(torch.isnan(got64), torch.isnan(value))
+    inf = torch.isinf(value)
+    assert torch.equal(torch.isinf(got64), inf) and torch.equal(got64[inf], value[inf])
+    keep = torch.isfinite(value)
+    near(got[keep], (value[keep], mags[keep], length), dtype)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('k,n', [(40, 24), (64, 64), (200, 130), (513, 257)])
+def test_infinities_and_large_values_are_those_of_the_formula(k, n, dtype):
+    """An infinity in a row, a weight or a gradient gives the sums that hold it (infinities of its sign; no number where it
+    meets its opposite or a zero), and values next to the type's largest, which 16 bits of their leading part may not hold, give their
+    products.  What holds none of them keeps its bits."""
+    x, w, offsets, b, gy, off = make([300, 0, 150], k, n, dtype, k + n)
+    clean_y = grouped.grouped_linear(x, w, offsets, b)
+    clean = [clean_y.detach()] + list(torch.autograd.grad(clean_y, [x, w, b], gy))
+    big = torch.finfo(dtype).max
+    with torch.no_grad():
+        x[7, 5], x[9, 0], x[9, 1], x[40, 3] = float('inf'), float('inf'), float('-inf'), float('-inf')
+        x[301, 2] = big * 2.0 ** -6      # (times a weight and added: far from the end, but for rounding up of its leading part)
+        x[302, :] = 0
+        x[302, 4] = big
+        w[2, :, 4] *= 2.0 ** -8
+        w[2, 3, 6] = float('inf')        # (row 302 holds a zero there)
+        gy[11, 1], gy[350, 2] = float('-inf'), big * 2.0 ** -6
+    y = grouped.grouped_linear(x, w, offsets, b)
+    got = [y.detach()] + list(torch.autograd.grad(y, [x, w, b], gy))
+    refs = reference(x, w, off, b, gy)
+    # a value past the type's range is an infinity in it; next to the range's end it may be either, and is not looked at
+    for a, (value, mags, length) in zip(got, refs):
+        over = value.abs() >= big * (1 + 2.0 ** -6)
+        either = torch.isfinite(value) & ~over & (value.abs() + 2.0 ** -7 * mags >= big)
+        value = torch.where(over, value.sign() * float('inf'), value).masked_fill(either, 0.0)
+        alike(a.masked_fill(either, 0.0), (value, mags, length), dtype)
+    rest = [i for i in range(300) if i not in (7, 9, 40)]
+    assert torch.equal(got[0][rest], clean[0][rest])
+    rest = [i for i in range(300) if i != 11]
+    assert torch.equal(got[1][rest], clean[1][rest])
