@@ -6,11 +6,18 @@
 //   nfi::residual_norm(h, residual?, gate?, weight?, bias?, next_weight?, next_bias?, norm, next_norm, slope, scale,
 //                      eps) -> Tensor[]       x, or x and y
 //   nfi::grouped_linear(x, weight, offsets, bias?) -> Tensor
-//   nfi::orthogonalize(u, steps, a, b, c, eps) -> Tensor
-//   nfi::muon_step(params, grads, momenta, ...) -> ()       in place
+//   nfi::residual_norm_fwd / _bwd, nfi::grouped_linear_fwd / _bwd      their halves as plain ops (CUDA + Meta kernels)
+//   nfi::orthogonalize(u, steps, a, b, c, eps) -> Tensor               (CUDA + Meta kernels)
+//   nfi::muon_step(params, grads, momenta, ...) -> ()       in place   (CUDA + Meta kernels)
+//
+// The autograd functions call the halves' functions themselves; where a tensor has no memory, or a dispatch mode looks on (meta and
+// fake tensors, tracing), they call them through the dispatcher, whose Meta kernels give shapes and touch no pointer.
+#include <array>
 #include <cmath>
 #include <vector>
 
+#include <ATen/core/dispatch/Dispatcher.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/autograd.h>
 #include <torch/library.h>
@@ -39,7 +46,16 @@ int32_t type_code(const Tensor& t, const char* what) {
 }
 
 void on_device(const char* what, const Tensor& first) {
-  TORCH_CHECK(first.is_cuda(), what, ": nfi ops run on HIP devices only (got a ", first.device(), " tensor)");
+  TORCH_CHECK(first.is_cuda() || first.is_meta(), what, ": nfi ops run on HIP devices only (got a ", first.device(), " tensor)");
+}
+// is the call one that is traced?  (its tensors may have no memory)
+bool traced(const Tensor& t) {
+  return t.is_meta() || t.key_set().has(c10::DispatchKey::Python) || t.key_set().has(c10::DispatchKey::Functionalize) ||
+         c10::impl::TorchDispatchModeTLS::any_modes_set();
+}
+template <class F>
+c10::TypedOperatorHandle<F> halves(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
 }
 void with(const char* what, const char* name, const Tensor& t, const Tensor& first) {
   TORCH_CHECK(!t.defined() || t.device() == first.device(), what, ": ", name, " is on ", t.device(), ", the first input on ",
@@ -49,6 +65,7 @@ void with(const char* what, const char* name, const Tensor& t, const Tensor& fir
 Tensor get(const Maybe& t) { return t ? *t : Tensor(); }
 Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); }
 Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+Tensor listed(const Tensor& t, const Tensor& like) { return t.defined() ? t : torch::empty({0}, like.options()); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor bytes(int64_t n, const Tensor& like) { return n > 0 ? torch::empty({n}, like.options().dtype(torch::kByte)) : Tensor(); }
 void once(const char* what) {
@@ -89,32 +106,83 @@ nfi_resnorm_args norm_args(const Tensor* in, const NormConf& c) {   // in: h, re
   return a;
 }
 
-struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
-  static variable_list forward(AutogradContext* ctx, Tensor h, Maybe residual_, Maybe gate_, Maybe weight_, Maybe bias_, Maybe next_weight_,
-                               Maybe next_bias_, int64_t norm, int64_t next, double slope, double scale, double eps, bool train) {
-    const c10::DeviceGuard guard(h.device());
-    const Tensor in[7] = {h, get(residual_), get(gate_), get(weight_), get(bias_), get(next_weight_), get(next_bias_)};
-    const NormConf c{norm, next, slope, scale, eps};
-    Tensor x = torch::empty_like(h), y = next ? torch::empty_like(h) : Tensor(), stats;
-    if (h.size(0) > 0) {
+// x, y and the statistics (those that are wanted); in: contiguous, h [rows, width]
+variable_list norm_forward(const Tensor* in, const NormConf& c, bool keep, bool shapes_only) {
+  const Tensor& h = in[0];
+  Tensor x = torch::empty_like(h), y = c.next ? torch::empty_like(h) : Tensor(), stats;
+  if (h.size(0) > 0) {
+    if (keep) stats = torch::empty({h.size(0), 4}, h.options().dtype(torch::kFloat));
+    if (!shapes_only) {
       nfi_resnorm_args a = norm_args(in, c);
-      if (train) stats = torch::empty({h.size(0), 4}, h.options().dtype(torch::kFloat));
       a.x = ptr(x);
       a.y = ptr(y);
       a.stats = (float*)ptr(stats);
       check(nfi_resnorm_forward(&a, stream_of(h)), "nfi_resnorm_forward");
     }
+  }
+  return {x, y, stats};
+}
+
+// the gradients of in[k] where needs[k]; gx, gy: contiguous, one of them at least
+variable_list norm_backward(const Tensor& gx, const Tensor& gy, const Tensor* in, const Tensor& stats, const NormConf& c, const std::array<bool, 7>& needs,
+                            bool shapes_only) {
+  variable_list out(7);
+  const bool none = in[0].size(0) == 0;
+  for (int k = 0; k < 7; ++k) {
+    if (!needs[k]) continue;
+    // (nothing reaches the next norm's parameters without a gradient of y)
+    out[k] = none || (k >= 5 && !gy.defined()) ? torch::zeros_like(in[k]) : torch::empty_like(in[k]);
+  }
+  if (none || shapes_only) return out;
+  nfi_resnorm_args a = norm_args(in, c);
+  a.stats = (float*)ptr(stats);
+  a.gx = ptr(gx);
+  a.gy = ptr(gy);
+  a.dh = ptr(out[0]);
+  a.dresidual = ptr(out[1]);
+  a.dgate = ptr(out[2]);
+  a.dweight = ptr(out[3]);
+  a.dbias = ptr(out[4]);
+  if (gy.defined()) {
+    a.dnext_weight = ptr(out[5]);
+    a.dnext_bias = ptr(out[6]);
+  }
+  const Tensor work = bytes(nfi_resnorm_work_bytes(a.rows, a.groups, a.affine_groups, a.width), in[0]);
+  a.work = (float*)ptr(work);
+  check(nfi_resnorm_backward(&a, stream_of(in[0])), "nfi_resnorm_backward");
+  return out;
+}
+
+typedef std::vector<Tensor> norm_fwd_t(const Tensor&, const Maybe&, const Maybe&, const Maybe&, const Maybe&, const Maybe&, const Maybe&, int64_t,
+                                       int64_t, double, double, double, bool);
+typedef std::vector<Tensor> norm_bwd_t(const Maybe&, const Maybe&, const Tensor&, const Maybe&, const Maybe&, const Maybe&, const Maybe&, const Maybe&,
+                                       const Maybe&, const Maybe&, int64_t, int64_t, double, double, double, std::array<bool, 7>);
+
+struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
+  static variable_list forward(AutogradContext* ctx, Tensor h, Maybe residual_, Maybe gate_, Maybe weight_, Maybe bias_, Maybe next_weight_,
+                               Maybe next_bias_, int64_t norm, int64_t next, double slope, double scale, double eps, bool train) {
+    variable_list r;
+    if (traced(h)) {
+      static auto op = halves<norm_fwd_t>("nfi::residual_norm_fwd");
+      r = op.call(h, residual_, gate_, weight_, bias_, next_weight_, next_bias_, norm, next, slope, scale, eps, train);
+      for (int k = 1; k < 3; ++k)
+        if (k == 1 ? next == 0 : !train || h.size(0) == 0) r[k] = Tensor();
+    } else {
+      const c10::DeviceGuard guard(h.device());
+      const Tensor in[7] = {h, get(residual_), get(gate_), get(weight_), get(bias_), get(next_weight_), get(next_bias_)};
+      r = norm_forward(in, NormConf{norm, next, slope, scale, eps}, train, false);
+    }
     if (train) {
       ctx->set_materialize_grads(false);
-      ctx->save_for_backward({in[0], in[1], in[2], in[3], in[4], in[5], in[6], stats});
+      ctx->save_for_backward({h, get(residual_), get(gate_), get(weight_), get(bias_), get(next_weight_), get(next_bias_), r[2]});
       ctx->saved_data["norm"] = norm;
       ctx->saved_data["next"] = next;
       ctx->saved_data["slope"] = slope;
       ctx->saved_data["scale"] = scale;
       ctx->saved_data["eps"] = eps;
     }
-    if (next) return {x, y};
-    return {x};
+    if (next) return {r[0], r[1]};
+    return {r[0]};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list g) {
@@ -125,45 +193,30 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
     const variable_list s = ctx->get_saved_variables();
     const NormConf c{ctx->saved_data["norm"].toInt(), ctx->saved_data["next"].toInt(), ctx->saved_data["slope"].toDouble(),
                      ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble()};
-    const c10::DeviceGuard guard(s[0].device());
-    const bool none = s[0].size(0) == 0;
-    for (int k = 0, edge = 0; k < 7; ++k) {   // (the graph's edges are those of the arguments that are there)
-      if (!s[k].defined() || !ctx->needs_input_grad(edge++)) continue;
-      // (nothing reaches the next norm's parameters without a gradient of y)
-      out[k] = none || (k >= 5 && !gy.defined()) ? torch::zeros_like(s[k]) : torch::empty_like(s[k]);
+    std::array<bool, 7> needs;
+    for (int k = 0, edge = 0; k < 7; ++k)   // (the graph's edges are those of the arguments that are there)
+      needs[k] = s[k].defined() && ctx->needs_input_grad(edge++);
+    variable_list r;
+    if (traced(s[0]) || traced(gx.defined() ? gx : gy)) {
+      static auto op = halves<norm_bwd_t>("nfi::residual_norm_bwd");
+      r = op.call(maybe(gx), maybe(gy), s[0], maybe(s[1]), maybe(s[2]), maybe(s[3]), maybe(s[4]), maybe(s[5]), maybe(s[6]), maybe(s[7]), c.norm, c.next,
+                  c.slope, c.scale, c.eps, needs);
+    } else {
+      const c10::DeviceGuard guard(s[0].device());
+      r = norm_backward(gx, gy, s.data(), s[7], c, needs, false);
     }
-    if (none) return out;
-    nfi_resnorm_args a = norm_args(s.data(), c);
-    a.stats = (float*)ptr(s[7]);
-    a.gx = ptr(gx);
-    a.gy = ptr(gy);
-    a.dh = ptr(out[0]);
-    a.dresidual = ptr(out[1]);
-    a.dgate = ptr(out[2]);
-    a.dweight = ptr(out[3]);
-    a.dbias = ptr(out[4]);
-    if (gy.defined()) {
-      a.dnext_weight = ptr(out[5]);
-      a.dnext_bias = ptr(out[6]);
-    }
-    const Tensor work = bytes(nfi_resnorm_work_bytes(a.rows, a.groups, a.affine_groups, a.width), s[0]);
-    a.work = (float*)ptr(work);
-    check(nfi_resnorm_backward(&a, stream_of(s[0])), "nfi_resnorm_backward");
+    for (int k = 0; k < 7; ++k)
+      if (needs[k]) out[k] = r[k];
     return out;
   }
 };
 
-std::vector<Tensor> residual_norm(const Tensor& h, const Maybe& residual_, const Maybe& gate_, const Maybe& weight_, const Maybe& bias_,
-                                  const Maybe& next_weight_, const Maybe& next_bias_, int64_t norm, int64_t next, double slope, double scale,
-                                  double eps) {
-  const char* what = "residual_norm";
-  Tensor residual = get(residual_), gate = get(gate_);
-  Tensor p[4] = {get(weight_), get(bias_), get(next_weight_), get(next_bias_)};
-  static const char* names[4] = {"weight", "bias", "next_weight", "next_bias"};
+// in: h, residual, gate, weight, bias, next_weight, next_bias.  Returns the first of the norms' parameters
+const Tensor* check_norm(const char* what, const Tensor* in, int64_t norm, int64_t next, double eps) {
+  static const char* names[7] = {"h", "residual", "gate", "weight", "bias", "next_weight", "next_bias"};
+  const Tensor &h = in[0], &residual = in[1], &gate = in[2];
   on_device(what, h);
-  with(what, "residual", residual, h);
-  with(what, "gate", gate, h);
-  for (int k = 0; k < 4; ++k) with(what, names[k], p[k], h);
+  for (int k = 1; k < 7; ++k) with(what, names[k], in[k], h);
   type_code(h, what);
   TORCH_CHECK_VALUE(norm >= 0 && norm <= 2 && next >= 0 && next <= 2, what, ": norms are 0, 1 or 2");
   TORCH_CHECK_VALUE(h.dim() >= 1 && h.size(-1) >= 1 && h.size(-1) <= NFI_RESNORM_MAX_WIDTH, what, ": rows of 1 to ", NFI_RESNORM_MAX_WIDTH,
@@ -173,27 +226,90 @@ std::vector<Tensor> residual_norm(const Tensor& h, const Maybe& residual_, const
   TORCH_CHECK_VALUE(!residual.defined() || (residual.sizes() == h.sizes() && residual.scalar_type() == h.scalar_type()), what,
                     ": residual is ", residual.sizes(), " ", residual.defined() ? residual.scalar_type() : h.scalar_type(), ", h ", h.sizes(), " ",
                     h.scalar_type());
-  TORCH_CHECK_VALUE(next != 0 || (!p[2].defined() && !p[3].defined()), what, ": next_weight and next_bias need next_norm");
+  TORCH_CHECK_VALUE(next != 0 || (!in[5].defined() && !in[6].defined()), what, ": next_weight and next_bias need next_norm");
   const Tensor* first = nullptr;
-  for (int k = 0; k < 4; ++k) {
-    if (!p[k].defined()) continue;
-    type_code(p[k], what);
-    const bool fits = (p[k].dim() == 1 && p[k].size(0) == d) ||
-                      (p[k].dim() == 2 && p[k].size(1) == d && p[k].size(0) >= 1 && rows % p[k].size(0) == 0);
-    TORCH_CHECK_VALUE(fits && (!first || (first->sizes() == p[k].sizes() && first->scalar_type() == p[k].scalar_type())), what, ": ", names[k],
-                      " is ", p[k].sizes(), " ", p[k].scalar_type(), "; [", d, "], or [G, ", d, "] with G a divisor of ", rows,
+  for (int k = 3; k < 7; ++k) {
+    const Tensor& p = in[k];
+    if (!p.defined()) continue;
+    type_code(p, what);
+    const bool fits = (p.dim() == 1 && p.size(0) == d) || (p.dim() == 2 && p.size(1) == d && p.size(0) >= 1 && rows % p.size(0) == 0);
+    TORCH_CHECK_VALUE(fits && (!first || (first->sizes() == p.sizes() && first->scalar_type() == p.scalar_type())), what, ": ", names[k],
+                      " is ", p.sizes(), " ", p.scalar_type(), "; [", d, "], or [G, ", d, "] with G a divisor of ", rows,
                       " rows is wanted, all of one shape and type");
-    if (!first) first = &p[k];
+    if (!first) first = &p;
   }
   if (gate.defined()) {
     type_code(gate, what);
+    const int64_t gates = gate.dim() == 2 ? gate.size(0) : 1;
+    TORCH_CHECK_VALUE((gate.dim() == 1 || gate.dim() == 2) && gate.size(-1) == d && gates >= 1 && rows % gates == 0, what, ": gate is ",
+                      gate.sizes(), "; [", d, "] or [G, ", d, "] with G a divisor of ", rows, " rows is wanted");
+    if (first && first->dim() == 2)
+      TORCH_CHECK_VALUE(gates == 1 || gates == first->size(0), what, ": ", gates, " gates and ", first->size(0), " groups of parameters");
+  }
+  return first;
+}
+
+// the halves as operators: everything contiguous, h and the gate [.., width]
+void check_halves(const char* what, const Tensor* in, int64_t norm, int64_t next, double eps) {
+  const Tensor* first = check_norm(what, in, norm, next, eps);
+  TORCH_CHECK_VALUE(in[0].dim() == 2, what, ": h [rows, width] is wanted, not ", in[0].sizes());
+  TORCH_CHECK_VALUE(!in[2].defined() || (in[2].dim() == 2 && (!first || first->dim() == 1 || first->size(0) == in[2].size(0))), what,
+                    ": a gate [G, width], and G groups of parameters where they have groups, are wanted");
+  for (int k = 0; k < 7; ++k) TORCH_CHECK_VALUE(!in[k].defined() || in[k].is_contiguous(), what, ": contiguous tensors are wanted");
+}
+
+template <bool META>
+std::vector<Tensor> residual_norm_fwd(const Tensor& h, const Maybe& residual, const Maybe& gate, const Maybe& weight, const Maybe& bias,
+                                      const Maybe& next_weight, const Maybe& next_bias, int64_t norm, int64_t next, double slope, double scale,
+                                      double eps, bool keep) {
+  const Tensor in[7] = {h, get(residual), get(gate), get(weight), get(bias), get(next_weight), get(next_bias)};
+  check_halves("residual_norm_fwd", in, norm, next, eps);
+  c10::OptionalDeviceGuard guard;
+  if (!META) guard.reset_device(h.device());
+  variable_list r = norm_forward(in, NormConf{norm, next, slope, scale, eps}, keep, META);
+  for (auto& t : r) t = listed(t, h);
+  return r;
+}
+
+template <bool META>
+std::vector<Tensor> residual_norm_bwd(const Maybe& gx_, const Maybe& gy_, const Tensor& h, const Maybe& residual, const Maybe& gate,
+                                      const Maybe& weight, const Maybe& bias, const Maybe& next_weight, const Maybe& next_bias,
+                                      const Maybe& stats_, int64_t norm, int64_t next, double slope, double scale, double eps,
+                                      std::array<bool, 7> needs) {
+  const char* what = "residual_norm_bwd";
+  const Tensor in[7] = {h, get(residual), get(gate), get(weight), get(bias), get(next_weight), get(next_bias)};
+  check_halves(what, in, norm, next, eps);
+  const Tensor gx = get(gx_), gy = get(gy_), stats = get(stats_);
+  TORCH_CHECK_VALUE(gx.defined() || gy.defined(), what, ": no gradient");
+  TORCH_CHECK_VALUE(next != 0 || !gy.defined(), what, ": gy without a next norm");
+  for (const Tensor& g : {gx, gy}) {
+    with(what, "a gradient", g, h);
+    TORCH_CHECK_VALUE(!g.defined() || (g.sizes() == h.sizes() && g.scalar_type() == h.scalar_type() && g.is_contiguous()), what,
+                      ": gradients like h, contiguous, are wanted");
+  }
+  with(what, "stats", stats, h);
+  TORCH_CHECK_VALUE(h.size(0) == 0 || (stats.defined() && stats.dim() == 2 && stats.size(0) == h.size(0) && stats.size(1) == 4 &&
+                                       stats.scalar_type() == torch::kFloat && stats.is_contiguous()),
+                    what, ": the forward's stats [rows, 4] are wanted");
+  for (int k = 0; k < 7; ++k) TORCH_CHECK_VALUE(!needs[k] || in[k].defined(), what, ": a gradient of an absent argument");
+  c10::OptionalDeviceGuard guard;
+  if (!META) guard.reset_device(h.device());
+  variable_list r = norm_backward(gx, gy, in, stats, NormConf{norm, next, slope, scale, eps}, needs, META);
+  for (auto& t : r) t = listed(t, h);
+  return r;
+}
+
+std::vector<Tensor> residual_norm(const Tensor& h, const Maybe& residual_, const Maybe& gate_, const Maybe& weight_, const Maybe& bias_,
+                                  const Maybe& next_weight_, const Maybe& next_bias_, int64_t norm, int64_t next, double slope, double scale,
+                                  double eps) {
+  Tensor residual = get(residual_), gate = get(gate_);
+  const Tensor p[4] = {get(weight_), get(bias_), get(next_weight_), get(next_bias_)};
+  const Tensor in[7] = {h, residual, gate, p[0], p[1], p[2], p[3]};
+  const Tensor* first = check_norm("residual_norm", in, norm, next, eps);
+  const int64_t d = h.size(-1), rows = h.numel() / d;
+  if (gate.defined()) {
     if (gate.dim() == 1) gate = gate.unsqueeze(0);
-    TORCH_CHECK_VALUE(gate.dim() == 2 && gate.size(1) == d && gate.size(0) >= 1 && rows % gate.size(0) == 0, what, ": gate is ", gate.sizes(),
-                      "; [", d, "] or [G, ", d, "] with G a divisor of ", rows, " rows is wanted");
-    if (first && first->dim() == 2 && gate.size(0) != first->size(0)) {
-      TORCH_CHECK_VALUE(gate.size(0) == 1, what, ": ", gate.size(0), " gates and ", first->size(0), " groups of parameters");
-      gate = gate.expand({first->size(0), d});
-    }
+    if (first && first->dim() == 2 && gate.size(0) != first->size(0)) gate = gate.expand({first->size(0), d});
     gate = gate.contiguous();
   }
   bool train = false;
@@ -227,54 +343,79 @@ nfi_grouped_args grouped_args(const Tensor& x, const Tensor& w, const Tensor& of
   return a;
 }
 
+Tensor grouped_forward(const Tensor& x, const Tensor& w, const Tensor& offsets, const Tensor& bias, bool shapes_only) {
+  Tensor y = torch::empty({x.size(0), w.size(1)}, x.options());
+  if (x.size(0) == 0 || shapes_only) return y;
+  nfi_grouped_args a = grouped_args(x, w, offsets);
+  a.bias = ptr(bias);
+  a.y = y.data_ptr();
+  a.work_bytes = nfi_grouped_forward_work_bytes(&a);
+  const Tensor work = bytes(a.work_bytes, x);
+  a.work = ptr(work);
+  check(nfi_grouped_forward(&a, stream_of(x)), "nfi_grouped_forward");
+  return y;
+}
+
+// the gradients of x, weight and bias, those that are needed
+variable_list grouped_backward(const Tensor& gy, const Tensor& x, const Tensor& w, const Tensor& offsets, const std::array<bool, 3>& needs,
+                               bool shapes_only) {
+  const bool none = x.size(0) == 0;
+  variable_list out(3);
+  auto make = [&](at::IntArrayRef sizes) { return none ? torch::zeros(sizes, x.options()) : torch::empty(sizes, x.options()); };
+  if (needs[0]) out[0] = make(x.sizes());
+  if (needs[1]) out[1] = make(w.sizes());
+  if (needs[2]) out[2] = make({w.size(0), w.size(1)});
+  if (none || shapes_only) return out;
+  nfi_grouped_args a = grouped_args(x, w, offsets);
+  a.gy = gy.data_ptr();
+  a.gx = ptr(out[0]);
+  a.gw = ptr(out[1]);
+  a.gb = ptr(out[2]);
+  a.work_bytes = nfi_grouped_backward_work_bytes(&a);
+  const Tensor work = bytes(a.work_bytes, x);
+  a.work = ptr(work);
+  check(nfi_grouped_backward(&a, stream_of(x)), "nfi_grouped_backward");
+  return out;
+}
+
+typedef Tensor grouped_fwd_t(const Tensor&, const Tensor&, const Tensor&, const Maybe&);
+typedef std::vector<Tensor> grouped_bwd_t(const Tensor&, const Tensor&, const Tensor&, const Tensor&, std::array<bool, 3>);
+
 struct GroupedLinear : public torch::autograd::Function<GroupedLinear> {
   static Tensor forward(AutogradContext* ctx, Tensor x, Tensor w, Tensor offsets, Maybe bias_, bool train) {
-    const Tensor bias = get(bias_);
-    const c10::DeviceGuard guard(x.device());
-    Tensor y = torch::empty({x.size(0), w.size(1)}, x.options());
-    if (x.size(0) > 0) {
-      nfi_grouped_args a = grouped_args(x, w, offsets);
-      a.bias = ptr(bias);
-      a.y = y.data_ptr();
-      a.work_bytes = nfi_grouped_forward_work_bytes(&a);
-      const Tensor work = bytes(a.work_bytes, x);
-      a.work = ptr(work);
-      check(nfi_grouped_forward(&a, stream_of(x)), "nfi_grouped_forward");
-    }
     if (train) ctx->save_for_backward({x, w, offsets});
-    ctx->saved_data["bias"] = bias.defined();
-    return y;
+    ctx->saved_data["bias"] = bias_.has_value();
+    if (traced(x)) {
+      static auto op = halves<grouped_fwd_t>("nfi::grouped_linear_fwd");
+      return op.call(x, w, offsets, bias_);
+    }
+    const c10::DeviceGuard guard(x.device());
+    return grouped_forward(x, w, offsets, get(bias_), false);
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     once("grouped_linear");
     const variable_list s = ctx->get_saved_variables();
-    const Tensor &x = s[0], &w = s[1], &offsets = s[2];
-    const c10::DeviceGuard guard(x.device());
-    const bool none = x.size(0) == 0;
-    variable_list out(5);
-    auto make = [&](const Tensor& like) { return none ? torch::zeros_like(like) : torch::empty_like(like); };
-    if (ctx->needs_input_grad(0)) out[0] = make(x);
-    if (ctx->needs_input_grad(1)) out[1] = make(w);
-    if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(3)) out[3] = none ? torch::zeros({w.size(0), w.size(1)}, x.options()) : torch::empty({w.size(0), w.size(1)}, x.options());
-    if (none) return out;
+    const std::array<bool, 3> needs = {ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+                                       ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(3)};
     const Tensor gy = g[0].contiguous();
-    nfi_grouped_args a = grouped_args(x, w, offsets);
-    a.gy = gy.data_ptr();
-    a.gx = ptr(out[0]);
-    a.gw = ptr(out[1]);
-    a.gb = ptr(out[3]);
-    a.work_bytes = nfi_grouped_backward_work_bytes(&a);
-    const Tensor work = bytes(a.work_bytes, x);
-    a.work = ptr(work);
-    check(nfi_grouped_backward(&a, stream_of(x)), "nfi_grouped_backward");
+    variable_list r;
+    if (traced(s[0]) || traced(gy)) {
+      static auto op = halves<grouped_bwd_t>("nfi::grouped_linear_bwd");
+      r = op.call(gy, s[0], s[1], s[2], needs);
+    } else {
+      const c10::DeviceGuard guard(s[0].device());
+      r = grouped_backward(gy, s[0], s[1], s[2], needs, false);
+    }
+    variable_list out(5);
+    if (needs[0]) out[0] = r[0];
+    if (needs[1]) out[1] = r[1];
+    if (needs[2]) out[3] = r[2];
     return out;
   }
 };
 
-Tensor grouped_linear(const Tensor& x, const Tensor& w, const Tensor& offsets, const Maybe& bias_) {
-  const char* what = "grouped_linear";
-  const Tensor bias = get(bias_);
+void check_grouped(const char* what, const Tensor& x, const Tensor& w, const Tensor& offsets, const Tensor& bias) {
   on_device(what, x);
   with(what, "weight", w, x);
   with(what, "offsets", offsets, x);
@@ -292,6 +433,38 @@ Tensor grouped_linear(const Tensor& x, const Tensor& w, const Tensor& offsets, c
               ": x, weight and bias are of one type, not ", x.scalar_type(), ", ", w.scalar_type());
   TORCH_CHECK_VALUE(!bias.defined() || (bias.dim() == 2 && bias.size(0) == e && bias.size(1) == n), what, ": bias [", e, ", ", n,
                     "] is wanted, not ", bias.sizes());
+}
+
+template <bool META>
+Tensor grouped_linear_fwd(const Tensor& x, const Tensor& w, const Tensor& offsets, const Maybe& bias_) {
+  const char* what = "grouped_linear_fwd";
+  const Tensor bias = get(bias_);
+  check_grouped(what, x, w, offsets, bias);
+  TORCH_CHECK_VALUE(x.is_contiguous() && w.is_contiguous() && offsets.is_contiguous() && (!bias.defined() || bias.is_contiguous()), what,
+                    ": contiguous tensors are wanted");
+  c10::OptionalDeviceGuard guard;
+  if (!META) guard.reset_device(x.device());
+  return grouped_forward(x, w, offsets, bias, META);
+}
+
+template <bool META>
+std::vector<Tensor> grouped_linear_bwd(const Tensor& gy, const Tensor& x, const Tensor& w, const Tensor& offsets, std::array<bool, 3> needs) {
+  const char* what = "grouped_linear_bwd";
+  check_grouped(what, x, w, offsets, Tensor());
+  with(what, "gy", gy, x);
+  TORCH_CHECK_VALUE(gy.dim() == 2 && gy.size(0) == x.size(0) && gy.size(1) == w.size(1) && gy.scalar_type() == x.scalar_type(), what, ": gy [",
+                    x.size(0), ", ", w.size(1), "] of x's type is wanted, not ", gy.sizes(), " ", gy.scalar_type());
+  TORCH_CHECK_VALUE(gy.is_contiguous() && x.is_contiguous() && w.is_contiguous() && offsets.is_contiguous(), what, ": contiguous tensors are wanted");
+  c10::OptionalDeviceGuard guard;
+  if (!META) guard.reset_device(x.device());
+  variable_list r = grouped_backward(gy, x, w, offsets, needs, META);
+  for (auto& t : r) t = listed(t, x);
+  return r;
+}
+
+Tensor grouped_linear(const Tensor& x, const Tensor& w, const Tensor& offsets, const Maybe& bias_) {
+  const Tensor bias = get(bias_);
+  check_grouped("grouped_linear", x, w, offsets, bias);
   const bool train = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (bias.defined() && bias.requires_grad()));
   return GroupedLinear::apply(x.contiguous(), w.contiguous(), offsets.contiguous(), maybe(dense(bias)), train);
 }
@@ -312,12 +485,14 @@ void ortho(const std::vector<nfi_ortho_item>& items, nfi_ortho_args a, const Ten
   check(nfi_ortho(&a, stream), "nfi_ortho");
 }
 
+template <bool META>
 Tensor orthogonalize(const Tensor& u, int64_t steps, double ca, double cb, double cc, double eps) {
   const char* what = "orthogonalize";
   on_device(what, u);
   nfi_ortho_args a{};
   a.g_type = a.w_type = type_code(u, what);
   TORCH_CHECK_VALUE(u.dim() >= 2, what, ": matrices are wanted, not ", u.sizes());
+  if (META) return torch::empty(u.sizes(), u.options());
   const c10::DeviceGuard guard(u.device());
   const Tensor src = u.contiguous();
   Tensor out = torch::empty_like(src);
@@ -336,6 +511,7 @@ Tensor orthogonalize(const Tensor& u, int64_t steps, double ca, double cb, doubl
   return out;
 }
 
+template <bool META>
 void muon_step(at::TensorList params, at::TensorList grads, at::TensorList momenta, bool batched, double lr, double momentum, double decay,
                bool nesterov, int64_t steps, double ca, double cb, double cc, double eps) {
   const char* what = "Muon";
@@ -375,10 +551,15 @@ void muon_step(at::TensorList params, at::TensorList grads, at::TensorList momen
     const int64_t cols = batched ? p.size(-1) : p.numel() / p.size(0), rows = batched ? p.size(-2) : p.size(0), count = p.numel() / (rows * cols);
     TORCH_CHECK_VALUE(rows <= NFI_ORTHO_MAX_SIDE && cols <= NFI_ORTHO_MAX_SIDE && count < (1ll << 31), what, ": sides of 1 to ", NFI_ORTHO_MAX_SIDE,
                       " are wanted, not ", count, " of ", rows, " x ", cols);
+    if (META) continue;
     g[i] = grads[i].contiguous();
     size_t l = 0;
     while (l < lots.size() && lots[l].kind != kind) ++l;
-    if (l == lots.size()) lots.push_back({kind, {}, {}, Tensor()});
+    if (l == lots.size()) {
+      lots.push_back({kind, {}, {}, Tensor()});
+      lots[l].items.reserve(n - i);
+      lots[l].of.reserve(n - i);
+    }
     lots[l].items.push_back({g[i].data_ptr(), m.data_ptr(), p.data_ptr(), (int32_t)rows, (int32_t)cols, (int32_t)count,
                              (float)std::sqrt(std::max(1.0, (double)rows / (double)cols))});
     lots[l].of.push_back(i);
@@ -406,7 +587,14 @@ void muon_step(at::TensorList params, at::TensorList grads, at::TensorList momen
 TORCH_LIBRARY_FRAGMENT(nfi, m) {
   m.def("residual_norm(Tensor h, Tensor? residual, Tensor? gate, Tensor? weight, Tensor? bias, Tensor? next_weight, Tensor? next_bias, "
         "int norm, int next_norm, float slope, float scale, float eps) -> Tensor[]");
+  m.def("residual_norm_fwd(Tensor h, Tensor? residual, Tensor? gate, Tensor? weight, Tensor? bias, Tensor? next_weight, Tensor? next_bias, "
+        "int norm, int next_norm, float slope, float scale, float eps, bool stats) -> Tensor[]");
+  m.def("residual_norm_bwd(Tensor? gx, Tensor? gy, Tensor h, Tensor? residual, Tensor? gate, Tensor? weight, Tensor? bias, "
+        "Tensor? next_weight, Tensor? next_bias, Tensor? stats, int norm, int next_norm, float slope, float scale, float eps, "
+        "bool[7] needs) -> Tensor[]");
   m.def("grouped_linear(Tensor x, Tensor weight, Tensor offsets, Tensor? bias=None) -> Tensor");
+  m.def("grouped_linear_fwd(Tensor x, Tensor weight, Tensor offsets, Tensor? bias=None) -> Tensor");
+  m.def("grouped_linear_bwd(Tensor gy, Tensor x, Tensor weight, Tensor offsets, bool[3] needs) -> Tensor[]");
   m.def("orthogonalize(Tensor u, int steps, float a, float b, float c, float eps) -> Tensor");
   m.def("muon_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] momenta, bool batched, float lr, float momentum, float decay, "
         "bool nesterov, int steps, float a, float b, float c, float eps) -> ()");
@@ -415,6 +603,30 @@ TORCH_LIBRARY_FRAGMENT(nfi, m) {
 TORCH_LIBRARY_IMPL(nfi, CompositeImplicitAutograd, m) {
   m.impl("residual_norm", &residual_norm);
   m.impl("grouped_linear", &grouped_linear);
-  m.impl("orthogonalize", &orthogonalize);
-  m.impl("muon_step", &muon_step);
+}
+
+TORCH_LIBRARY_IMPL(nfi, CUDA, m) {
+  m.impl("residual_norm_fwd", &residual_norm_fwd<false>);
+  m.impl("residual_norm_bwd", &residual_norm_bwd<false>);
+  m.impl("grouped_linear_fwd", &grouped_linear_fwd<false>);
+  m.impl("grouped_linear_bwd", &grouped_linear_bwd<false>);
+}
+
+TORCH_LIBRARY_IMPL(nfi, CompositeExplicitAutograd, m) {   // (other devices' tensors are refused, and no tensors are no work)
+  m.impl("orthogonalize", &orthogonalize<false>);
+  m.impl("muon_step", &muon_step<false>);
+}
+
+TORCH_LIBRARY_IMPL(nfi, Autograd, m) {   // (not differentiable; the default would box every argument to say so, 2 us)
+  m.impl("orthogonalize", torch::CppFunction::makeFallthrough());
+  m.impl("muon_step", torch::CppFunction::makeFallthrough());
+}
+
+TORCH_LIBRARY_IMPL(nfi, Meta, m) {
+  m.impl("residual_norm_fwd", &residual_norm_fwd<true>);
+  m.impl("residual_norm_bwd", &residual_norm_bwd<true>);
+  m.impl("grouped_linear_fwd", &grouped_linear_fwd<true>);
+  m.impl("grouped_linear_bwd", &grouped_linear_bwd<true>);
+  m.impl("orthogonalize", &orthogonalize<true>);
+  m.impl("muon_step", &muon_step<true>);
 }

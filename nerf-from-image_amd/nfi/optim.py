@@ -28,6 +28,10 @@ def _op(name):
     return op
 
 
+def _capturing():
+    return torch.cuda.device_count() > 0 and torch.cuda.is_current_stream_capturing()
+
+
 def _check(what, steps, coefficients, eps):
     if not 1 <= int(steps) <= 64:
         raise ValueError(f'{what}: 1 to 64 steps are wanted, not {steps}')
@@ -92,12 +96,13 @@ class Muon(torch.optim.Optimizer):
                 g = p.grad
                 if g is None or p.numel() == 0:
                     continue
-                m = self.state[p].get('momentum_buffer') if p in self.state else None
+                state = self.state[p]
+                m = state.get('momentum_buffer')
                 if m is None:
-                    if torch.cuda.is_current_stream_capturing():
+                    if _capturing():
                         raise RuntimeError('Muon: the first step of a parameter makes its momentum, and in a graph every replay would '
                                            'clear it again: take one step before the capture')
-                    m = self.state[p]['momentum_buffer'] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
+                    m = state['momentum_buffer'] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
                 params.append(p)
                 grads.append(g)
                 momenta.append(m)

@@ -12,7 +12,8 @@ arguments as nfi.ops / nfi.stages; load() fails loudly when the library is missi
   torch.ops.nfi.sample_pdf / compute_near_far_planes / cumprod_exclusive /
   render_volume_density_weights_only                        the nerf_utils seams
   torch.ops.nfi.residual_norm / grouped_linear / orthogonalize / muon_step
-                              behind nfi.norms, nfi.grouped and nfi.optim (csrc/nfi_torch_learn.cpp)
+                              behind nfi.norms, nfi.grouped and nfi.optim (csrc/nfi_torch_learn.cpp);
+  residual_norm_fwd / _bwd, grouped_linear_fwd / _bwd      their halves (these and the two above: CUDA + Meta kernels)
 """
 
 from __future__ import annotations
@@ -28,7 +29,8 @@ LIBRARY = os.path.join(HERE, 'libnfi_torch.so')
 OPS = ('rays', 'pack_decoder', 'volume_render', 'volume_render_fwd', 'volume_render_bwd', 'sample_pdf',
        'compute_near_far_planes', 'cumprod_exclusive', 'render_volume_density_weights_only',
        'render_fwd', 'render_bwd', 'composite_fwd', 'composite_bwd', 'triplane_mlp_fwd', 'triplane_mlp_bwd',
-       'residual_norm', 'grouped_linear', 'orthogonalize', 'muon_step')
+       'residual_norm', 'residual_norm_fwd', 'residual_norm_bwd', 'grouped_linear', 'grouped_linear_fwd', 'grouped_linear_bwd',
+       'orthogonalize', 'muon_step')
 _loaded = False
 
 

@@ -215,3 +215,84 @@ def test_bank_of_an_empty_batch(images, rays):
     assert x.shape == (images, rays, 32)
     gv, gw = torch.autograd.grad(x.sum(), [v, b.mappers[0].fc1.weight])
     assert gv.shape == v.shape and float(gw.abs().max()) == 0
+
+
+def test_traced_and_scripted_calls():
+    """Fake tensors of the device give shapes, forward and backward, without a launch; under a mode that looks on, and
+    from TorchScript, the values and gradients are the call's own, bit for bit."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from test_learn_host import shapes_of_calls
+    from nfi import grouped, norms, torch_ops
+    with FakeTensorMode():
+        shapes_of_calls('cuda', True)
+
+    seen = []
+
+    class Looks(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    g = torch.Generator(device=DEV).manual_seed(9)
+
+    def rnd(*shape):
+        return torch.randn(shape, device=DEV, generator=g)
+    h, gate, weight, gx = rnd(12, 40), rnd(3, 40), rnd(40), rnd(12, 40)
+    x, w, b, gy = rnd(30, 24), rnd(2, 16, 24), rnd(2, 16), rnd(30, 16)
+    off = torch.tensor([0, 13, 28], device=DEV)
+    leaves = [t.requires_grad_() for t in (h, gate, weight, x, w, b)]
+
+    def all_of_it():
+        n = norms.residual_norm(h, None, gate, weight, slope=0.2, next_norm='rms')
+        y = grouped.grouped_linear(x, w, off, b)
+        return [*(t.detach() for t in (*n, y)), *torch.autograd.grad([*n, y], leaves, [gx, gx, gy]), optim.orthogonalize(w)]
+    want = all_of_it()
+    with Looks():
+        got = all_of_it()
+    assert all(torch.equal(a, c) for a, c in zip(want, got))
+    for name in ('residual_norm_fwd', 'residual_norm_bwd', 'grouped_linear_fwd', 'grouped_linear_bwd', 'orthogonalize'):
+        assert any(name in s for s in seen), name
+
+    torch_ops.load()
+    unit = torch.jit.CompilationUnit('''
+def run(h: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, x: torch.Tensor, w: torch.Tensor, off: torch.Tensor, b: torch.Tensor):
+    n = torch.ops.nfi.residual_norm(h, None, gate, weight, None, None, None, 1, 2, 0.2, 1.0, 1e-5)
+    y = torch.ops.nfi.grouped_linear(x, w, off, b)
+    return n[0], n[1], y, torch.ops.nfi.orthogonalize(w.detach(), 5, 3.4445, -4.7750, 2.0315, 1e-7)
+''')
+    for _ in range(3):
+        n0, n1, y, o = unit.run(h, gate, weight, x, w, off, b)
+        got = [n0.detach(), n1.detach(), y.detach(), *torch.autograd.grad([n0, n1, y], leaves, [gx, gx, gy]), o]
+        assert all(torch.equal(a, c) for a, c in zip(want, got))
+
+
+def test_halves_refuse_what_they_cannot_take():
+    """The plain operators behind the two autograd functions check their own arguments."""
+    from nfi import torch_ops
+    torch_ops.load()
+    ops = torch.ops.nfi
+    z = torch.zeros
+    h, st = z((4, 8), device=DEV), z((4, 4), device=DEV)
+    conf = (1, 0, 1.0, 1.0, 1e-5)
+    none6 = (None,) * 6
+    needs = [True] + [False] * 6
+    assert ops.residual_norm_fwd(h, *none6, *conf, True)[2].shape == (4, 4)
+    assert ops.residual_norm_bwd(h, None, h, *none6, st, *conf, needs)[0].shape == (4, 8)
+    x, w, off = z((5, 8), device=DEV), z((2, 3, 8), device=DEV), z((3,), device=DEV, dtype=torch.int64)
+    gy = z((5, 3), device=DEV)
+    for f, word in ((lambda: ops.residual_norm_fwd(z((2, 2, 8), device=DEV), *none6, *conf, True), 'rows, width'),
+                    (lambda: ops.residual_norm_fwd(h.t(), *none6, *conf, True), 'contiguous'),
+                    (lambda: ops.residual_norm_fwd(h, None, z((8,), device=DEV), *none6[2:], *conf, True), 'gate'),
+                    (lambda: ops.residual_norm_bwd(None, None, h, *none6, st, *conf, needs), 'no gradient'),
+                    (lambda: ops.residual_norm_bwd(h, None, h, *none6, None, *conf, needs), 'stats'),
+                    (lambda: ops.residual_norm_bwd(h, None, h, *none6, st[:3], *conf, needs), 'stats'),
+                    (lambda: ops.residual_norm_bwd(h[:3], None, h, *none6, st, *conf, needs), 'gradients like h'),
+                    (lambda: ops.residual_norm_bwd(h, h, h, *none6, st, *conf, needs), 'next norm'),
+                    (lambda: ops.residual_norm_bwd(h, None, h, *none6, st, *conf, [True] * 7), 'absent'),
+                    (lambda: ops.grouped_linear_fwd(x, w.transpose(1, 2).contiguous().transpose(1, 2), off), 'contiguous'),
+                    (lambda: ops.grouped_linear_bwd(gy[:4], x, w, off, [True] * 3), 'gy'),
+                    (lambda: ops.grouped_linear_bwd(gy.half(), x, w, off, [True] * 3), 'gy'),
+                    (lambda: ops.grouped_linear_bwd(gy, x, w, off[:2], [True] * 3), 'offsets')):
+        with pytest.raises((RuntimeError, ValueError), match=word):
+            f()

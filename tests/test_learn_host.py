@@ -192,7 +192,7 @@ def test_muon_refuses_a_first_step_in_a_capture(monkeypatch):
     a.grad, b.grad = torch.ones(3, 4), torch.ones(3, 4)
     stepped = []
     monkeypatch.setattr(optim, '_op', lambda name: lambda params, *rest: stepped.extend(params))
-    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+    monkeypatch.setattr(optim, '_capturing', lambda: True)
     with pytest.raises(RuntimeError, match='before the capture'):
         o.step()
     assert not stepped and 'momentum_buffer' not in o.state.get(b, {})
@@ -200,7 +200,7 @@ def test_muon_refuses_a_first_step_in_a_capture(monkeypatch):
     o.step()                     # (a parameter without a gradient has no part in it)
     assert stepped == [a]
     b.grad = torch.ones(3, 4)
-    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: False)
+    monkeypatch.setattr(optim, '_capturing', lambda: False)
     o.step()
     assert stepped == [a, a, b] and float(o.state[b]['momentum_buffer'].abs().max()) == 0
 
@@ -282,3 +282,100 @@ def test_bank_of_an_empty_batch(plain_bank, images, rays):
     assert x.shape == (images, rays, 32)
     gv, gw = torch.autograd.grad(x.sum(), [v, plain_bank.mappers[0].fc1.weight])
     assert gv.shape == v.shape and float(gw.abs().max()) == 0
+
+
+@pytest.fixture
+def fake():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode() as mode:
+        yield mode
+
+
+def shapes_of_calls(device, backward):
+    """Every operator on tensors of `device` without memory: shapes, types and devices of what it gives."""
+    def empty(*shape, dtype=torch.bfloat16):
+        return torch.empty(shape, device=device, dtype=dtype, requires_grad=dtype != torch.int64)
+
+    def like(got, want):
+        for a, b in zip(got, want):
+            assert (a.shape, a.dtype, a.device) == (b.shape, b.dtype, b.device)
+
+    def grads(out, leaves, given):
+        if backward:
+            like(torch.autograd.grad(out, leaves, given), leaves)
+    h, res, gate, w, b, w2, b2 = empty(2, 3, 40), empty(2, 3, 40), empty(2, 40, dtype=torch.float32), *(empty(40) for _ in range(4))
+    x, y = norms.residual_norm(h, res, gate, w, b, next_weight=w2, next_bias=b2, next_norm='rms')
+    like([x, y], [h, h])
+    grads([x, y], [h, res, gate, w, b, w2, b2], [h, h])
+    x, y = norms.residual_norm(h, None, None, w, next_norm='layer')
+    grads([x], [h, w], [h])
+    x = norms.residual_norm(h, res)
+    like([x], [h])
+    grads([x], [res], [h])
+    empties = norms.residual_norm(empty(0, 40), weight=w)
+    like([empties], [empty(0, 40)])
+    grads([empties], [w], [empty(0, 40)])
+    with torch.no_grad():
+        like([norms.residual_norm(h)], [h])
+
+    x, w, bias, off = empty(50, 24), empty(3, 16, 24), empty(3, 16), empty(4, dtype=torch.int64)
+    y = grouped.grouped_linear(x, w, off, bias)
+    like([y], [empty(50, 16)])
+    grads([y], [x, w, bias], [y])
+    grads([grouped.grouped_linear(x, w, off)], [w], [empty(50, 16)])
+
+    u = empty(2, 30, 20)
+    like([optim.orthogonalize(u), optim.orthogonalize(u.transpose(1, 2))], [u, u.transpose(1, 2)])
+
+
+def test_traced_calls_give_shapes(fake):
+    """Through the Meta kernels, with no launch (here there is no device that could take one)."""
+    shapes_of_calls('cuda', False)
+
+
+def test_meta_tensors_give_shapes_and_gradients():
+    shapes_of_calls('meta', True)
+
+
+def test_traced_calls_are_checked(fake):
+    """What a call refuses it refuses in a trace too."""
+    def empty(*shape, dtype=torch.float32):
+        return torch.empty(shape, device='cuda', dtype=dtype)
+    for f, word in ((lambda: norms.residual_norm(empty(4, 8), empty(4, 9)), 'residual'),
+                    (lambda: norms.residual_norm(empty(4, 8), gate=empty(3, 8)), 'gate'),
+                    (lambda: norms.residual_norm(empty(4, 8), weight=empty(2, 8), gate=empty(4, 8)), 'groups of parameters'),
+                    (lambda: grouped.grouped_linear(empty(4, 8), empty(2, 5, 8), empty(2, dtype=torch.int32)), 'offsets'),
+                    (lambda: optim.orthogonalize(empty(8)), 'matrices')):
+        with pytest.raises((RuntimeError, ValueError), match=word):
+            f()
+
+
+def test_traced_steps(fake):
+    """Muon's step over tensors without memory: its state's shapes, the checks of every parameter, and empty parameters, which
+    divide nothing."""
+    def param(*shape, dtype=torch.float32):
+        p = torch.nn.Parameter(torch.empty(shape, device='cuda', dtype=dtype))
+        p.grad = torch.empty_like(p)
+        return p
+    ps = [param(6, 4, 3, 3), param(0, 3), param(8, 8, dtype=torch.bfloat16)]
+    o = optim.Muon(ps)
+    o.step()
+    assert o.state[ps[2]]['momentum_buffer'].dtype == torch.float32 and o.state[ps[0]]['momentum_buffer'].shape == ps[0].shape
+    from nfi import torch_ops
+
+    def step(shapes, batched):
+        ts = [torch.empty(s, device='cuda') for s in shapes]
+        torch_ops.op('muon_step')(ts, [torch.empty_like(t) for t in ts], [torch.empty_like(t) for t in ts], batched, 0.1, 0.9, 0.0, True, 5,
+                                  *optim.QUINTIC, 1e-7)
+    step([(0, 3), (3, 0), (0, 0), (4, 0, 3), (5, 6)], False)
+    step([(2, 0, 4), (0, 3, 4), (2, 3, 0), (2, 3, 4)], True)
+    with pytest.raises(ValueError, match='sides'):
+        step([(5, 6), (2, 300000)], False)
+    with pytest.raises(RuntimeError, match='dense gradients'):
+        torch_ops.op('muon_step')([torch.empty(8, device='cuda')], [torch.empty(8, device='cuda')], [torch.empty(8, device='cuda')], False, 0.1,
+                                  0.9, 0.0, True, 5, *optim.QUINTIC, 1e-7)
+
+
+def test_no_tensors_are_no_step():
+    from nfi import torch_ops
+    torch_ops.op('muon_step')([], [], [], False, 0.1, 0.9, 0.0, True, 5, *optim.QUINTIC, 1e-7)
