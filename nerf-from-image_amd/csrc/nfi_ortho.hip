@@ -47,12 +47,13 @@ struct Args {
   float up_x, up_a, up_q;                 // powers of two
 };
 
-// The launch's arguments: a kernel takes room for 1, 8 or 32 items (3.4 KB of arguments cost 10 us of a launch)
+// The launch's arguments: a kernel takes room for 1, 8 or 32 items (the 4 KB of 32 cost 10 us of a launch)
 template <int N>
 struct Table : Args {
   int first[N];   // the launch's first unit of each item (behind the last: beyond any)
   Item item[N];
 };
+static_assert(sizeof(Table<ITEMS>) <= 4096, "kernel arguments");
 
 typedef _Float16 h4v __attribute__((ext_vector_type(4)));
 
@@ -905,10 +906,12 @@ __device__ __forceinline__ void run_lds(const Args& p, const Item& t, int matrix
   }
 }
 
-// Both: one workgroup for each matrix
-template <int BYTES, int N>
+// Both: one workgroup for each matrix.  Its 16 waves of 128 registers fill a compute unit, whatever LDS it takes
+constexpr int SMALL_BYTES = 155648;
+static_assert(ROWS16_BYTES <= SMALL_BYTES, "rows16 fits");
+template <int N>
 __global__ void __launch_bounds__(SMALL_THREADS) ortho_small(const Table<N> p, int steps) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds[BYTES];
+  __shared__ __attribute__((aligned(16))) unsigned char lds[SMALL_BYTES];
   __shared__ double red[SMALL_WAVES];
   int matrix, unit;
   const int it = locate(p, blockIdx.x, matrix, unit, [](const Item&) { return 1; });
@@ -923,18 +926,14 @@ __global__ void __launch_bounds__(SMALL_THREADS) ortho_small(const Table<N> p, i
 
 // ---- host --------------------------------------------------------------------------------------------------------------
 
-constexpr int SMALL_SIZES[2] = {81920, 155648};   // bytes of LDS: two workgroups for a compute unit, or one
-static_assert(ROWS16_BYTES <= SMALL_SIZES[0], "rows16 fits");
 static inline int ceil_to(int v, int k) { return (v + k - 1) / k * k; }
 static inline int64_t up(int64_t v) { return (v + 255) / 256 * 256; }
 
-// How a matrix runs: -1 as tiles, 0 or 1 in one workgroup of that size
-static int kind_of(const nfi_ortho_item& q) {
+// Does a matrix run in one workgroup (else as tiles)?
+static bool is_small(const nfi_ortho_item& q) {
   const int m = std::min(q.rows, q.cols), n = std::max(q.rows, q.cols);
-  if (m <= 16 && n <= 2048) return 0;
-  if (m <= 16 || m > 64 || n > 65536) return -1;
-  const int need = SmallShape(m, n).bytes();
-  return need <= SMALL_SIZES[0] ? 0 : need <= SMALL_SIZES[1] ? 1 : -1;
+  if (m <= 16) return n <= 2048;
+  return m <= 64 && n <= 65536 && SmallShape(m, n).bytes() <= SMALL_BYTES;
 }
 
 // a table in the smallest size that holds its items
@@ -956,11 +955,10 @@ static unsigned number_units(Table<N>& t, F per) {
   return (unsigned)all;
 }
 template <int N>
-static void launch_small(const Table<ITEMS>& a, int size, int steps, hipStream_t s) {
+static void launch_small(const Table<ITEMS>& a, int steps, hipStream_t s) {
   Table<N> t = smaller<N>(a);
   const unsigned blocks = number_units(t, [](const Item&) { return 1; });
-  if (size == 0) ortho_small<SMALL_SIZES[0], N><<<blocks, SMALL_THREADS, 0, s>>>(t, steps);
-  else ortho_small<SMALL_SIZES[1], N><<<blocks, SMALL_THREADS, 0, s>>>(t, steps);
+  ortho_small<N><<<blocks, SMALL_THREADS, 0, s>>>(t, steps);
 }
 template <int N>
 static void launch_tiles(const Table<ITEMS>& a, int steps, hipStream_t s) {
@@ -989,7 +987,7 @@ constexpr int MOST_SPLIT = 8;
 
 static int64_t item_bytes(const nfi_ortho_item& s) {
   const int m = std::min(s.rows, s.cols), n = std::max(s.rows, s.cols);
-  if (kind_of(s) >= 0) return 0;
+  if (is_small(s)) return 0;
   const int64_t mp = padded_side(m), np = padded_side(n), size = (int64_t)s.rows * s.cols;
   return s.count * (2 * up(mp * np * 4) + 2 * up(mp * mp * 4)) + up(s.count * ((size + NORM_CHUNK - 1) / NORM_CHUNK) * 8);
 }
@@ -1145,32 +1143,20 @@ int32_t nfi_ortho(const nfi_ortho_args* p, void* stream) {
     t.np = ceil_to(t.n, unit);
     return t;
   };
-  // small matrices: in one launch if every compute unit gets one at most, else by size (two workgroups of the smaller
-  // for a unit)
-  int64_t counts[2] = {0, 0};
-  for (int i = 0; i < p->n_items; ++i)
-    if (kind_of(p->items[i]) >= 0) counts[kind_of(p->items[i])] += p->items[i].count;
-  const bool together = counts[0] + counts[1] <= 256 && counts[1] > 0;
-  for (int size = 0; size < 2; ++size) {
-    Table<ITEMS> a;
-    (Args&)a = base;
-    auto flush = [&]() {
-      if (a.items == 1) launch_small<1>(a, size, p->steps, s);
-      else if (a.items > 0 && a.items <= 8) launch_small<8>(a, size, p->steps, s);
-      else if (a.items > 8) launch_small<ITEMS>(a, size, p->steps, s);
-      a.items = 0;
-    };
-    for (int i = 0; i < p->n_items; ++i) {
-      const nfi_ortho_item& q = p->items[i];
-      const int kind = kind_of(q);
-      if (kind < 0 || (together ? 1 : kind) != size) continue;
-      a.item[a.items++] = item(q, 16);
-      if (a.items == ITEMS) flush();
-    }
-    flush();
-  }
   Table<ITEMS> a;
   (Args&)a = base;
+  auto flush_small = [&]() {
+    if (a.items == 1) launch_small<1>(a, p->steps, s);
+    else if (a.items > 0 && a.items <= 8) launch_small<8>(a, p->steps, s);
+    else if (a.items > 8) launch_small<ITEMS>(a, p->steps, s);
+    a.items = 0;
+  };
+  for (int i = 0; i < p->n_items; ++i) {
+    if (!is_small(p->items[i])) continue;
+    a.item[a.items++] = item(p->items[i], 16);
+    if (a.items == ITEMS) flush_small();
+  }
+  flush_small();
   unsigned char* work = (unsigned char*)p->work;
   auto flush = [&]() {
     choose_splits(a.item, a.items, work);   // (behind the last item)
@@ -1182,7 +1168,7 @@ int32_t nfi_ortho(const nfi_ortho_args* p, void* stream) {
   };
   for (int i = 0; i < p->n_items; ++i) {
     const nfi_ortho_item& q = p->items[i];
-    if (kind_of(q) >= 0) continue;
+    if (is_small(q)) continue;
     Item t = item(q, TILE);
     const int64_t sx = up((int64_t)t.mp * t.np * 4) * t.count, sa = up((int64_t)t.mp * t.mp * 4) * t.count;
     t.x = (_Float16*)work;
