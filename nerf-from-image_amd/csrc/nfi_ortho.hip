@@ -936,6 +936,8 @@ static bool is_small(const nfi_ortho_item& q) {
   return m <= 64 && n <= 65536 && SmallShape(m, n).bytes() <= SMALL_BYTES;
 }
 
+constexpr int MOST_SMALL = 1 << 21;   // workgroups of a launch (a launch has fewer than 2^32 threads)
+
 // a table in the smallest size that holds its items
 template <int N>
 static Table<N> smaller(const Table<ITEMS>& t) {
@@ -1151,10 +1153,25 @@ int32_t nfi_ortho(const nfi_ortho_args* p, void* stream) {
     else if (a.items > 8) launch_small<ITEMS>(a, p->steps, s);
     a.items = 0;
   };
+  int64_t held = 0;   // workgroups of the launch
   for (int i = 0; i < p->n_items; ++i) {
-    if (!is_small(p->items[i])) continue;
-    a.item[a.items++] = item(p->items[i], 16);
-    if (a.items == ITEMS) flush_small();
+    const nfi_ortho_item& q = p->items[i];
+    if (!is_small(q)) continue;
+    const int64_t size = (int64_t)q.rows * q.cols;
+    for (int done = 0; done < q.count;) {   // (a run of more matrices than a launch takes leaves in pieces)
+      Item t = item(q, 16);
+      t.g = (const unsigned char*)q.g + done * size * type_bytes(p->g_type);
+      if (t.mom) t.mom += done * size;
+      t.w = (unsigned char*)q.w + done * size * type_bytes(p->w_type);
+      t.count = (int)std::min<int64_t>(q.count - done, MOST_SMALL - held);
+      done += t.count;
+      held += t.count;
+      a.item[a.items++] = t;
+      if (a.items == ITEMS || held == MOST_SMALL) {
+        flush_small();
+        held = 0;
+      }
+    }
   }
   flush_small();
   unsigned char* work = (unsigned char*)p->work;

@@ -335,3 +335,23 @@ def test_the_first_step_is_refused_in_a_capture():
         torch.cuda.synchronize()
         other.step()
         assert torch.equal(p, q)
+
+
+def test_more_small_matrices_than_a_launch_takes():
+    """4,300,000 of 2 x 3 (a launch has fewer than 2^32 threads, 2^22 workgroups of 1024): each as in a call of its own."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    n = 4300000
+    u = torch.randn((n, 2, 3), device=DEV, generator=g)
+    out = optim.orthogonalize(u)
+    for at in (0, (1 << 21) - 3, (1 << 21), (1 << 22) - 5, (1 << 22), n - 9):
+        assert torch.equal(out[at:at + 9], optim.orthogonalize(u[at:at + 9].clone())), at
+    ref = formula(u.double())
+    # (each matrix's own bound, see above: |X|_F is at most sqrt(2))
+    assert float((out.double() - ref).norm(dim=(1, 2)).max()) <= 341 * 8 * 2.0 ** -22 * 2 ** 0.5
+    p = torch.nn.Parameter(torch.ones((n, 2, 3), device=DEV, dtype=torch.bfloat16))
+    p.grad = u.bfloat16()
+    opt = optim.Muon([p], lr=0.5, momentum=0.0, batched=True)
+    opt.step()
+    o = optim.orthogonalize(p.grad)
+    assert float((p.detach().float() - (1 - 0.5 * o.float())).abs().max()) <= 2.0 ** -7 * 2
+    assert torch.equal(opt.state[p]['momentum_buffer'], p.grad.float())
