@@ -309,7 +309,8 @@ std::vector<Tensor> residual_norm(const Tensor& h, const Maybe& residual_, const
   const int64_t d = h.size(-1), rows = h.numel() / d;
   if (gate.defined()) {
     if (gate.dim() == 1) gate = gate.unsqueeze(0);
-    if (first && first->dim() == 2 && gate.size(0) != first->size(0)) gate = gate.expand({first->size(0), d});
+    // (in 32 bits: the groups' gradients of one gate are added up unrounded)
+    if (first && first->dim() == 2 && gate.size(0) != first->size(0)) gate = gate.to(torch::kFloat).expand({first->size(0), d});
     gate = gate.contiguous();
   }
   bool train = false;

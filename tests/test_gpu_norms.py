@@ -346,3 +346,31 @@ def test_captured_and_replayed():
         want = step()
         for a, b in zip(held, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+def test_one_gate_beside_groups_of_parameters(dtype):
+    """A [D] or [1, D] gate for rows whose norms have parameters of groups: its gradient is summed over all of them in 32 bits
+    and rounded once, where gradients of opposite signs cancel too."""
+    g = torch.Generator(device=DEV).manual_seed(12)
+    rows, groups, width = 512, 64, 40
+
+    def rnd(*shape, shift=0.0, scale=0.5):
+        return (torch.randn(shape, device=DEV, generator=g) * scale + shift).to(dtype)
+    h, gate, weight, bias = rnd(rows, width), rnd(width, shift=1).requires_grad_(), rnd(groups, width, scale=0.1), rnd(groups, width, shift=2)
+    gx = rnd(rows, width, shift=1, scale=0.1)
+    gx[rows // groups * (groups // 2):] *= -1      # (half of the groups against the other half)
+    p64 = {'h': h.double(), 'residual': None, 'gate': gate.detach().double().expand(groups, width),
+           'weight': weight.double().repeat_interleave(rows // groups, 0), 'bias': bias.double().repeat_interleave(rows // groups, 0),
+           'next_weight': None, 'next_bias': None}
+    v, _ = formula({**p64, 'gate': None}, 'layer', None, 0.2, 1.0)
+    rx, _ = formula(p64, 'layer', None, 0.2, 1.0)
+    terms = gx.double() * v
+    e = torch.finfo(dtype).eps / 2
+    # each v is off by 64 u of the largest value that enters it (below 8), and sums of rows / groups, 16 and groups terms follow
+    tol = 64 * U * 8 * gx.double().abs().sum(0) + (rows // groups + 16 + groups) * U * terms.abs().sum(0) + e * (1 + 2 ** -8) * terms.sum(0).abs()
+    for shape in ((width,), (1, width)):
+        x = norms.residual_norm(h, None, gate.view(shape), weight, bias, slope=0.2)
+        near(x.detach(), rx, dtype, 8)
+        got, = torch.autograd.grad(x, [gate], gx)
+        assert float(((got.double() - terms.sum(0)).abs() / tol).max()) <= 1
