@@ -242,3 +242,42 @@ def test_infinities_and_large_values_are_those_of_the_formula(k, n, dtype):
     assert torch.equal(got[0][rest], clean[0][rest])
     rest = [i for i in range(300) if i != 11]
     assert torch.equal(got[1][rest], clean[1][rest])
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('sizes,before,behind', [([1] * 200, 1, 1), ([129] * 9, 129, 1), ([1, 127, 128, 129, 0, 1], 1, 127), ([2] * 62, 0, 3),
+                                                 ([0] * 70 + [1], 0, 0), ([0] * 63 + [5] + [0] * 64 + [200], 257, 129)])
+def test_every_row_of_any_division_is_written(sizes, before, behind, dtype):
+    """As many row tiles as a division can need, each with few rows: no row of y or gx keeps what its memory held."""
+    x, w, offsets, b, gy, off = make(sizes, 40, 72, dtype, len(sizes), True, before, behind)
+    for shape in (gy.shape, x.shape):
+        junk = [torch.full(shape, float('nan'), device=DEV, dtype=dtype) for _ in range(3)]
+        del junk
+    y = grouped.grouped_linear(x, w, offsets, b)
+    got = [y.detach()] + list(torch.autograd.grad(y, [x, w, b], gy))
+    for a, ref in zip(got, reference(x, w, off, b, gy)):
+        near(a, ref, dtype)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('sizes,k,n', [([3, 0, 2], 16, 24), ([700, 1300], 48, 40), ([40000], 8, 130), ([5000, 0, 3000, 100], 64, 64), ([300] * 30, 33, 257)])
+def test_each_gradient_alone(sizes, k, n, dtype):
+    """The gradient of one argument without the others' (the bias has a kernel of its own then, its rows split where they are
+    many): those of x and the weight are the same bits as together, the bias's within its sum's rounding."""
+    x, w, offsets, b, gy, off = make(sizes, k, n, dtype, k + n, True, 2, 5)
+    y = grouped.grouped_linear(x, w, offsets, b)
+    refs = reference(x, w, off, b, gy)[1:]
+    together = torch.autograd.grad(y, [x, w, b], gy, retain_graph=True)
+    for i, leaf in enumerate((x, w, b)):
+        alone, = torch.autograd.grad(y, [leaf], gy, retain_graph=True)
+        near(alone, refs[i], dtype)
+        again, = torch.autograd.grad(y, [leaf], gy, retain_graph=True)
+        assert torch.equal(alone, again) and (leaf is b or torch.equal(alone, together[i]))
+    pair = torch.autograd.grad(y, [x, b], gy)
+    near(pair[1], refs[2], dtype)
+    assert torch.equal(pair[0], together[0])
+    # without a gradient of x and the weight there is none to make
+    with torch.no_grad():
+        xd, wd = x.clone(), w.clone()
+    alone, = torch.autograd.grad(grouped.grouped_linear(xd, wd, offsets, b), [b], gy)
+    near(alone, refs[2], dtype)

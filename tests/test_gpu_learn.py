@@ -296,3 +296,125 @@ def test_halves_refuse_what_they_cannot_take():
                     (lambda: ops.grouped_linear_bwd(gy, x, w, off[:2], [True] * 3), 'offsets')):
         with pytest.raises((RuntimeError, ValueError), match=word):
             f()
+
+
+def behind(need, held=0xa5):
+    """A work buffer of `need` bytes at the head of a longer one, and a function that says whether what follows is untouched."""
+    buf = torch.full((max(need, 0) + (1 << 20),), 0xa5, device=DEV, dtype=torch.uint8)
+    buf[:max(need, 0)] = held
+    return buf.data_ptr(), lambda: bool((buf[max(need, 0):] == 0xa5).all())
+
+
+@pytest.mark.parametrize('width', [24, 64, 512, 513, 1000, 1024, 1025, 2048, 2049, 4100, 8192])
+@pytest.mark.parametrize('groups,affine', [(0, 0), (7, 0), (7, 1), (400, 1), (800, 0), (1600, 1)])
+def test_norm_workspace_is_enough(width, groups, affine):
+    """Every layout's backward through the C interface, its work buffer of the size that it is told: nothing behind it is
+    written, and the parameters' gradients do not depend on what it held."""
+    import ctypes
+    from nfi import _lib
+    lib = _lib.load()
+    rows = 2800 if groups == 7 else 1600
+    t = {k: torch.randn((rows, width), device=DEV) for k in ('h', 'residual', 'gx', 'gy')}
+    t.update(stats=torch.rand((rows, 4), device=DEV) + 0.5, dh=torch.empty((rows, width), device=DEV), dresidual=torch.empty((rows, width), device=DEV))
+    per = (groups, width) if affine else (width,)
+    for k in ('weight', 'bias', 'next_weight', 'next_bias'):
+        t[k], t['d' + k] = torch.randn(per, device=DEV), torch.empty(per, device=DEV)
+    if groups:
+        t['gate'], t['dgate'] = torch.randn((groups, width), device=DEV), torch.empty((groups, width), device=DEV)
+    a = _lib.NfiResnormArgs()
+    for k, v in t.items():
+        setattr(a, k, v.data_ptr())
+    a.rows, a.groups, a.width, a.norm, a.next_norm, a.affine_groups = rows, groups, width, 1, 2, affine
+    a.slope, a.scale, a.eps = 0.2, 0.7, 1e-5
+    need = lib.nfi_resnorm_work_bytes(rows, groups, affine, width)
+    kept = []
+    for held in (0, 0xff):
+        a.work, untouched = behind(need, held)
+        assert lib.nfi_resnorm_backward(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == 0, lib.nfi_last_error()
+        torch.cuda.synchronize()
+        assert untouched()
+        kept.append([t[k].clone() for k in t if k[0] == 'd'])
+    assert all(torch.equal(p, q) for p, q in zip(*kept))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('rows,groups,k,n,need', [(700, 3, 33, 65, 'xwb'), (5000, 1, 64, 64, 'xwb'), (5000, 2, 129, 40, 'xw'), (40000, 1, 7, 130, 'b'),
+                                                  (3000, 2, 200, 136, 'wb'), (90, 20, 31, 33, 'x')])
+def test_grouped_workspace_is_enough(rows, groups, k, n, need, dtype):
+    import ctypes
+    from nfi import _lib
+    lib = _lib.load()
+    x, w, gy = (torch.randn(s, device=DEV).to(dtype) for s in ((rows, k), (groups, n, k), (rows, n)))
+    bias = torch.randn((groups, n), device=DEV).to(dtype)
+    off = torch.linspace(0, rows, groups + 1, device=DEV).to(torch.int32)
+    y, gx, gw, gb = (torch.empty_like(v) for v in (gy, x, w, bias))
+    a = _lib.NfiGroupedArgs()
+    a.x, a.w, a.bias, a.offsets, a.y = (v.data_ptr() for v in (x, w, bias, off, y))
+    a.rows, a.groups, a.in_width, a.out_width, a.dtype = rows, groups, k, n, 0 if dtype == torch.float32 else 1
+    stream = torch.cuda.current_stream().cuda_stream
+    for size, call in ((lib.nfi_grouped_forward_work_bytes, lib.nfi_grouped_forward), (lib.nfi_grouped_backward_work_bytes, lib.nfi_grouped_backward)):
+        if call is lib.nfi_grouped_backward:
+            a.gy = gy.data_ptr()
+            a.gx, a.gw, a.gb = (v.data_ptr() if c in need else None for c, v in zip('xwb', (gx, gw, gb)))
+        a.work_bytes = size(ctypes.byref(a))
+        a.work, untouched = behind(a.work_bytes)
+        assert call(ctypes.byref(a), stream) == 0, lib.nfi_last_error()
+        torch.cuda.synchronize()
+        assert untouched()
+
+
+def test_ortho_workspace_is_enough():
+    import ctypes
+    from nfi import _lib
+    lib = _lib.load()
+    shapes = [(200, 300, 1), (65, 1300, 3), (640, 70, 2), (15, 2049, 1), (64, 64, 5)] + [(70 + i, 90, 1) for i in range(40)] + [(300, 300, 2)]
+    held = [torch.randn((c, r, n), device=DEV) for r, n, c in shapes]
+    out = [torch.empty_like(v) for v in held]
+    items = (_lib.NfiOrthoItem * len(shapes))(*[_lib.NfiOrthoItem(v.data_ptr(), None, o.data_ptr(), r, n, c, 1.0)
+                                                for v, o, (r, n, c) in zip(held, out, shapes)])
+    a = _lib.NfiOrthoArgs()
+    a.items, a.n_items, a.steps, a.eps = ctypes.cast(items, ctypes.POINTER(_lib.NfiOrthoItem)), len(shapes), 5, 1e-7
+    a.a, a.b, a.c = optim.QUINTIC
+    a.work_bytes = lib.nfi_ortho_work_bytes(items, len(shapes))
+    results = []
+    for fill in (0, 0xff):
+        a.work, untouched = behind(a.work_bytes, fill)
+        assert lib.nfi_ortho(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == 0, lib.nfi_last_error()
+        torch.cuda.synchronize()
+        assert untouched()
+        results.append([o.clone() for o in out])
+    assert all(torch.equal(p, q) for p, q in zip(*results))
+    for v, o in zip(held, out):
+        alone = optim.orthogonalize(v)
+        assert float((alone.double() - o.double()).norm()) <= 2 * 341 * 8 * 2.0 ** -22 * float(alone.double().norm())
+
+
+def test_a_captured_bank():
+    """Forward and backward captured, replayed with other rays and other images' mappers between eager calls."""
+    b = bank(3)
+    v = torch.nn.functional.normalize(torch.randn((4, 50, 3), device=DEV), dim=-1).requires_grad_()
+    image, g = torch.tensor([1, 0, 2, 1], device=DEV), torch.randn((4, 50, 32), device=DEV)
+    params = [p for k, p in b.named_parameters() if 'output' not in k]
+
+    def step():
+        x = b(v, image)
+        return [x.detach(), *torch.autograd.grad(x, [v] + params, g)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for which in ([1, 0, 2, 1], [2, 2, 0, 0], [0, 0, 0, 0], [5, 1, -1, 2], [0, 1, 2, 2]):
+        with torch.no_grad():
+            v.copy_(torch.nn.functional.normalize(torch.randn_like(v), dim=-1))
+            image.copy_(torch.tensor(which))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(held, step())), which
+        torch.cuda.synchronize()

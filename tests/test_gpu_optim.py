@@ -355,3 +355,27 @@ def test_more_small_matrices_than_a_launch_takes():
     o = optim.orthogonalize(p.grad)
     assert float((p.detach().float() - (1 - 0.5 * o.float())).abs().max()) <= 2.0 ** -7 * 2
     assert torch.equal(opt.state[p]['momentum_buffer'], p.grad.float())
+
+
+@pytest.mark.parametrize('count', [9, 32, 33, 70])
+def test_many_tiled_matrices(count):
+    """More matrices that run as tiles than one, eight or thirty-two of a launch: each launch has the work buffer to itself, and the
+    next begins behind it."""
+    g = torch.Generator(device=DEV).manual_seed(count)
+    shapes = [(65 + 7 * (i % 11), 66 + 31 * (i % 7)) if i % 3 else (260 - 3 * (i % 5), 70 + i) for i in range(count)]
+    params = [torch.nn.Parameter(torch.randn(s, device=DEV, generator=g)) for s in shapes]
+    for p in params:
+        p.grad = torch.randn(p.shape, device=DEV, generator=g)
+    before = [p.detach().clone() for p in params]
+    opt = optim.Muon(params, lr=0.05, momentum=0.9, weight_decay=0.1)
+    opt.step()
+    for p, old in zip(params, before):
+        w, m = reference_step(old, p.grad, torch.zeros_like(old), 0.05, 0.9, 0.1, True)
+        tall = math.sqrt(max(1.0, p.shape[0] / p.shape[1]))
+        tol = 0.05 * tall * 341 * 8 * 2.0 ** -22 * 1.2 * math.sqrt(min(p.shape)) + 4 * 2.0 ** -24 * float(w.norm())
+        assert float((p.detach().double() - w).norm()) <= tol, tuple(p.shape)
+        # each alone, in a call of its own, is the same update within 32 bits (its products may be divided otherwise)
+        alone = torch.nn.Parameter(old.clone())
+        alone.grad = p.grad
+        optim.Muon([alone], lr=0.05, momentum=0.9, weight_decay=0.1).step()
+        assert float((alone.detach().double() - p.detach().double()).norm()) <= 2 * tol

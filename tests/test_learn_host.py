@@ -379,3 +379,18 @@ def test_traced_steps(fake):
 def test_no_tensors_are_no_step():
     from nfi import torch_ops
     torch_ops.op('muon_step')([], [], [], False, 0.1, 0.9, 0.0, True, 5, *optim.QUINTIC, 1e-7)
+
+
+@pytest.mark.parametrize('affine', [0, 1])
+@pytest.mark.parametrize('width,workgroups', [(24, 512), (512, 512), (513, 768), (1024, 768), (1025, 512), (2048, 512), (2049, 256), (8192, 256)])
+def test_resnorm_work_holds_every_workgroup_of_each_width(width, workgroups, affine):
+    """The plan (restated) with the workgroups that a width takes, for every number of rows one may hold."""
+    lib = _lib.load()
+    for rows, groups in [(1, 0), (1, 1), (7, 7), (10 ** 6, 0), (10 ** 6, 2), (4096, 512), (4096, 2048), (511 * 3, 511), (769 * 5, 769), (255 * 9, 255),
+                         (257 * 2, 257), (768, 768), (3 * 10 ** 5, 300)]:
+        for slots in (1, 4, 8, 16, 32):
+            g = groups if groups and (groups < rows or affine) else 1
+            splits = min(max(1, workgroups // g), -(-(rows // g) // slots))
+            segments = g * splits
+            per = 1 if splits > 1 else -(-segments // workgroups)
+            assert lib.nfi_resnorm_work_bytes(rows, groups, affine, width) >= -(-segments // per) * 5 * width * 4, (rows, groups, slots)
