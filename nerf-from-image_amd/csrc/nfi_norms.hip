@@ -597,6 +597,7 @@ int32_t nfi_resnorm_backward(const nfi_resnorm_args* a, void* stream) {
   NFI_REQUIRE(a->stats && a->work, "resnorm_backward: null statistics or work buffer");
   NFI_REQUIRE(a->gx || a->gy, "resnorm_backward: no gradient");
   NFI_REQUIRE(!a->gy || a->next_norm != NFI_NORM_NONE, "resnorm_backward: gy without a next norm");
+  NFI_REQUIRE(!a->dgate || a->gate, "resnorm_backward: dgate without a gate");
   run(*a, true, (hipStream_t)stream);
   NFI_CHECK_LAUNCH("resnorm_backward");
   return NFI_OK;

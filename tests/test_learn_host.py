@@ -394,3 +394,13 @@ def test_resnorm_work_holds_every_workgroup_of_each_width(width, workgroups, aff
             segments = g * splits
             per = 1 if splits > 1 else -(-segments // workgroups)
             assert lib.nfi_resnorm_work_bytes(rows, groups, affine, width) >= -(-segments // per) * 5 * width * 4, (rows, groups, slots)
+
+
+@pytest.mark.parametrize('groups', [0, 2, 4])
+def test_resnorm_backward_refuses_a_gradient_of_no_gate(groups):
+    lib = _lib.load()
+    one = ctypes.c_void_p(16)
+    a = _lib.NfiResnormArgs()
+    a.h = a.x = a.stats = a.work = a.gx = a.dh = a.dgate = one
+    a.rows, a.width, a.groups, a.norm, a.eps = 4, 8, groups, 1, 1e-5
+    assert lib.nfi_resnorm_backward(ctypes.byref(a), None) == -1 and b'without a gate' in lib.nfi_last_error()
