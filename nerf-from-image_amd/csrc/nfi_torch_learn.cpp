@@ -12,6 +12,7 @@
 //
 // The autograd functions call the halves' functions themselves; where a tensor has no memory, or a dispatch mode looks on (meta and
 // fake tensors, tracing), they call them through the dispatcher, whose Meta kernels give shapes and touch no pointer.
+#include <algorithm>
 #include <array>
 #include <cmath>
 #include <vector>
@@ -565,6 +566,15 @@ void muon_step(at::TensorList params, at::TensorList grads, at::TensorList momen
                              (float)std::sqrt(std::max(1.0, (double)rows / (double)cols))});
     lots[l].of.push_back(i);
   }
+  // what is updated lies apart: all matrices are stepped at a time
+  std::vector<std::pair<const char*, const char*>> spans;
+  spans.reserve(2 * n);
+  for (const Lot& l : lots)
+    for (size_t i : l.of)
+      for (const Tensor* t : {&params[i], &momenta[i]}) spans.emplace_back((const char*)t->data_ptr(), (const char*)t->data_ptr() + t->nbytes());
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    TORCH_CHECK_VALUE(spans[i].first >= spans[i - 1].second, what, ": parameters and momenta that share memory (each is stepped on its own)");
   for (Lot& l : lots) {
     const Tensor& p = params[l.of[0]];
     const c10::DeviceGuard guard(p.device());

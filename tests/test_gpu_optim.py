@@ -379,3 +379,22 @@ def test_many_tiled_matrices(count):
         alone.grad = p.grad
         optim.Muon([alone], lr=0.05, momentum=0.9, weight_decay=0.1).step()
         assert float((alone.detach().double() - p.detach().double()).norm()) <= 2 * tol
+
+
+def test_parameters_that_share_memory_are_refused():
+    """The same tensor twice, a view beside its base, a momentum that two share: their steps would run at a time."""
+    w, g = torch.ones((12, 8), device=DEV), torch.randn((12, 8), device=DEV)
+    m, m2 = torch.zeros_like(w), torch.zeros_like(w)
+    for params, grads, momenta in (([w, w], [g, g], [m, m2]), ([w, w[4:9]], [g, g[4:9]], [m, m2[4:9]]), ([w, w[:1]], [g, g[:1]], [m, m2[:1]]),
+                                   ([w, w.clone()], [g, g], [m, m]), ([w], [g], [w])):
+        with pytest.raises(ValueError, match='share memory'):
+            step_op(params, grads, momenta)
+    a = torch.nn.Parameter(w)
+    b = torch.nn.Parameter(w[2:5])
+    a.grad, b.grad = g, g[2:5]
+    with pytest.raises(ValueError, match='share memory'):
+        optim.Muon([a, b]).step()
+    assert torch.equal(w, torch.ones_like(w)) and float(m.abs().max()) == 0 and float(m2.abs().max()) == 0
+    # neighbours in one buffer, and one gradient for two, are separate parameters
+    step_op([w[:6], w[6:]], [g[:6], g[:6]], [m[:6], m[6:]])
+    assert torch.equal(w[:6], w[6:]) and torch.equal(m[:6], g[:6])
