@@ -97,7 +97,9 @@ typedef struct nfi_ortho_item {
 /* Every matrix of every item:  M <- momentum M + G (where it has one);  U = G + momentum M with nesterov,
  * else M (G without M);  X = U / max(|U|_F, eps);  `steps` times X <- (a + b X X^T + c (X X^T)^2) X, for
  * rows <= cols (else of the transposed matrix);  then w = X, or with update w <- (1 - decay) w - step
- * scale X.  Products are held to 32-bit accuracy for every type, and the result is rounded once.  `items` is
+ * scale X.  For every type products are of 32-bit values (up to 16 rows) or of pairs of halves, which keep 22 bits of values down to
+ * 2^-17 of the largest that an iterate can hold and 2^-40 of that below (|U| far below eps), with 32-bit sums; the result is
+ * rounded once.  `items` is
  * host memory, read during the call.  A polynomial under which singular values leave [0, 64) is refused.
  * work: nfi_ortho_work_bytes (-1 for items that nfi_ortho refuses by their sizes), or NULL where that is 0. */
 typedef struct nfi_ortho_args {

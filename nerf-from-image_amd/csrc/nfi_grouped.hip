@@ -6,13 +6,13 @@
 // 2 T K N operations each way and product; the offsets stay on the device: a launch covers every tile that
 // any division into groups could need, and a workgroup finds its group by a scan of the tile counts.
 //
-// 16 experts, 32,749 rows of 1024 -> 4096 in bf16: forward 365 us, dx 345, dw 361 (275 GF each: 750 .. 800 TF).  Per step
+// 16 experts, 32,749 rows of 1024 -> 4096 in bf16: forward 358 us, dx 347, dw 355 (275 GF each: 770 .. 790 TF).  Per step
 // a compute unit's LDS takes 32 KB of loads and gives 64 KB of fragments, 768 clocks against 512 of its matrix cores, which
-// bounds these tiles: without the products the forward takes 85 % of its time, without the loads 70 %.  Tiles of 256 x 256
-// on eight waves read less but hide neither their first loads nor their last stores, and spill: 371 us against 400 (both
-// before tiles were turned in LDS, 365 since), the other directions slower: not taken.  Rows padded by 128 or 384 bytes and steps that start at another place in each tile changed nothing.
-// 16,411 rows of 512 -> 512, 32-bit as three bf16 parts: 74 us each (116 TF of 192 that six products leave), bound by
-// cutting the parts, 5 operations for each value and part.  Few rows are bound by reading the weights (48 rows, 67 MB: 14 us).
+// bounds these tiles: the matrix cores are busy 0.39 .. 0.42 of the cycles (at 1.9 GHz), the waves ready but not issued half of
+// theirs.  Tiles of 256 x 256 on eight waves read less but spill, and hide neither their first loads nor their last stores: not
+// taken.  16,411 rows of 512 -> 512, 32-bit as three bf16 parts: 73, 74 and 64 .. 76 us (116 TF of 192 that six products
+// leave), bound by cutting the parts, 5 operations for each value and part.  Few rows are bound by reading the weights (48
+// rows, 67 MB: 14 us).
 #include <algorithm>
 
 #include "nfi_mm.h"

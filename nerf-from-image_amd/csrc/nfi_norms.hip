@@ -17,8 +17,9 @@
 // take a workgroup, in the backward of twice or four times as many lanes as in the forward (dispatch).  The parameter
 // gradients stay in registers over a workgroup's rows and leave as one partial per workgroup, summed by a second launch in a
 // fixed order.  16,384 rows of 1024 bf16, both norms, eight gates: forward 31 us (134 MB, 4.3 TB/s), backward 57 + 5 us
-// (201 MB, 3.5 TB/s: the vector pipes are busy two thirds of it, with 2 x 2 sums over four waves and 50 operations an
-// element).  131,072 rows of 64 32-bit values: 17 us (101 MB).
+// (201 MB, 3.5 TB/s: vector instructions issue in 0.55 of the cycles, with 2 x 2 sums over four waves and 50 operations an
+// element, and its two waves a SIMD wait in 0.59 of theirs).  131,072 rows of 64 32-bit values: 17 us (101 MB), and with their
+// gradients 50 (269 MB), or 52 where each of 8 groups has parameters of its own.
 #include <algorithm>
 
 #include "nfi_learn.h"

@@ -7,16 +7,18 @@
 // U = G + beta M, M <- beta M + G (or U = M) before, and W <- (1 - decay) W - step X behind.  Per step m^2 n + m^3 + 2 m^2 n
 // operations (A and A A are symmetric: half of each product is computed and mirrored).
 //
-// Small singular values grow by up to `a` each step, and rounding errors with them, so every product is held to 32-bit
-// accuracy whatever the type of the weights: operands are pairs of halves hi = f16(v 2^s), lo = f16(v 2^s - hi), three
+// Small singular values grow by up to `a` each step, and rounding errors with them, so products are near 32-bit ones
+// whatever the type of the weights: operands are pairs of halves hi = f16(v 2^s), lo = f16(v 2^s - hi), three
 // products hi hi + hi lo + lo hi on the 16-bit matrix cores into 32-bit sums (lo lo is below 2^-22 of the product).  All
 // operands are bounded (singular values start at <= 1 and the polynomial is known), so the scales are constants of the
-// call.  Memory holds 32 hi and 32 lo halves of 32 neighbouring columns together: 128 bytes that are one step of a tile.
+// call; a value keeps 22 bits down to 2^-17 of its bound, and 2^-40 of the bound below (a lo half is subnormal there).  Two of
+// 2048 x 2048: 2.4e-6 of the norm off after five steps, the formula in 32-bit products 3.8e-6.  Memory holds 32 hi and 32 lo halves of 32 neighbouring columns together: 128 bytes that are one step of a tile.
 //
 // Matrices of up to 64 rows that fit into LDS run whole in one workgroup each; the others run as tiles of 128 x 128, all
-// matrices of the call in each launch: their grid holds one tile after the other.
+// matrices of the call in each launch: their grid holds one tile after the other.  Sides are padded to 128, and the padding is
+// computed (64 x 576 takes what 128 x 1152 does, 180 us).
 //
-// Two of 2048 x 2048: A 77 us, Q 83, X' 98 a step (of 3 products: X' at 1050 TF, as fast as a large f16 product of a library;
+// Two of 2048 x 2048: A 76 us, Q 82, X' 96 a step (of 3 products: X' at 1080 TF, as fast as a large f16 product of a library;
 // A and Q have 272 tiles for 256 compute units, one each, where two hide each other's waits).  A generator's 26 matrices up to
 // 512 x 4608: 56 + 12 (A in pieces, joined), 25, 92 us a step, momentum and norm 61 (316 MB at 5.2 TB/s), the start 80.
 #include <algorithm>

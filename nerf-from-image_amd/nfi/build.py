@@ -14,8 +14,8 @@ SOURCES = ['nfi_rays.hip', 'nfi_render.hip', 'nfi_producer.hip', 'nfi_conv.hip',
            'nfi_norms.hip', 'nfi_grouped.hip', 'nfi_ortho.hip']
 HEADERS = ['nfi_common.h', 'nfi_host.h', 'nfi_learn.h', 'nfi_mm.h']
 # -packed-fp32-ops: no v_pk_add / mul / fma_f32 in the build.  Some of their forms have given wrong results
-# on this hardware now and then; measured cost on the renderer 1 % (p3d_car B = 8 step 5.85 -> 5.91 ms, within
-# two runs' spread), none on the inversion step.  (hipcc's host pass warns that it does not know the feature.)
+# on this hardware now and then; measured cost on the renderer 2 % (p3d_car B = 8 step 5.88 -> 5.97 ms), none
+# on the inversion step.  (hipcc's host pass warns that it does not know the feature.)
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-shared', '-munsafe-fp-atomics',
          '-Wall', '-Wno-unused-result', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 

@@ -44,8 +44,9 @@ def _check(what, steps, coefficients, eps):
 @torch.no_grad()
 def orthogonalize(u: torch.Tensor, steps: int = 5, coefficients: Sequence[float] = QUINTIC, eps: float = 1e-7) -> torch.Tensor:
     """u [..., m, n] (float32, bfloat16 or float16) with each matrix's singular values brought near 1: X = u / max(|u|_F,
-    eps), then `steps` times X <- (a + b X X^T + c (X X^T)^2) X, (a, b, c) = `coefficients`.  Products are held to 32-bit
-    accuracy whatever u's type; the result is rounded once.  Not differentiable."""
+    eps), then `steps` times X <- (a + b X X^T + c (X X^T)^2) X, (a, b, c) = `coefficients`.  Products keep 22 bits or
+    more of their operands whatever u's type (fewer of values below 2^-17: |u|_F far below eps), sums 32; the result is rounded
+    once.  Not differentiable."""
     _check('orthogonalize', steps, coefficients, eps)
     return _op('orthogonalize')(u, int(steps), *coefficients, eps)
 
