@@ -14,7 +14,8 @@
 //
 // 32-bit values meet as three bf16 ones each, v = h + m + l (24 bits in 8 + 8 + 8, exactly), in six products l h + h l + m m +
 // m h + h m + h h on the bf16 matrix cores: 96 clocks of them for 32 contracted values against 256 of
-// v_mfma_f32_16x16x4_f32, and what is left out is at most 2^-24 of a product.  An infinity, or a value that bf16 rounds to
+// v_mfma_f32_16x16x4_f32, and what is left out is at most 2^-24 of a product (a value below
+// 2^-110 keeps fewer bits: its parts' last step is 2^-133, bf16's smallest).  An infinity, or a value that bf16 rounds to
 // one, has parts that are no numbers: sums that do not come out finite are taken again in 32-bit products (any_wave).
 #pragma once
 #include "nfi_learn.h"

@@ -25,7 +25,7 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     group holds give zeros.  offsets [groups + 1] int32 or int64 on the device, not decreasing (it is not read on the host:
     values outside [0, rows] count as the nearest end, and decreasing ones give wrong rows, never a wrong access).
 
-    Sums are held in 32 bits and rounded once; what is not finite gives what such a sum gives, in its own rows and columns.  Gradients reach x, weight and bias, summed in a fixed order (no double
+    Sums are held in 32 bits and rounded once (32-bit values to 2^-24 of themselves, and 2^-133); what is not finite gives what such a sum gives, in its own rows and columns.  Gradients reach x, weight and bias, summed in a fixed order (no double
     backward); an empty group's weight and bias get zeros."""
     global _op
     if _op is None:

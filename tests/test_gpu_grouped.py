@@ -281,3 +281,23 @@ def test_each_gradient_alone(sizes, k, n, dtype):
         xd, wd = x.clone(), w.clone()
     alone, = torch.autograd.grad(grouped.grouped_linear(xd, wd, offsets, b), [b], gy)
     near(alone, refs[2], dtype)
+
+
+@pytest.mark.parametrize('ex,ew', [(-100, 90), (-110, 100), (-120, 100), (-126, 110), (90, -126)])
+def test_values_next_to_the_smallest(ex, ew):
+    """32-bit values are three 16-bit parts with bf16's range, whose smallest step is 2^-133: below 2^-110 that is what a value is
+    held to, beside its own 24 bits (half a step of each operand, with the other's magnitude)."""
+    x, w, offsets, b, gy, off = make([70, 30], 96, 40, torch.float32, 9, False)
+    with torch.no_grad():
+        x.mul_(2.0 ** (ex / 2)).mul_(2.0 ** (ex / 2))
+        w.mul_(2.0 ** (ew / 2)).mul_(2.0 ** (ew / 2))
+    y = grouped.grouped_linear(x, w, offsets)
+    got = [y.detach()] + list(torch.autograd.grad(y, [x, w], gy))
+    step = 2.0 ** -133
+    ones = lambda t: torch.full_like(t.detach(), step, dtype=torch.float64)
+    for i, (a, ref) in enumerate(zip(got, reference(x, w, off, None, gy))):
+        value, mags, length = ref
+        held = {'x': reference(ones(x), w, off, None, gy), 'w': reference(x, ones(w), off, None, gy), 'gy': reference(x, w, off, None, ones(gy))}
+        lost = sum(held[k][i][1] for k in (('x', 'w'), ('gy', 'w'), ('gy', 'x'))[i])   # (its two factors)
+        tol = (length + 2) * U * mags + lost + torch.finfo(torch.float32).smallest_normal
+        assert float(((a.double() - value).abs() / tol).max()) <= 1, i
