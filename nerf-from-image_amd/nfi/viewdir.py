@@ -78,6 +78,7 @@ class ViewDirectionMapperBank(torch.nn.Module):
         self.mappers = torch.nn.ModuleList(mappers)
         if len(self.mappers) == 0:
             raise ValueError('ViewDirectionMapperBank: no mappers')
+        self.register_buffer('ends', torch.arange(len(self.mappers) + 1, device=self.mappers[0].fc0.weight.device), persistent=False)
         first = self._form(self.mappers[0])
         for i, m in enumerate(self.mappers):
             if self._form(m) != first:
@@ -108,7 +109,7 @@ class ViewDirectionMapperBank(torch.nn.Module):
 
     def _norm(self, name, h, image, shortcut=None):
         layers = [getattr(m, name) for m in self.mappers]
-        w, b = (torch.stack([getattr(n, k) for n in layers])[image] for k in ('weight', 'bias'))
+        w, b = torch.stack([getattr(n, k) for k in ('weight', 'bias') for n in layers]).view(2, len(layers), -1)[:, image].unbind()
         return residual_norm(h, shortcut, None, w, b, slope=0.2, scale=1.0 if shortcut is None else math.sqrt(2) / 2,
                              eps=layers[0].eps)
 
@@ -122,8 +123,7 @@ class ViewDirectionMapperBank(torch.nn.Module):
             return viewdir_trunk(self.mappers[0], viewdir.unsqueeze(-2)).squeeze(-2)
         # the products want a mapper's rows side by side: the images are brought into their mappers' order, and back
         image, order = torch.sort(mapper_of_image, stable=True)
-        ends = torch.arange(len(self.mappers) + 1, device=viewdir.device)
-        offsets = torch.searchsorted(image, ends) * rays
+        offsets = torch.searchsorted(image, self.ends.to(image.device)) * rays
         image = image.clamp(0, len(self.mappers) - 1)   # (the products leave such images' rows out)
         x = F.leaky_relu(self._linear('fc0', viewdir.index_select(0, order).reshape(images * rays, 3), offsets), 0.2)
         for a, b in ((1, 2), (3, 4)):
@@ -131,4 +131,4 @@ class ViewDirectionMapperBank(torch.nn.Module):
             x = self._norm(f'norm{b}', self._linear(f'fc{b}', h, offsets), image, shortcut=x)
         x = F.leaky_relu(self._linear('fc5', x, offsets), 0.2)
         x = self._linear('fc6', x, offsets).view(images, rays, -1)
-        return x.index_select(0, torch.argsort(order))
+        return torch.empty_like(x).index_copy_(0, order, x)
